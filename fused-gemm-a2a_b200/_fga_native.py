@@ -5,12 +5,31 @@ shared object is missing or a call fails, an exception is raised.
 """
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p, POINTER
 
 _HERE = os.path.dirname(os.path.realpath(__file__))
 LIB_PATH = os.environ.get('FGA_LIB') or os.path.join(_HERE, 'libfga.so')  # FGA_LIB: another build of the same ABI
 
 _lib = None
+
+
+class FgaRotary(ctypes.Structure):
+    """Arguments of fga_rotary_forward / fga_rotary_backward (include/fga.h)."""
+    _fields_ = [('x', c_void_p * 2), ('x_token_stride', c_int64 * 2), ('x_head_stride', c_int64 * 2),
+                ('dy', c_void_p * 2), ('out', c_void_p * 2), ('weight', c_void_p * 2), ('dweight', c_void_p * 2),
+                ('positions', c_void_p), ('inv_freq', c_void_p), ('scratch', c_void_p), ('tokens', c_int64),
+                ('heads', c_int32 * 2), ('positions_int64', c_int32), ('inv_freq_f64', c_int32), ('axes', c_int32),
+                ('sections', c_int32 * 4), ('interleaved', c_int32), ('dweight_f32', c_int32 * 2),
+                ('dweight_accumulate', c_int32 * 2), ('eps', c_float)]
+
+
+class FgaNorm(ctypes.Structure):
+    """Arguments of fga_norm_forward / fga_norm_backward (include/fga.h)."""
+    _fields_ = ([(name, c_void_p) for name in (
+        'x', 'branch', 'weight', 'gate', 'scale', 'shift', 'cu_seqlens', 'y', 'r', 'rstd', 'mean', 'dy', 'dr', 'dx',
+        'dbranch', 'dweight', 'dgate', 'dscale', 'dshift', 'scratch')]
+        + [('tokens', c_int64), ('hidden', c_int32), ('samples', c_int32), ('center', c_int32),
+           ('dweight_f32', c_int32), ('dweight_accumulate', c_int32), ('eps', c_float)])
 
 
 class FgaError(RuntimeError):
@@ -67,12 +86,21 @@ def _declare(l):
     l.fga_bias_grad_static_capacity_floats.restype = i64
     l.fga_bias_grad_static.argtypes = [vp, i64, i, vp, i, i, vp]
     l.fga_mx_quantize.argtypes = [vp, i64, i, i64, i64, vp, vp, i64, i, vp]
+    l.fga_rotary_forward.argtypes = [vp, vp]
+    l.fga_rotary_backward.argtypes = [vp, vp]
+    l.fga_rotary_scratch_floats.argtypes = [i64, i, i]
+    l.fga_rotary_scratch_floats.restype = i64
+    l.fga_norm_forward.argtypes = [vp, vp]
+    l.fga_norm_backward.argtypes = [vp, vp]
+    l.fga_norm_scratch_floats.argtypes = [i64, i, i, i, i]
+    l.fga_norm_scratch_floats.restype = i64
     for name in ('fga_symm_alloc', 'fga_symm_export', 'fga_symm_open', 'fga_symm_close',
                  'fga_symm_free', 'fga_symm_alloc_vmm', 'fga_symm_open_vmm', 'fga_symm_release_vmm', 'fga_barrier', 'fga_gemm_push', 'fga_gemm_recv',
                  'fga_gemm_push_gqa', 'fga_gemm_recv_gqa',
                  'fga_gemm_local', 'fga_gemm_local_mx', 'fga_gemm_push_mx', 'fga_gemm_recv_mx',
                  'fga_gemm_push_gqa_mx', 'fga_gemm_recv_gqa_mx', 'fga_copy_rank_rows', 'fga_bias_grad', 'fga_bias_grad_static',
-                 'fga_mx_quantize'):
+                 'fga_mx_quantize', 'fga_rotary_forward', 'fga_rotary_backward', 'fga_norm_forward',
+                 'fga_norm_backward'):
         getattr(l, name).restype = i
 
 
@@ -81,7 +109,9 @@ EXPORTS = ('fga_version', 'fga_last_error', 'fga_sm_count', 'fga_launch_count', 
            'fga_symm_open_vmm', 'fga_symm_release_vmm', 'fga_barrier', 'fga_gemm_push',
            'fga_gemm_recv', 'fga_gemm_push_gqa', 'fga_gemm_recv_gqa', 'fga_gemm_local', 'fga_gemm_local_mx', 'fga_gemm_push_mx', 'fga_gemm_recv_mx',
            'fga_gemm_push_gqa_mx', 'fga_gemm_recv_gqa_mx', 'fga_copy_rank_rows', 'fga_bias_grad_scratch_floats',
-           'fga_bias_grad', 'fga_bias_grad_static_capacity_floats', 'fga_bias_grad_static', 'fga_mx_quantize')
+           'fga_bias_grad', 'fga_bias_grad_static_capacity_floats', 'fga_bias_grad_static', 'fga_mx_quantize',
+           'fga_rotary_forward', 'fga_rotary_backward', 'fga_rotary_scratch_floats', 'fga_norm_forward',
+           'fga_norm_backward', 'fga_norm_scratch_floats')
 
 
 def check(rc, exc=FgaError):

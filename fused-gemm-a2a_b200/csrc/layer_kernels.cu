@@ -1,0 +1,846 @@
+// Memory-bound sm_100a kernels that stand around the fused projections of an attention layer: rotary
+// positions with the normalisation of query and key heads in front of them, and the norm around a block
+// with its gate, residual sum, scale and shift. Forward and backward, C ABI at the end of the file.
+//
+// All of them are byte movers: 16-byte accesses, every element of the large tensors read and written
+// once, sums in FP32, one rounding to BF16 at the end. Reductions over tokens (gradients of weights and
+// of per-sample vectors) go through FP32 partial sums in caller-provided scratch and are finished in a
+// fixed order, so results do not depend on scheduling.
+#include <cstdint>
+#include <cuda_bf16.h>
+#include "../../include/fga.h"
+#include "common.cuh"
+#include "seq_bounds.cuh"
+
+namespace fga {
+namespace {
+
+constexpr int kHeadDim = 128;
+
+__device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = lo_f32(w[i]);
+    f[2 * i + 1] = hi_f32(w[i]);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+}
+__device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ void store16(uint16_t* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
+
+// =============================================================================================
+// Rotary positions. Pair i of a head turns by angle pos[axis(i)] * inv_freq[i]; interleaved pairs are
+// elements (2i, 2i+1), half-split pairs (i, i+64). With a weight w the head is first divided by its root
+// mean square and multiplied by w:  y = R(x * rstd * w).
+//
+// Angles: a position of 10^6 times a frequency of 1 leaves an FP32 product with errors of 0.06 rad. The
+// angle is only needed modulo one turn, so the frequency is held as a 64-bit fixed-point number of turns
+// (2^-64 each), the product with the integer position wraps modulo 2^64 exactly, and only the top 32 bits
+// become a float: the error is below 2^-25 turns at every position below 2^31.
+//
+// Mapping: one warp per token (several when tokens are few), which computes the token's 64 sines and
+// cosines once for all heads; a half-warp holds one head row, 8 elements a lane.
+// =============================================================================================
+constexpr int kRotaryWarps = 8;
+
+struct RotaryParams {
+  const uint16_t* x[2];       // forward: inputs; backward: the forward's inputs (only read where w is set)
+  const uint16_t* dy[2];      // backward: incoming gradients
+  uint16_t* out[2];           // forward: outputs; backward: gradients of x
+  const uint16_t* w[2];       // [128] or null
+  long long x_tok[2], x_head[2], dy_tok[2], dy_head[2];  // strides in elements; out is contiguous
+  int heads[2];
+  const void* pos;            // [tokens, axes]
+  int pos64;
+  int axes;
+  int ends[4];                // pairs of axis a are ends[a-1] .. ends[a]-1
+  const void* freq;           // [64]
+  int freq64;
+  int tokens;
+  int splits;                 // warps per token
+  float eps;
+  float* partial;             // backward with weights: [grid][2][128]
+};
+
+__device__ __forceinline__ void warp_rotation(const RotaryParams& P, const unsigned long long* turns, int token, int lane,
+                                              float2* table) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int pair = lane + 32 * i;
+    int axis = 0;
+    while (axis + 1 < P.axes && pair >= P.ends[axis]) ++axis;
+    const long long at = static_cast<long long>(token) * P.axes + axis;
+    const long long pos = P.pos64 ? __ldg(static_cast<const long long*>(P.pos) + at)
+                                  : static_cast<long long>(__ldg(static_cast<const int*>(P.pos) + at));
+    const unsigned long long phase = turns[pair] * static_cast<unsigned long long>(pos);
+    // top 32 bits as a signed fraction of a turn; sincospi takes half turns
+    const float half_turns = static_cast<float>(static_cast<int>(phase >> 32)) * 4.656612873077393e-10f;  // 2^-31
+    float s, c;
+    sincospif(half_turns, &s, &c);
+    table[pair] = make_float2(c, s);
+  }
+  __syncwarp();
+}
+
+// Rotation of a lane's 8 elements; `sign` -1 turns back. Half-split rows exchange their halves between
+// lanes l and l ^ 8.
+template <bool kInterleaved>
+__device__ __forceinline__ void rotate8(float (&f)[8], const float (&c)[8], const float (&s)[8], bool upper, float sign) {
+  if constexpr (kInterleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = f[2 * i], b = f[2 * i + 1], sn = sign * s[i];
+      f[2 * i] = a * c[i] - b * sn;
+      f[2 * i + 1] = b * c[i] + a * sn;
+    }
+  } else {
+    const float flip = upper ? sign : -sign;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, f[i], 8);
+      f[i] = f[i] * c[i] + other * (flip * s[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ float half_warp_sum(float v) {
+#pragma unroll
+  for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <bool kInterleaved, bool kBackward, bool kNorm>
+__global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryParams P) {
+  __shared__ unsigned long long turns[64];
+  __shared__ float2 tables[kRotaryWarps][64];
+  __shared__ float reduce[kBackward && kNorm ? kRotaryWarps : 1][2][kHeadDim];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < 64) {
+    const double f = P.freq64 ? __ldg(static_cast<const double*>(P.freq) + threadIdx.x)
+                              : static_cast<double>(__ldg(static_cast<const float*>(P.freq) + threadIdx.x));
+    const double t = f * 0.15915494309189533577;  // turns per position
+    turns[threadIdx.x] = static_cast<unsigned long long>((t - floor(t)) * 18446744073709551616.0);
+  }
+  __syncthreads();
+  const int sub = lane & 15, half = lane >> 4;
+  const bool upper = sub >= 8;
+  float w[2][8];
+  float dw[2][8];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[t][i] = 0.f;
+    if (kNorm && P.w[t] != nullptr) unpack8(load16(P.w[t] + sub * 8), w[t]);
+  }
+  const long long units = static_cast<long long>(P.tokens) * P.splits;
+  for (long long u = static_cast<long long>(blockIdx.x) * kRotaryWarps + warp; u < units;
+       u += static_cast<long long>(gridDim.x) * kRotaryWarps) {
+    const int token = static_cast<int>(u / P.splits), split = static_cast<int>(u % P.splits);
+    warp_rotation(P, turns, token, lane, tables[warp]);
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < (kInterleaved ? 4 : 8); ++i) {
+      const float2 e = tables[warp][kInterleaved ? sub * 4 + i : (sub & 7) * 8 + i];
+      c[i] = e.x;
+      s[i] = e.y;
+    }
+    __syncwarp();  // the table is rewritten for the next token
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int heads = P.heads[t];
+      const bool normed = kNorm && P.w[t] != nullptr;
+      const uint16_t* xp = P.x[t] + token * P.x_tok[t] + sub * 8;
+      const uint16_t* gp = kBackward ? P.dy[t] + token * P.dy_tok[t] + sub * 8 : nullptr;
+      uint16_t* op = P.out[t] + static_cast<long long>(token) * heads * kHeadDim + sub * 8;
+#pragma unroll 4
+      for (int h0 = 2 * split; h0 < heads; h0 += 2 * P.splits) {  // the same trips for all lanes
+        const int h = h0 + half;
+        const bool active = h < heads;
+        uint4 raw = make_uint4(0, 0, 0, 0), xraw = make_uint4(0, 0, 0, 0);
+        if constexpr (kBackward) {
+          if (active) raw = load16(gp + h * P.dy_head[t]);
+          if (normed && active) xraw = load16(xp + h * P.x_head[t]);
+        } else {
+          if (active) raw = load16(xp + h * P.x_head[t]);
+        }
+        float f[8];
+        unpack8(raw, f);
+        if constexpr (!kBackward) {
+          if (normed) {
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq += f[i] * f[i];
+            const float rstd = rsqrtf(half_warp_sum(sq) * (1.f / kHeadDim) + P.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * w[t][i];
+          }
+          rotate8<kInterleaved>(f, c, s, upper, 1.f);
+        } else {
+          rotate8<kInterleaved>(f, c, s, upper, -1.f);
+          if (normed) {
+            // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n))
+            float x[8], sq = 0.f, dot = 0.f;
+            unpack8(xraw, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              sq += x[i] * x[i];
+              dot += f[i] * w[t][i] * x[i];
+            }
+            const float rstd = rsqrtf(half_warp_sum(sq) * (1.f / kHeadDim) + P.eps);
+            const float mean = half_warp_sum(dot) * rstd * (1.f / kHeadDim);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float n = x[i] * rstd;
+              if (active) dw[t][i] += f[i] * n;
+              f[i] = rstd * (f[i] * w[t][i] - n * mean);
+            }
+          }
+        }
+        if (active) store16(op + h * kHeadDim, pack8(f));
+      }
+    }
+  }
+  if constexpr (kBackward && kNorm) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = dw[t][i] + __shfl_xor_sync(0xffffffffu, dw[t][i], 16);
+        if (half == 0) reduce[warp][t][sub * 8 + i] = v;
+      }
+    __syncthreads();
+    const int t = threadIdx.x >> 7, col = threadIdx.x & 127;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRotaryWarps; ++k) v += reduce[k][t][col];
+    P.partial[(static_cast<long long>(blockIdx.x) * 2 + t) * kHeadDim + col] = v;
+  }
+}
+
+// =============================================================================================
+// Column sums of FP32 partials: out[s][col] (=|+=) sum over slots first(s) .. last(s) of part[slot][col].
+// 32 columns a block, 16 threads a column that each take every 16th slot, joined in order.
+// =============================================================================================
+struct FinishParams {
+  const float* part;       // slot pitch `pitch`
+  long long pitch;
+  int width;
+  int slots;               // samples == 0: slots 0 .. slots-1 go into one row
+  const int* cu;           // samples > 0: the slots of sample s are c + s for its row chunks c
+  int samples, tokens, chunk_rows;
+  void* out[4];            // up to four results whose partials lie `width` floats apart in a slot
+  int out_f32[4], accumulate[4];
+};
+
+__global__ void __launch_bounds__(512) finish_sums_kernel(const FinishParams P) {
+  __shared__ float sums[16][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + lane, which = blockIdx.y, sample = blockIdx.z;
+  if (P.out[which] == nullptr) return;
+  int first = 0, last = P.slots;
+  if (P.samples > 0) {
+    const int a = seq_bound(P.cu, sample, P.samples, P.tokens), b = seq_bound(P.cu, sample + 1, P.samples, P.tokens);
+    first = a / P.chunk_rows + sample;
+    last = b > a ? (b - 1) / P.chunk_rows + sample + 1 : first;
+  }
+  float v = 0.f;
+  if (col < P.width) {
+    const float* p = P.part + static_cast<long long>(which) * P.width + col;
+#pragma unroll 4
+    for (int i = first + slice; i < last; i += 16) v += p[i * P.pitch];
+  }
+  sums[slice][lane] = v;
+  __syncthreads();
+  if (slice == 0 && col < P.width) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) v += sums[k][lane];
+    const long long at = static_cast<long long>(sample) * P.width + col;
+    if (P.out_f32[which]) {
+      float* o = static_cast<float*>(P.out[which]) + at;
+      *o = P.accumulate[which] ? *o + v : v;
+    } else {
+      static_cast<__nv_bfloat16*>(P.out[which])[at] = __float2bfloat16(v);
+    }
+  }
+}
+
+// =============================================================================================
+// Norm around a block.  r = x + gate * branch;  n = (r - mean) * rstd (mean only when centred);
+// y = n * weight * (1 + scale) + shift.  gate, scale and shift are one row per packed sample.
+//
+// A block takes a chunk of consecutive rows, a thread the same 8 * kVec columns of each, so weight,
+// scale, shift and gate stay in registers from row to row and the column sums of the backward pass are
+// register sums over the chunk. Slot chunk + sample of the partial sums is unique: walking down the rows
+// either of the two grows.
+// =============================================================================================
+struct NormParams {
+  const uint16_t *x, *branch, *weight, *gate, *scale, *shift;
+  const int* cu;
+  int samples, tokens, hidden, chunk_rows, center;
+  float eps;
+  uint16_t *y, *r;            // forward outputs (r may be null: no branch)
+  float *rstd, *mean;         // [tokens]: written by forward (may be null), read by backward
+  const uint16_t *dy, *dr;    // backward: either may be null
+  uint16_t *dx, *dbranch;     // dbranch only with a gate
+  float* part_weight;         // [chunks][hidden] or null
+  float* part_mod;            // [chunks + samples][3][hidden]: gate, scale, shift; or null
+};
+
+// Sum of N values over the block; `buf` alternates between two halves so that one barrier is enough.
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float* buf, int warps) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) buf[i * 32 + warp] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float s = lane < warps ? buf[i * 32 + lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    v[i] = s;
+  }
+}
+
+struct RowRange {
+  int sample, end;  // current sample (or P.samples: padding) and the row at which it ends
+};
+
+__device__ __forceinline__ RowRange range_of(const NormParams& P, int row) {
+  RowRange s;
+  s.sample = P.cu == nullptr ? 0 : seq_of_row(P.cu, P.samples, P.tokens, row);
+  s.end = s.sample < P.samples ? seq_bound(P.cu, s.sample + 1, P.samples, P.tokens) : P.tokens;
+  if (s.end <= row) s.end = row + 1;  // offsets that do not ascend
+  return s;
+}
+
+template <int kVec>
+__global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormParams P) {
+  __shared__ float buf[2][64];
+  const int warps = blockDim.x >> 5;
+  const int row0 = blockIdx.x * P.chunk_rows, row1 = min(row0 + P.chunk_rows, P.tokens);
+  const int vecs = P.hidden >> 3;
+  const float inv_h = 1.f / P.hidden;
+  uint4 wt[kVec], gt[kVec], sc[kVec], sh[kVec], xv[kVec], bv[kVec];
+  bool on[kVec];
+  int col[kVec];
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) {
+    const int v = threadIdx.x + k * blockDim.x;
+    on[k] = v < vecs;
+    col[k] = v * 8;
+    wt[k] = gt[k] = sc[k] = sh[k] = xv[k] = bv[k] = make_uint4(0, 0, 0, 0);
+    if (on[k] && P.weight != nullptr) wt[k] = load16(P.weight + col[k]);
+  }
+  auto fetch = [&](int row) {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k]) {
+        const long long at = static_cast<long long>(row) * P.hidden + col[k];
+        xv[k] = load16(P.x + at);
+        if (P.branch != nullptr) bv[k] = load16(P.branch + at);
+      }
+  };
+  if (row0 < row1) fetch(row0);
+  RowRange s{0, 0};
+  int parity = 0;
+  for (int row = row0; row < row1; ++row) {
+    if (row == row0 || row >= s.end) {
+      s = range_of(P, row);
+      if (s.sample < P.samples) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+          if (on[k]) {
+            const long long at = static_cast<long long>(s.sample) * P.hidden + col[k];
+            if (P.gate != nullptr) gt[k] = load16(P.gate + at);
+            if (P.scale != nullptr) sc[k] = load16(P.scale + at);
+            if (P.shift != nullptr) sh[k] = load16(P.shift + at);
+          }
+      }
+    }
+    const bool padding = s.sample >= P.samples;
+    float r[kVec][8];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      unpack8(xv[k], r[k]);
+      if (P.branch != nullptr && !(padding && P.gate != nullptr)) {
+        float b[8], g[8];
+        unpack8(bv[k], b);
+        unpack8(gt[k], g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[k][i] += P.gate != nullptr ? g[i] * b[i] : b[i];
+      }
+    }
+    if (row + 1 < row1) fetch(row + 1);
+    float mean = 0.f;
+    if (P.center) {
+      float t[1] = {0.f};
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[0] += r[k][i];  // columns beyond the row hold zeros
+      block_sum(t, buf[parity], warps);
+      parity ^= 1;
+      mean = t[0] * inv_h;
+    }
+    float t[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k])
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = r[k][i] - mean;
+          t[0] += d * d;
+        }
+    block_sum(t, buf[parity], warps);
+    parity ^= 1;
+    const float rstd = rsqrtf(t[0] * inv_h + P.eps);
+    if (threadIdx.x == 0 && P.rstd != nullptr) {
+      P.rstd[row] = rstd;
+      if (P.mean != nullptr) P.mean[row] = mean;
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k]) {
+        const long long at = static_cast<long long>(row) * P.hidden + col[k];
+        if (P.r != nullptr) store16(P.r + at, pack8(r[k]));
+        float y[8], w[8], a[8], b[8];
+        unpack8(wt[k], w);
+        unpack8(sc[k], a);
+        unpack8(sh[k], b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = (r[k][i] - mean) * rstd;
+          if (P.weight != nullptr) y[i] *= w[i];
+          if (P.scale != nullptr) y[i] *= 1.f + a[i];
+          if (P.shift != nullptr) y[i] += b[i];
+        }
+        store16(P.y + at, padding ? make_uint4(0, 0, 0, 0) : pack8(y));
+      }
+  }
+}
+
+// dz = dy * (1 + scale);  dn = dz * weight;  dc = rstd * (dn - n * mean(dn * n)) (- its mean when centred)
+// dx = dr + dc;  dbranch = gate * dx;  sums over the rows of a sample: dgate = sum dx * branch,
+// dshift = sum dy, a = sum dy * n, from which dscale = a * weight and dweight gets (1 + scale) * a. The
+// mean over a centred row of dc is rstd * mean(dn), because the mean of n is zero up to rounding.
+template <int kVec, bool kMod>
+__global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormParams P) {
+  __shared__ float buf[2][64];
+  const int warps = blockDim.x >> 5;
+  const int row0 = blockIdx.x * P.chunk_rows, row1 = min(row0 + P.chunk_rows, P.tokens);
+  const int vecs = P.hidden >> 3;
+  const float inv_h = 1.f / P.hidden;
+  uint4 wt[kVec], gt[kVec], sc[kVec], rv[kVec], bv[kVec], yv[kVec], dv[kVec];
+  float sa[kVec][8], dg[kVec][8], dh[kVec][8];
+  bool on[kVec];
+  int col[kVec];
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sa[k][i] = dg[k][i] = dh[k][i] = 0.f;
+  };
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) {
+    const int v = threadIdx.x + k * blockDim.x;
+    on[k] = v < vecs;
+    col[k] = v * 8;
+    wt[k] = gt[k] = sc[k] = rv[k] = bv[k] = yv[k] = dv[k] = make_uint4(0, 0, 0, 0);
+    if (on[k] && P.weight != nullptr) wt[k] = load16(P.weight + col[k]);
+  }
+  clear();
+  auto fetch = [&](int row) {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k]) {
+        const long long at = static_cast<long long>(row) * P.hidden + col[k];
+        rv[k] = load16(P.x + at);
+        if (kMod && P.gate != nullptr) bv[k] = load16(P.branch + at);
+        if (P.dy != nullptr) yv[k] = load16(P.dy + at);
+        if (P.dr != nullptr) dv[k] = load16(P.dr + at);
+      }
+  };
+  // Leaves the sums of the rows of `sample` behind. `fresh`: the first flush of this block.
+  auto flush = [&](int sample, bool fresh) {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k]) {
+        float w[8], a[8];
+        unpack8(wt[k], w);
+        unpack8(sc[k], a);
+        if (kMod && P.part_mod != nullptr) {
+          float* base = P.part_mod + static_cast<long long>(blockIdx.x + sample) * 3 * P.hidden + col[k];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            base[i] = dg[k][i];
+            base[P.hidden + i] = P.weight != nullptr ? sa[k][i] * w[i] : sa[k][i];
+            base[2 * P.hidden + i] = dh[k][i];
+          }
+        }
+        if (P.part_weight != nullptr) {
+          float* base = P.part_weight + static_cast<long long>(blockIdx.x) * P.hidden + col[k];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float v = kMod && P.scale != nullptr ? sa[k][i] * (1.f + a[i]) : sa[k][i];
+            base[i] = fresh ? v : base[i] + v;
+          }
+        }
+      }
+    clear();
+  };
+  if (row0 < row1) fetch(row0);
+  RowRange s{P.samples, 0};
+  int parity = 0;
+  bool fresh = true;
+  for (int row = row0; row < row1; ++row) {
+    if (row == row0 || row >= s.end) {
+      if (row != row0 && s.sample < P.samples) {
+        flush(s.sample, fresh);
+        fresh = false;
+      }
+      s = range_of(P, row);
+      if (kMod && s.sample < P.samples) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+          if (on[k]) {
+            const long long at = static_cast<long long>(s.sample) * P.hidden + col[k];
+            if (P.gate != nullptr) gt[k] = load16(P.gate + at);
+            if (P.scale != nullptr) sc[k] = load16(P.scale + at);
+          }
+      }
+    }
+    const bool padding = s.sample >= P.samples;
+    const float rstd = __ldg(P.rstd + row), mean = P.mean != nullptr ? __ldg(P.mean + row) : 0.f;
+    float n[kVec][8], dn[kVec][8];
+    uint4 b0[kVec], d0[kVec];
+    float t[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      b0[k] = bv[k];
+      d0[k] = dv[k];
+      float w[8], a[8];
+      unpack8(rv[k], n[k]);
+      unpack8(yv[k], dn[k]);
+      unpack8(wt[k], w);
+      unpack8(sc[k], a);
+      if (!padding && on[k])
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          n[k][i] = (n[k][i] - mean) * rstd;
+          sa[k][i] += dn[k][i] * n[k][i];
+          if (kMod) dh[k][i] += dn[k][i];
+          if (kMod && P.scale != nullptr) dn[k][i] *= 1.f + a[i];
+          if (P.weight != nullptr) dn[k][i] *= w[i];
+          t[0] += dn[k][i] * n[k][i];
+          t[1] += dn[k][i];
+        }
+    }
+    if (row + 1 < row1) fetch(row + 1);
+    block_sum(t, buf[parity], warps);
+    parity ^= 1;
+    const float dot = t[0] * inv_h, avg = P.center ? t[1] * inv_h : 0.f;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k]) {
+        const long long at = static_cast<long long>(row) * P.hidden + col[k];
+        float d[8];
+        unpack8(d0[k], d);
+        if (!padding)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] += rstd * (dn[k][i] - avg - n[k][i] * dot);
+        store16(P.dx + at, pack8(d));
+        if (kMod && P.dbranch != nullptr) {
+          float b[8], g[8];
+          unpack8(b0[k], b);
+          unpack8(gt[k], g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (!padding) dg[k][i] += d[i] * b[i];
+            g[i] = padding ? 0.f : g[i] * d[i];
+          }
+          store16(P.dbranch + at, pack8(g));
+        }
+      }
+  }
+  if (row0 < row1) {
+    if (s.sample < P.samples) {
+      flush(s.sample, fresh);
+    } else if (fresh && P.part_weight != nullptr) {
+      float* base = P.part_weight + static_cast<long long>(blockIdx.x) * P.hidden;  // nothing but padding
+      for (int i = threadIdx.x; i < P.hidden; i += blockDim.x) base[i] = 0.f;
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// Rows a norm block walks: two resident blocks on every SM share the rows evenly; at least one row.
+int norm_chunk_rows(long long tokens, int sms) { return static_cast<int>(ceil_div(tokens, 2ll * sms)); }
+
+struct NormShape {
+  int vec, threads;
+};
+// 8 columns a thread up to 2048 columns, 16 above: a block of at most 256 threads for 2048 columns and
+// 512 for 8192 keeps two blocks on an SM beside the FP32 column sums.
+NormShape norm_shape(int hidden) {
+  const int vecs = hidden / 8, vec = hidden <= 2048 ? 1 : 2;
+  return {vec, static_cast<int>(ceil_div(ceil_div(vecs, vec), 32) * 32)};
+}
+
+int rotary_grid(long long units, bool sums, int sms) {
+  // With sums every block leaves a row of partials behind, so the grid is what is resident at once.
+  const long long blocks = ceil_div(units, kRotaryWarps), most = sums ? 2ll * sms : 8ll * sms;
+  return static_cast<int>(blocks < most ? blocks : most);
+}
+
+// Warps a token's heads are spread over: as many as it takes to give every SM 16 warps.
+int rotary_splits(long long tokens, int heads, int sms) {
+  const long long want = ceil_div(16ll * sms, tokens), most = (heads + 1) / 2;
+  return static_cast<int>(want < most ? want : most);
+}
+
+int launch_rotary(const RotaryParams& P, int interleaved, bool backward, bool norm, int grid, cudaStream_t st) {
+  const dim3 g(grid), b(32 * kRotaryWarps);
+  if (interleaved) {
+    if (!backward) {
+      if (norm) rotary_kernel<true, false, true><<<g, b, 0, st>>>(P);
+      else rotary_kernel<true, false, false><<<g, b, 0, st>>>(P);
+    } else {
+      if (norm) rotary_kernel<true, true, true><<<g, b, 0, st>>>(P);
+      else rotary_kernel<true, true, false><<<g, b, 0, st>>>(P);
+    }
+  } else {
+    if (!backward) {
+      if (norm) rotary_kernel<false, false, true><<<g, b, 0, st>>>(P);
+      else rotary_kernel<false, false, false><<<g, b, 0, st>>>(P);
+    } else {
+      if (norm) rotary_kernel<false, true, true><<<g, b, 0, st>>>(P);
+      else rotary_kernel<false, true, false><<<g, b, 0, st>>>(P);
+    }
+  }
+  FGA_LAUNCHED();
+  return kSuccess;
+}
+
+int check_rotary(const FgaRotary* a, bool backward, RotaryParams& P) {
+  FGA_REQUIRE(a != nullptr, "rotary: null arguments");
+  FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fffffff, "rotary: tokens must be in [1, 2^31)");
+  FGA_REQUIRE(a->positions != nullptr && a->inv_freq != nullptr, "rotary: null pointer");
+  FGA_REQUIRE(a->axes >= 1 && a->axes <= 4, "rotary: one to four axes");
+  int at = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    FGA_REQUIRE(a->sections[i] >= 0 && a->sections[i] <= 64, "rotary: a section has 0 to 64 pairs");
+    at += a->sections[i];
+    P.ends[i] = at;
+  }
+  FGA_REQUIRE(at == 64, "rotary: the sections must add up to 64 pairs, not %d", at);
+  for (int t = 0; t < 2; ++t) {
+    FGA_REQUIRE(a->heads[t] >= 1 && a->heads[t] <= 65536, "rotary: 1 to 65536 heads");
+    const bool reads_x = !backward || a->weight[t] != nullptr;
+    FGA_REQUIRE(a->out[t] != nullptr && (a->x[t] != nullptr || !reads_x) && (a->dy[t] != nullptr || !backward),
+                "rotary: null pointer");
+    FGA_REQUIRE(aligned16(a->x[t]) && aligned16(a->dy[t]) && aligned16(a->out[t]) && aligned16(a->weight[t]),
+                "rotary: pointers must be 16-byte aligned");
+    FGA_REQUIRE(a->x_token_stride[t] % 8 == 0 && a->x_head_stride[t] % 8 == 0,
+                "rotary: strides must be multiples of 8 elements");
+    P.x[t] = static_cast<const uint16_t*>(a->x[t]);
+    P.dy[t] = static_cast<const uint16_t*>(a->dy[t]);
+    P.out[t] = static_cast<uint16_t*>(a->out[t]);
+    P.w[t] = static_cast<const uint16_t*>(a->weight[t]);
+    P.x_tok[t] = a->x_token_stride[t];
+    P.x_head[t] = a->x_head_stride[t];
+    P.dy_tok[t] = static_cast<long long>(a->heads[t]) * kHeadDim;
+    P.dy_head[t] = kHeadDim;
+    P.heads[t] = a->heads[t];
+  }
+  P.pos = a->positions;
+  P.pos64 = a->positions_int64;
+  P.axes = a->axes;
+  P.freq = a->inv_freq;
+  P.freq64 = a->inv_freq_f64;
+  P.tokens = static_cast<int>(a->tokens);
+  P.eps = a->eps;
+  P.splits = rotary_splits(a->tokens, a->heads[0] > a->heads[1] ? a->heads[0] : a->heads[1], sm_count());
+  return kSuccess;
+}
+
+int check_norm(const FgaNorm* a, NormParams& P) {
+  FGA_REQUIRE(a != nullptr, "norm: null arguments");
+  FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fffffff, "norm: tokens must be in [1, 2^31)");
+  FGA_REQUIRE(a->hidden >= 8 && a->hidden % 8 == 0 && a->hidden <= 8192, "norm: hidden must be a multiple of 8 up to 8192");
+  FGA_REQUIRE(a->samples >= 1 && a->samples <= 65535, "norm: 1 to 65535 samples");
+  FGA_REQUIRE(a->cu_seqlens != nullptr || a->samples == 1, "norm: several samples need cu_seqlens");
+  FGA_REQUIRE(a->gate == nullptr || a->branch != nullptr, "norm: a gate needs a branch");
+  const void* all[] = {a->x, a->branch, a->weight, a->gate, a->scale, a->shift, a->y, a->r, a->dy, a->dr, a->dx,
+                       a->dbranch, a->scratch};
+  for (const void* p : all) FGA_REQUIRE(aligned16(p), "norm: pointers must be 16-byte aligned");
+  P.x = static_cast<const uint16_t*>(a->x);
+  P.branch = static_cast<const uint16_t*>(a->branch);
+  P.weight = static_cast<const uint16_t*>(a->weight);
+  P.gate = static_cast<const uint16_t*>(a->gate);
+  P.scale = static_cast<const uint16_t*>(a->scale);
+  P.shift = static_cast<const uint16_t*>(a->shift);
+  P.cu = a->cu_seqlens;
+  P.center = a->center;
+  P.eps = a->eps;
+  P.y = static_cast<uint16_t*>(a->y);
+  P.r = static_cast<uint16_t*>(a->r);
+  P.rstd = a->rstd;
+  P.mean = a->center ? a->mean : nullptr;
+  P.dy = static_cast<const uint16_t*>(a->dy);
+  P.dr = static_cast<const uint16_t*>(a->dr);
+  P.dx = static_cast<uint16_t*>(a->dx);
+  P.dbranch = static_cast<uint16_t*>(a->dbranch);
+  P.tokens = static_cast<int>(a->tokens);
+  P.hidden = a->hidden;
+  P.samples = a->samples;
+  P.chunk_rows = norm_chunk_rows(a->tokens, sm_count());
+  return kSuccess;
+}
+
+}  // namespace
+}  // namespace fga
+
+using namespace fga;
+
+extern "C" {
+
+int fga_rotary_forward(const FgaRotary* args, void* stream) {
+  RotaryParams P = {};
+  const int rc = check_rotary(args, false, P);
+  if (rc != kSuccess) return rc;
+  const int grid = rotary_grid(static_cast<long long>(P.tokens) * P.splits, false, sm_count());
+  return launch_rotary(P, args->interleaved, false, P.w[0] || P.w[1], grid, static_cast<cudaStream_t>(stream));
+}
+
+int64_t fga_rotary_scratch_floats(int64_t tokens, int q_heads, int k_heads) {
+  if (tokens < 1 || q_heads < 1 || k_heads < 1) return 0;
+  const int sms = sm_count();
+  const int splits = rotary_splits(tokens, q_heads > k_heads ? q_heads : k_heads, sms);
+  return static_cast<int64_t>(rotary_grid(tokens * splits, true, sms)) * 2 * kHeadDim;
+}
+
+int fga_rotary_backward(const FgaRotary* args, void* stream) {
+  RotaryParams P = {};
+  int rc = check_rotary(args, true, P);
+  if (rc != kSuccess) return rc;
+  const bool norm = P.w[0] || P.w[1];
+  FGA_REQUIRE(!norm || args->scratch != nullptr, "rotary: weight gradients need scratch");
+  P.partial = args->scratch;
+  const int grid = rotary_grid(static_cast<long long>(P.tokens) * P.splits, norm, sm_count());
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  rc = launch_rotary(P, args->interleaved, true, norm, grid, st);
+  if (rc != kSuccess || !norm || (!args->dweight[0] && !args->dweight[1])) return rc;
+  FinishParams F = {};
+  F.part = args->scratch;
+  F.pitch = 2 * kHeadDim;
+  F.width = kHeadDim;
+  F.slots = grid;
+  for (int t = 0; t < 2; ++t) {
+    F.out[t] = args->weight[t] ? args->dweight[t] : nullptr;
+    F.out_f32[t] = args->dweight_f32[t];
+    F.accumulate[t] = args->dweight_accumulate[t];
+  }
+  finish_sums_kernel<<<dim3(kHeadDim / 32, 2, 1), 512, 0, st>>>(F);
+  FGA_LAUNCHED();
+  return kSuccess;
+}
+
+int fga_norm_forward(const FgaNorm* args, void* stream) {
+  NormParams P = {};
+  const int rc = check_norm(args, P);
+  if (rc != kSuccess) return rc;
+  FGA_REQUIRE(P.x != nullptr && P.y != nullptr && (P.branch == nullptr) == (P.r == nullptr),
+              "norm: x, y, and r exactly where there is a branch");
+  FGA_REQUIRE(P.rstd == nullptr || !P.center || P.mean != nullptr, "norm: a centred norm keeps its means beside rstd");
+  const NormShape shape = norm_shape(P.hidden);
+  const int grid = static_cast<int>(ceil_div(P.tokens, P.chunk_rows));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (shape.vec == 1)
+    norm_forward_kernel<1><<<grid, shape.threads, 0, st>>>(P);
+  else
+    norm_forward_kernel<2><<<grid, shape.threads, 0, st>>>(P);
+  FGA_LAUNCHED();
+  return kSuccess;
+}
+
+int64_t fga_norm_scratch_floats(int64_t tokens, int hidden, int samples, int has_weight, int modulated) {
+  if (tokens < 1 || hidden < 1 || samples < 1) return 0;
+  const int64_t chunks = ceil_div(tokens, norm_chunk_rows(tokens, sm_count()));
+  return (has_weight ? chunks * hidden : 0) + (modulated ? (chunks + samples) * 3 * hidden : 0);
+}
+
+int fga_norm_backward(const FgaNorm* args, void* stream) {
+  NormParams P = {};
+  int rc = check_norm(args, P);
+  if (rc != kSuccess) return rc;
+  P.x = P.r;  // what the forward normalised: the residual sum, or x itself where there is no branch
+  const bool modulated = args->dgate || args->dscale || args->dshift;
+  FGA_REQUIRE(P.x != nullptr && P.dx != nullptr && P.rstd != nullptr && (!P.center || P.mean != nullptr),
+              "norm: null pointer");
+  FGA_REQUIRE(P.gate == nullptr || P.dbranch != nullptr, "norm: a gate needs dbranch");
+  FGA_REQUIRE(args->scratch != nullptr || (!modulated && args->dweight == nullptr), "norm: sums over rows need scratch");
+  const long long chunks = ceil_div(P.tokens, P.chunk_rows);
+  if (args->dweight != nullptr) P.part_weight = args->scratch;
+  if (modulated) P.part_mod = args->scratch + (args->dweight != nullptr ? chunks * P.hidden : 0);
+  const NormShape shape = norm_shape(P.hidden);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int grid = static_cast<int>(chunks);
+  const bool mod = P.gate || P.scale || modulated;
+  if (shape.vec == 1) {
+    if (mod) norm_backward_kernel<1, true><<<grid, shape.threads, 0, st>>>(P);
+    else norm_backward_kernel<1, false><<<grid, shape.threads, 0, st>>>(P);
+  } else {
+    if (mod) norm_backward_kernel<2, true><<<grid, shape.threads, 0, st>>>(P);
+    else norm_backward_kernel<2, false><<<grid, shape.threads, 0, st>>>(P);
+  }
+  FGA_LAUNCHED();
+  const int blocks = static_cast<int>(ceil_div(P.hidden, 32));
+  if (args->dweight != nullptr) {
+    FinishParams F = {};
+    F.part = P.part_weight;
+    F.pitch = P.hidden;
+    F.width = P.hidden;
+    F.slots = static_cast<int>(chunks);
+    F.out[0] = args->dweight;
+    F.out_f32[0] = args->dweight_f32;
+    F.accumulate[0] = args->dweight_accumulate;
+    finish_sums_kernel<<<dim3(blocks, 1, 1), 512, 0, st>>>(F);
+    FGA_LAUNCHED();
+  }
+  if (modulated) {
+    FinishParams F = {};
+    F.part = P.part_mod;
+    F.pitch = 3ll * P.hidden;
+    F.width = P.hidden;
+    F.cu = P.cu;
+    F.samples = P.samples;
+    F.tokens = P.tokens;
+    F.chunk_rows = P.chunk_rows;
+    F.out[0] = args->dgate;
+    F.out[1] = args->dscale;
+    F.out[2] = args->dshift;
+    finish_sums_kernel<<<dim3(blocks, 3, P.samples), 512, 0, st>>>(F);
+    FGA_LAUNCHED();
+  }
+  return kSuccess;
+}
+
+}  // extern "C"

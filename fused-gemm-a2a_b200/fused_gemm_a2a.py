@@ -1296,3 +1296,7 @@ class FusedOutputProjection(_CallerOwnedProjection):
         if CHECK_TOKENS:
             _agree_on_tokens(workspace.comm, tokens)
         return _FusedOutput.apply(o, self.weight, self.bias, self, workspace._view(tokens, 1), tokens)
+
+
+# Operators around the projections (their own module; part of this module's public surface)
+from fused_layer_ops import residual_norm, rotary_embedding  # noqa: E402,F401

@@ -1,0 +1,310 @@
+"""Operators around the fused projections of an attention layer (B200 / sm_100a): rotary positions and
+the norm around a block, forward and backward, on the layouts the projections use: head side BF16
+[tokens, heads, 128], sequence side BF16 [tokens, hidden].
+
+    y, x = residual_norm(x, branch, weight=w)             # x + branch, normalised for the next block
+    q, k, v = FusedQKVProjection(...)(y, workspace)
+    q, k = rotary_embedding(q, k, positions, inv_freq, sections)
+
+The reference leaves these to its callers. As with the projections, weights are caller-owned BF16
+tensors; a weight with a Megatron `main_grad` gets its gradient accumulated there. Packed sequences are
+described by `cu_seqlens`, an int32 device tensor [samples + 1] of ascending offsets into the token axis
+that starts at 0 and is never read by the host; rows from its last offset on belong to no sequence.
+All device work is one or a few launches of libfga.so on the current stream of the tensors' device; there
+is no CPU or PyTorch fallback. Calls may be captured into CUDA graphs.
+"""
+from ctypes import byref
+
+import torch
+
+import _fga_native as _native
+
+HEAD_DIM = 128
+MAX_HIDDEN = 8192
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _same_device(first, *others):
+    if not first.is_cuda:
+        raise ValueError('The fused kernels only run on CUDA tensors; there is no CPU path')
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError('All tensors of a call must be on the same CUDA device')
+
+
+def _launch(entry, args, device):
+    """Call a libfga entry point on the current stream of `device`, whichever device is current."""
+    if torch.cuda.current_device() == device.index:
+        _native.check(entry(byref(args), torch.cuda.current_stream().cuda_stream))
+        return
+    with torch.cuda.device(device):
+        _native.check(entry(byref(args), torch.cuda.current_stream().cuda_stream))
+
+
+def _head_tensor(t, label):
+    """[tokens, heads, 128] BF16 whose heads are contiguous 16-byte aligned rows, with any token and head
+    stride that keeps them so."""
+    if t.ndim != 3 or t.shape[2] != HEAD_DIM or t.dtype != torch.bfloat16:
+        raise ValueError(f'{label} must be a BF16 tensor [tokens, heads, {HEAD_DIM}], got {t.dtype} {tuple(t.shape)}')
+    if t.shape[1] < 1:
+        raise ValueError(f'{label} needs at least one head')
+    token, head, inner = t.stride()
+    if (inner != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (token % 8 or token < HEAD_DIM))
+            or (t.shape[1] > 1 and (head % 8 or head < HEAD_DIM))):
+        raise ValueError(f'{label} needs contiguous 16-byte aligned heads: strides {t.stride()}')
+
+
+def _strides(t):
+    """Token and head stride; those of extents of one are never used and may be anything."""
+    token, head, _ = t.stride()
+    return token if t.shape[0] > 1 else t.shape[1] * HEAD_DIM, head if t.shape[1] > 1 else HEAD_DIM
+
+
+def _vector(t, length, label):
+    if t is None:
+        return
+    if tuple(t.shape) != (length,) or t.dtype != torch.bfloat16 or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f'{label} must be a contiguous, 16-byte aligned BF16 vector of {length} entries')
+
+
+def _offsets(cu_seqlens, label='cu_seqlens'):
+    if (cu_seqlens.ndim != 1 or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous()
+            or cu_seqlens.shape[0] < 2):
+        raise ValueError(f'{label} must be a contiguous int32 vector of at least two offsets')
+
+
+def _grad_rows(g, like):
+    """A gradient in the layout the kernels read: contiguous and 16-byte aligned (autograd may hand over
+    expanded or transposed ones)."""
+    if g.dtype != torch.bfloat16 or g.shape != like:
+        raise ValueError(f'gradients must be BF16 of shape {tuple(like)}')
+    g = g.contiguous()
+    return g if g.data_ptr() % 16 == 0 else g.clone()
+
+
+def _weight_target(weight, wanted):
+    """(tensor the gradient of `weight` goes to, accumulate): its FP32 main_grad where it has one, else a
+    fresh tensor of its own type."""
+    if weight is None or not wanted:
+        return None, False
+    main_grad = getattr(weight, 'main_grad', None)
+    if main_grad is None:
+        return torch.empty_like(weight), False
+    if (main_grad.shape != weight.shape or main_grad.dtype != torch.float32 or not main_grad.is_contiguous()
+            or main_grad.device != weight.device):
+        raise ValueError('main_grad must match the weight shape with contiguous FP32 storage')
+    return main_grad, True
+
+
+def _weight_result(weight, target, accumulated):
+    if target is None or not accumulated:
+        return target
+    from fused_gemm_a2a import _accumulated
+    return _accumulated(weight)
+
+
+# ----------------------------------------------------------------------------------------------
+# Rotary positions
+# ----------------------------------------------------------------------------------------------
+def _rotary_args(xs, outs, weights, positions, inv_freq, sections, interleaved, eps):
+    args = _native.FgaRotary()
+    for t in range(2):
+        args.out[t] = outs[t].data_ptr()
+        args.heads[t] = outs[t].shape[1]
+        args.weight[t] = _address(weights[t])
+        if xs[t] is not None:
+            args.x[t] = xs[t].data_ptr()
+            args.x_token_stride[t], args.x_head_stride[t] = _strides(xs[t])
+    args.positions, args.positions_int64 = positions.data_ptr(), positions.dtype == torch.int64
+    args.inv_freq, args.inv_freq_f64 = inv_freq.data_ptr(), inv_freq.dtype == torch.float64
+    args.tokens, args.axes, args.interleaved, args.eps = outs[0].shape[0], len(sections), interleaved, eps
+    for i, pairs in enumerate(sections):
+        args.sections[i] = pairs
+    return args
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, sections, interleaved, eps):
+        outs = tuple(torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+        if q.shape[0]:
+            _launch(_native.lib().fga_rotary_forward,
+                    _rotary_args((q, k), outs, (q_weight, k_weight), positions, inv_freq, sections, interleaved, eps),
+                    q.device)
+        # without a head norm the rotation's gradient does not need its input
+        ctx.save_for_backward(q if q_weight is not None else None, k if k_weight is not None else None, q_weight,
+                              k_weight, positions, inv_freq)
+        ctx.owners = (q_weight, k_weight)      # the caller's own parameters, which carry main_grad
+        ctx.shapes, ctx.rule = (q.shape, k.shape), (sections, interleaved, eps)
+        return outs
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+        sections, interleaved, eps = ctx.rule
+        grads = [_grad_rows(g, shape) for g, shape in zip((dq_out, dk_out), ctx.shapes)]
+        outs = [torch.empty(shape, device=positions.device, dtype=torch.bfloat16) for shape in ctx.shapes]
+        targets = [_weight_target(w, needed) for w, needed in zip(ctx.owners, ctx.needs_input_grad[2:4])]
+        tokens = outs[0].shape[0]
+        if tokens:
+            lib = _native.lib()
+            args = _rotary_args((q, k), outs, (q_weight, k_weight), positions, inv_freq, sections, interleaved, eps)
+            for t, (target, accumulate) in enumerate(targets):
+                args.dy[t] = grads[t].data_ptr()
+                args.dweight[t] = _address(target)
+                args.dweight_f32[t] = target is not None and target.dtype == torch.float32
+                args.dweight_accumulate[t] = accumulate
+            if q_weight is not None or k_weight is not None:
+                with torch.cuda.device(positions.device):
+                    floats = lib.fga_rotary_scratch_floats(tokens, args.heads[0], args.heads[1])
+                scratch = torch.empty(floats, device=positions.device, dtype=torch.float32)
+                args.scratch = scratch.data_ptr()
+            _launch(lib.fga_rotary_backward, args, positions.device)
+        else:
+            for target, accumulate in targets:
+                if target is not None and not accumulate:
+                    target.zero_()
+        dw = [_weight_result(w, *target) for w, target in zip(ctx.owners, targets)]
+        return (*outs, *dw, None, None, None, None, None)
+
+
+def rotary_embedding(q, k, positions, inv_freq, sections=None, *, interleaved=True, q_weight=None, k_weight=None,
+                     eps=1e-6):
+    """Rotary positions of the query and key heads, with several axes: q [tokens, heads, 128], k [tokens,
+    kv_heads, 128] BF16 -> new contiguous tensors of the same shapes. One launch for both.
+
+    positions: int32 or int64 [tokens, axes] (or [tokens] for one axis), any integer below 2^31 in size
+    (int64 positions wrap beyond that as int64 products do not: all 64 bits count). inv_freq: FP32 or FP64
+    [64], radians per position of each pair of elements; the first sections[0] pairs turn with axis 0
+    (time), the next sections[1] with axis 1 (height), and so on (default: all with one axis). Pairs are
+    elements (2i, 2i+1) when `interleaved`, (i, i+64) otherwise. Angles are exact modulo a turn whatever
+    the position (64-bit fixed point), so far positions lose nothing.
+
+    q_weight / k_weight (BF16 [128], each optional): the head is first divided by its root mean square
+    (mean of squares + eps) and multiplied by the weight, in FP32 with the rotation. Gradients flow to q,
+    k and the weights."""
+    _head_tensor(q, 'q')
+    _head_tensor(k, 'k')
+    if q.shape[0] != k.shape[0]:
+        raise ValueError('q and k must have the same number of tokens')
+    positions = positions.unsqueeze(1) if positions.ndim == 1 else positions
+    sections = (HEAD_DIM // 2,) if sections is None else tuple(sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != HEAD_DIM // 2:
+        raise ValueError(f'sections must split {HEAD_DIM // 2} pairs over one to four axes, got {sections}')
+    if (tuple(positions.shape) != (q.shape[0], len(sections)) or positions.dtype not in (torch.int32, torch.int64)
+            or not positions.is_contiguous()):
+        raise ValueError(f'positions must be contiguous int32 or int64 [tokens, {len(sections)}]')
+    if (tuple(inv_freq.shape) != (HEAD_DIM // 2,) or inv_freq.dtype not in (torch.float32, torch.float64)
+            or not inv_freq.is_contiguous()):
+        raise ValueError(f'inv_freq must be a contiguous FP32 or FP64 vector of {HEAD_DIM // 2} frequencies')
+    _vector(q_weight, HEAD_DIM, 'q_weight')
+    _vector(k_weight, HEAD_DIM, 'k_weight')
+    _same_device(q, k, positions, inv_freq, q_weight, k_weight)
+    return _Rotary.apply(q, k, q_weight, k_weight, positions, inv_freq, sections, bool(interleaved), float(eps))
+
+
+# ----------------------------------------------------------------------------------------------
+# Norm around a block
+# ----------------------------------------------------------------------------------------------
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, weight, gate, scale, shift, cu_seqlens, samples, eps, center):
+        tokens, hidden = x.shape
+        keep = any(ctx.needs_input_grad)
+        y = torch.empty_like(x)
+        r = None if branch is None else torch.empty_like(x)
+        rstd = torch.empty(tokens, device=x.device, dtype=torch.float32) if keep else None
+        mean = torch.empty(tokens, device=x.device, dtype=torch.float32) if keep and center else None
+        if tokens:
+            args = _native.FgaNorm(_address(x), _address(branch), _address(weight), _address(gate), _address(scale),
+                                   _address(shift), _address(cu_seqlens), _address(y), _address(r), _address(rstd),
+                                   _address(mean))
+            args.tokens, args.hidden, args.samples, args.center, args.eps = tokens, hidden, samples, center, eps
+            _launch(_native.lib().fga_norm_forward, args, x.device)
+        ctx.set_materialize_grads(False)
+        if keep:
+            ctx.save_for_backward(x if r is None else r, branch if gate is not None else None, weight, gate, scale,
+                                  cu_seqlens, rstd, mean)
+        ctx.owner, ctx.has_branch, ctx.has_shift = weight, branch is not None, shift is not None
+        ctx.rule = (samples, eps, center)
+        return y, x if r is None else r
+
+    @staticmethod
+    def backward(ctx, dy, dr):
+        r, branch, weight, gate, scale, cu_seqlens, rstd, mean = ctx.saved_tensors
+        samples, eps, center = ctx.rule
+        tokens, hidden = r.shape
+        needs = ctx.needs_input_grad
+        dy, dr = (None if g is None else _grad_rows(g, r.shape) for g in (dy, dr))
+        dx = torch.empty_like(r)
+        dbranch = torch.empty_like(r) if gate is not None else None
+        target, accumulate = _weight_target(ctx.owner, needs[2])
+        rows = [torch.empty((samples, hidden), device=r.device, dtype=r.dtype) if present and needed else None
+                for present, needed in ((gate is not None, needs[3]), (scale is not None, needs[4]),
+                                        (ctx.has_shift, needs[5]))]
+        if tokens:
+            lib = _native.lib()
+            modulated = any(t is not None for t in rows)
+            scratch = None
+            if target is not None or modulated:
+                with torch.cuda.device(r.device):
+                    floats = lib.fga_norm_scratch_floats(tokens, hidden, samples, target is not None, modulated)
+                scratch = torch.empty(floats, device=r.device, dtype=torch.float32)
+            args = _native.FgaNorm(None, _address(branch), _address(weight), _address(gate), _address(scale), None,
+                                   _address(cu_seqlens), None, _address(r), _address(rstd), _address(mean),
+                                   _address(dy), _address(dr), _address(dx), _address(dbranch), _address(target),
+                                   *(_address(t) for t in rows), _address(scratch))
+            args.tokens, args.hidden, args.samples, args.center, args.eps = tokens, hidden, samples, center, eps
+            args.dweight_f32 = target is not None and target.dtype == torch.float32
+            args.dweight_accumulate = accumulate
+            _launch(lib.fga_norm_backward, args, r.device)
+        else:
+            for t in (*rows, None if accumulate else target):
+                if t is not None:
+                    t.zero_()
+        if ctx.has_branch and gate is None:
+            dbranch = dx
+        return (dx, dbranch, _weight_result(ctx.owner, target, accumulate), *rows, None, None, None, None)
+
+
+def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=None, cu_seqlens=None, eps=1e-6,
+                  center=False):
+    """The step between two blocks: r = x + gate * branch, y = norm(r) * weight * (1 + scale) + shift, in
+    one pass. Returns (y, r); without a branch r is x. All BF16; sums and statistics in FP32, y computed
+    from the unrounded r.
+
+    x, branch: contiguous [tokens, hidden], hidden a multiple of 8 up to 8192. The norm divides by the root
+    mean square of the row, after subtracting its mean with `center` (a layer norm). weight: [hidden].
+    gate, scale, shift: [samples, hidden], one row for each packed sequence of cu_seqlens (one sample, or
+    [hidden], without it). With cu_seqlens, rows behind the last sequence have a gate of 0
+    and y = 0, and pass dr through to x in the backward pass. Gradients flow to everything but cu_seqlens."""
+    if x.ndim != 2 or x.dtype != torch.bfloat16 or not x.is_contiguous() or x.data_ptr() % 16:
+        raise ValueError('x must be a contiguous, 16-byte aligned BF16 tensor [tokens, hidden]')
+    tokens, hidden = x.shape
+    if hidden < 8 or hidden % 8 or hidden > MAX_HIDDEN:
+        raise ValueError(f'hidden must be a multiple of 8 up to {MAX_HIDDEN}, got {hidden}')
+    if branch is not None and (branch.shape != x.shape or branch.dtype != x.dtype or not branch.is_contiguous()
+                               or branch.data_ptr() % 16):
+        raise ValueError('branch must be a contiguous, 16-byte aligned BF16 tensor of the shape of x')
+    if gate is not None and branch is None:
+        raise ValueError('gate scales the branch: pass one')
+    _vector(weight, hidden, 'weight')
+    samples = 1
+    if cu_seqlens is not None:
+        _offsets(cu_seqlens)
+        samples = cu_seqlens.shape[0] - 1
+        if samples > 65535:
+            raise ValueError('at most 65535 packed sequences')
+    rows = []
+    for label, t in (('gate', gate), ('scale', scale), ('shift', shift)):
+        if t is not None and t.ndim == 1 and samples == 1:
+            t = t.unsqueeze(0)
+        if t is not None and (tuple(t.shape) != (samples, hidden) or t.dtype != torch.bfloat16
+                              or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f'{label} must be a contiguous, 16-byte aligned BF16 tensor [{samples}, {hidden}]')
+        rows.append(t)
+    _same_device(x, branch, weight, cu_seqlens, *rows)
+    return _ResidualNorm.apply(x, branch, weight, *rows, cu_seqlens, samples, float(eps), bool(center))

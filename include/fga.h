@@ -240,6 +240,63 @@ int fga_bias_grad_static(const void* dy, int64_t rows, int width, void* out, int
 int fga_mx_quantize(const void* a, int64_t rows, int k, int64_t stride_row, int64_t stride_k,
                     void* q, void* sf, int64_t rows_padded, int k_padded, void* stream);
 
+/* ---- operators around the projections ------------------------------------------------------
+ * No counterpart in the reference, which leaves these to its callers. Head-side tensors are BF16
+ * [tokens, heads, 128], sequence-side tensors BF16 [tokens, hidden]. Arguments travel in structs; a
+ * pointer that an operator does not use is NULL. cu_seqlens: device int32 [samples + 1] ascending
+ * offsets of packed sequences into the token axis, the first read as 0; rows from the last offset on
+ * belong to no sequence. NULL means one sequence of all rows. The host never reads it; offsets outside
+ * [0, tokens] are clamped by the kernels. */
+
+/* Rotary positions of q ([0]) and k ([1]), with the norm of each head in front where weight is set:
+ * out = R(positions * inv_freq) (x * rsqrt(mean(x^2) + eps) * weight). Pair i of a head (elements 2i and
+ * 2i+1 when interleaved, i and i+64 otherwise) turns by positions[token, axis] * inv_freq[i], where the
+ * first sections[0] pairs belong to axis 0, the next to axis 1, and so on; the sections add up to 64.
+ * backward: dy (contiguous) in, out = gradient of x, dweight (=|+=) gradient of the weight through
+ * `scratch` of fga_rotary_scratch_floats() floats; x is read only where weight is set. */
+typedef struct FgaRotary {
+  const void* x[2];          /* BF16, strides in elements, multiples of 8; the 128 elements of a head adjoin */
+  int64_t x_token_stride[2], x_head_stride[2];
+  const void* dy[2];         /* backward only */
+  void* out[2];              /* contiguous */
+  const void* weight[2];     /* BF16 [128] or NULL */
+  void* dweight[2];          /* backward: BF16 or FP32 [128], or NULL */
+  const void* positions;     /* [tokens, axes] int32 or int64 */
+  const void* inv_freq;      /* [64] FP32 or FP64 */
+  float* scratch;
+  int64_t tokens;
+  int32_t heads[2];
+  int32_t positions_int64, inv_freq_f64, axes, sections[4], interleaved;
+  int32_t dweight_f32[2], dweight_accumulate[2];
+  float eps;
+} FgaRotary;
+int fga_rotary_forward(const FgaRotary* args, void* stream);
+int64_t fga_rotary_scratch_floats(int64_t tokens, int q_heads, int k_heads);
+int fga_rotary_backward(const FgaRotary* args, void* stream);
+
+/* Norm around a block: r = x + gate * branch (gate 1 where NULL; no r without a branch),
+ * n = r * rsqrt(mean(r^2) + eps), or (r - mean) * rsqrt(var + eps) with center; y = n * weight * (1 +
+ * scale) + shift. weight: [hidden]; gate, scale, shift: one row of [samples, hidden] for each packed
+ * sequence. Rows behind the last sequence have a gate of 0 and y = 0: dx = dr. hidden: a multiple of 8
+ * up to 8192. backward reads r as the forward left it (x where there is no branch), rstd and mean; dy and
+ * dr may be NULL. The gradient of a branch without a gate is dx. scratch: fga_norm_scratch_floats() with
+ * has_weight = (dweight != NULL) and modulated = (any of dgate, dscale, dshift). */
+typedef struct FgaNorm {
+  const void *x, *branch, *weight, *gate, *scale, *shift;
+  const int32_t* cu_seqlens;
+  void *y, *r;
+  float *rstd, *mean;        /* [tokens] FP32: statistics kept for the backward pass (mean only with center) */
+  const void *dy, *dr;
+  void *dx, *dbranch, *dweight, *dgate, *dscale, *dshift;
+  float* scratch;
+  int64_t tokens;
+  int32_t hidden, samples, center, dweight_f32, dweight_accumulate;
+  float eps;
+} FgaNorm;
+int fga_norm_forward(const FgaNorm* args, void* stream);
+int64_t fga_norm_scratch_floats(int64_t tokens, int hidden, int samples, int has_weight, int modulated);
+int fga_norm_backward(const FgaNorm* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
