@@ -32,6 +32,14 @@ class FgaNorm(ctypes.Structure):
            ('dweight_f32', c_int32), ('dweight_accumulate', c_int32), ('eps', c_float)])
 
 
+class FgaAttention(ctypes.Structure):
+    """Arguments of fga_attention_forward / fga_attention_backward (include/fga.h)."""
+    _fields_ = ([(name, c_void_p) for name in (
+        'q', 'k', 'v', 'o', 'lse', 'd_o', 'dq', 'dk', 'dv', 'delta', 'cu_seqlens', 'status')]
+        + [('timeout_ns', c_uint64), ('token_stride', c_int64 * 3), ('head_stride', c_int64 * 3), ('tokens', c_int64),
+           ('heads', c_int32), ('kv_heads', c_int32), ('samples', c_int32), ('causal', c_int32), ('scale', c_float)])
+
+
 class FgaError(RuntimeError):
     """A libfga entry point returned a non-zero status."""
 
@@ -91,6 +99,7 @@ def _declare(l):
     l.fga_rotary_scratch_floats.argtypes = [i64, i, i]
     l.fga_rotary_scratch_floats.restype = i64
     l.fga_norm_forward.argtypes = [vp, vp]
+    l.fga_attention_forward.argtypes = [vp, vp]
     l.fga_norm_backward.argtypes = [vp, vp]
     l.fga_norm_scratch_floats.argtypes = [i64, i, i, i, i]
     l.fga_norm_scratch_floats.restype = i64
@@ -100,7 +109,7 @@ def _declare(l):
                  'fga_gemm_local', 'fga_gemm_local_mx', 'fga_gemm_push_mx', 'fga_gemm_recv_mx',
                  'fga_gemm_push_gqa_mx', 'fga_gemm_recv_gqa_mx', 'fga_copy_rank_rows', 'fga_bias_grad', 'fga_bias_grad_static',
                  'fga_mx_quantize', 'fga_rotary_forward', 'fga_rotary_backward', 'fga_norm_forward',
-                 'fga_norm_backward'):
+                 'fga_norm_backward', 'fga_attention_forward'):
         getattr(l, name).restype = i
 
 
@@ -111,7 +120,7 @@ EXPORTS = ('fga_version', 'fga_last_error', 'fga_sm_count', 'fga_launch_count', 
            'fga_gemm_push_gqa_mx', 'fga_gemm_recv_gqa_mx', 'fga_copy_rank_rows', 'fga_bias_grad_scratch_floats',
            'fga_bias_grad', 'fga_bias_grad_static_capacity_floats', 'fga_bias_grad_static', 'fga_mx_quantize',
            'fga_rotary_forward', 'fga_rotary_backward', 'fga_rotary_scratch_floats', 'fga_norm_forward',
-           'fga_norm_backward', 'fga_norm_scratch_floats')
+           'fga_norm_backward', 'fga_norm_scratch_floats', 'fga_attention_forward')
 
 
 def check(rc, exc=FgaError):

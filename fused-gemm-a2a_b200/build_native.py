@@ -11,7 +11,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libfga.so')
-SOURCES = ('runtime.cu', 'aux_kernels.cu', 'gemm_sm100a.cu', 'layer_kernels.cu')
+SOURCES = ('runtime.cu', 'aux_kernels.cu', 'gemm_sm100a.cu', 'layer_kernels.cu', 'attention_sm100a.cu')
 FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17',
          '-Xcompiler', '-fPIC', '-shared']
 

@@ -54,6 +54,11 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
                    uint64_t rows, uint64_t cols, uint64_t row_pitch_elems, uint32_t box_rows,
                    uint32_t box_cols, bool swizzle128 = true);
 
+// Encode a 3-D BF16 tensor map [rows, planes, cols] with a [box_rows, 1, box_cols] box and 128-byte
+// swizzle (box_cols must be 64); pitches in elements, multiples of 8.
+int encode_tmap_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t planes, uint64_t cols,
+                   uint64_t row_pitch_elems, uint64_t plane_pitch_elems, uint32_t box_rows, uint32_t box_cols);
+
 int sm_count();
 
 }  // namespace fga

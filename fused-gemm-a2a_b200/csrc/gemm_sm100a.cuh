@@ -25,6 +25,7 @@
 #include "common.cuh"
 #include "mx_quant.cuh"
 #include "schedule.cuh"
+#include "wait.cuh"
 
 namespace fga {
 
@@ -101,50 +102,6 @@ struct GemmParams {
   int* status;
   unsigned long long timeout_ns;
 };
-
-struct WaitCtx {
-  int* status;
-  unsigned long long timeout_ns;
-  uint32_t abort_flag;  // shared address of this CTA's abort word
-  bool dead;
-};
-
-__device__ __forceinline__ void report(WaitCtx& w, int code, int where, int detail) {
-  if (atomicCAS(w.status, 0, code) == 0) {
-    w.status[1] = where;
-    w.status[2] = detail;
-  }
-  asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(w.abort_flag), "r"(1u) : "memory");
-  w.dead = true;
-}
-
-__device__ __forceinline__ bool should_abort(WaitCtx& w) {
-  uint32_t f;
-  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(f) : "r"(w.abort_flag) : "memory");
-  if (f != 0 || ld_relaxed_sys_s32(w.status) != 0) {
-    w.dead = true;
-    return true;
-  }
-  return false;
-}
-
-// Bounded mbarrier wait. Returns false when the kernel is aborting.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, WaitCtx& w, int where) {
-  if (w.dead) return false;
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t it = 0;
-  while (!mbar_try_wait(bar, parity)) {
-    if ((++it & 0x3ff) == 0) {
-      if (should_abort(w)) return false;
-      if (globaltimer_ns() - t0 > w.timeout_ns) {
-        report(w, kErrPipelineTimeout, where, static_cast<int>(bar));
-        return false;
-      }
-    }
-  }
-  return true;
-}
 
 // Bounded acquire-poll of a global counter until it reaches `target`.
 __device__ __forceinline__ bool counter_wait(const int* ctr, int target, WaitCtx& w, int where,

@@ -78,6 +78,24 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
   return kSuccess;
 }
 
+int encode_tmap_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t planes, uint64_t cols,
+                   uint64_t row_pitch_elems, uint64_t plane_pitch_elems, uint32_t box_rows, uint32_t box_cols) {
+  auto enc = tmap_encoder();
+  if (enc == nullptr) return set_error(kCudaError, "cuTensorMapEncodeTiled is not available");
+  cuuint64_t dims[3] = {cols, planes, rows};
+  cuuint64_t strides[2] = {plane_pitch_elems * 2, row_pitch_elems * 2};
+  cuuint32_t box[3] = {box_cols, 1, box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(kCudaError, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%llu planes=%llu)",
+                     static_cast<int>(r), static_cast<unsigned long long>(rows),
+                     static_cast<unsigned long long>(planes));
+  return kSuccess;
+}
+
 // ---- virtual-memory-management allocations -----------------------------------------------------
 // Driver entry points are looked up through the runtime, so the library does not link libcuda.
 struct VmmApi {

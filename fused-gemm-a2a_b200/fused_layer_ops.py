@@ -1,10 +1,11 @@
-"""Operators around the fused projections of an attention layer (B200 / sm_100a): rotary positions and
-the norm around a block, forward and backward, on the layouts the projections use: head side BF16
-[tokens, heads, 128], sequence side BF16 [tokens, hidden].
+"""Operators around the fused projections of an attention layer (B200 / sm_100a): attention over packed
+sequences, rotary positions and the norm around a block, forward and backward, on the layouts the
+projections use: head side BF16 [tokens, heads, 128], sequence side BF16 [tokens, hidden].
 
     y, x = residual_norm(x, branch, weight=w)             # x + branch, normalised for the next block
     q, k, v = FusedQKVProjection(...)(y, workspace)
     q, k = rotary_embedding(q, k, positions, inv_freq, sections)
+    branch = FusedOutputProjection(...)(packed_attention(q, k, v, cu_seqlens), workspace)
 
 The reference leaves these to its callers. As with the projections, weights are caller-owned BF16
 tensors; a weight with a Megatron `main_grad` gets its gradient accumulated there. Packed sequences are
@@ -18,6 +19,7 @@ from ctypes import byref
 import torch
 
 import _fga_native as _native
+import fused_gemm_a2a_kernels as _k
 
 HEAD_DIM = 128
 MAX_HIDDEN = 8192
@@ -104,6 +106,85 @@ def _weight_result(weight, target, accumulated):
         return target
     from fused_gemm_a2a import _accumulated
     return _accumulated(weight)
+
+
+# ----------------------------------------------------------------------------------------------
+# Attention
+# ----------------------------------------------------------------------------------------------
+def _status(device):
+    """The device's status word for kernels outside a CP group, which the check_status() of any group on
+    the device covers. Zeroed before any stream may read it, and never from inside a capture."""
+    word = _k._local_status.get(device)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('Call packed_attention once on this device before capturing it into a CUDA graph')
+        with torch.cuda.device(device):
+            word = _k._status_word(device)
+            torch.cuda.current_stream().synchronize()
+    return word
+
+
+def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale):
+    args = _native.FgaAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr())
+    args.cu_seqlens, args.status = _address(cu_seqlens), _status(q.device).data_ptr()
+    args.timeout_ns = _k.DEVICE_TIMEOUT_NS
+    for i, t in enumerate((q, k, v)):
+        args.token_stride[i], args.head_stride[i] = _strides(t)
+    args.tokens, args.heads, args.kv_heads = q.shape[0], q.shape[1], k.shape[1]
+    args.samples = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    args.causal, args.scale = causal, scale
+    return args
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, causal, scale):
+        tokens, heads, _ = q.shape
+        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32)
+        if tokens:
+            _launch(_native.lib().fga_attention_forward, _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale),
+                    q.device)
+        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+        ctx.rule = (causal, scale)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+
+def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, return_lse=False):
+    """softmax(scale * q k^T) v within each packed sequence, for each query head: q [tokens, heads, 128],
+    k and v [tokens, kv_heads, 128] BF16 -> o [tokens, heads, 128], contiguous. kv_heads divides heads;
+    query head h reads key/value head h // (heads // kv_heads). That is what FusedQKVProjection returns and
+    FusedOutputProjection takes.
+
+    cu_seqlens: sequence offsets (default: all tokens are one sequence); a token sees the tokens of its own
+    sequence, with `causal` those up to itself. Lengths may be anything, zero and one included. Rows behind
+    the last sequence give o = 0 and gradients of 0, and what they hold in q, k, v and in the incoming
+    gradient is not looked at. scale: positive, default 128 ** -0.5. return_lse: also return the FP32
+    [heads, tokens] logarithms of the rows' sums of exponentials (-inf behind the last sequence; no gradient
+    flows through them).
+
+    Scores, softmax statistics and all sums are FP32; the probabilities (and in the backward pass the
+    gradients of the scores) are rounded to BF16 for the second product. Results, gradients included, are
+    the same bits in every run. Kernel waits are bounded as in the projections and report through the
+    status word that comm.check_status() reads."""
+    for t, label in ((q, 'q'), (k, 'k'), (v, 'v')):
+        _head_tensor(t, label)
+    if k.shape != v.shape or k.shape[0] != q.shape[0]:
+        raise ValueError('k and v must have one shape, and q, k and v the same number of tokens')
+    if q.shape[1] % k.shape[1]:
+        raise ValueError('Query heads must be a multiple of key/value heads')
+    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float('inf'):
+        raise ValueError('scale must be positive and finite')
+    if cu_seqlens is not None:
+        _offsets(cu_seqlens)
+        if cu_seqlens.shape[0] > 65536:
+            raise ValueError('at most 65535 packed sequences')
+    _same_device(q, k, v, cu_seqlens)
+    o, lse = _Attention.apply(q, k, v, cu_seqlens, bool(causal), scale)
+    return (o, lse) if return_lse else o
 
 
 # ----------------------------------------------------------------------------------------------

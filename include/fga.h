@@ -297,6 +297,30 @@ int fga_norm_forward(const FgaNorm* args, void* stream);
 int64_t fga_norm_scratch_floats(int64_t tokens, int hidden, int samples, int has_weight, int modulated);
 int fga_norm_backward(const FgaNorm* args, void* stream);
 
+/* Attention over packed sequences: o = softmax(scale * q k^T) v for each sequence and query head, with
+ * causal only over keys at or before the query's position; query head h reads key/value head
+ * h / (heads / kv_heads). lse[h, row] is the natural logarithm of the row's sum of exponentials. Rows
+ * behind the last sequence: o = 0, lse = -inf, all gradients 0. scale > 0. status and timeout_ns as for
+ * the GEMMs; the calls of a device share its status word, whatever their streams.
+ * backward reads q, k, v, o, lse and the contiguous gradient d_o, and writes contiguous dq, dk, dv;
+ * delta: scratch of heads * tokens floats. The results do not depend on scheduling: no atomics. */
+typedef struct FgaAttention {
+  const void *q, *k, *v;     /* BF16 [tokens, heads | kv_heads, 128] with strides in elements, multiples of 8 */
+  void* o;                   /* contiguous */
+  float* lse;                /* [heads, tokens] */
+  const void* d_o;
+  void *dq, *dk, *dv;
+  float* delta;
+  const int32_t* cu_seqlens;
+  int32_t* status;
+  uint64_t timeout_ns;
+  int64_t token_stride[3], head_stride[3];  /* of q, k, v */
+  int64_t tokens;
+  int32_t heads, kv_heads, samples, causal;
+  float scale;
+} FgaAttention;
+int fga_attention_forward(const FgaAttention* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

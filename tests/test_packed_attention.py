@@ -1,0 +1,163 @@
+"""Attention over packed sequences: refusals on the CPU, the kernels against the 64-bit form on the GPU.
+
+Tolerances. Probabilities are rounded to BF16 for the product with V, each by at most 2^-8 of its value
+relative to the row's sum (the sum itself is FP32 and unrounded), so o is off by at most 2^-8 of
+sum_j p_j |v_j|, and once more by 2^-8 of its own value for the output. FP32 products, the exponential (2
+ulp) and the scores (|s| times 2^-23 as an error of the exponent) come on top: 2^-14 of sum_j p_j |v_j|.
+The backward pass rounds P and dS to BF16 in the same way, and reads o rounded: delta = sum(do * o) is off
+by 2^-8 sum |do||o| (and o's own error above); the bounds below carry these through with absolute values.
+"""
+import math
+
+import pytest
+import torch
+
+from tests import layer_reference as plain
+
+HALF = 2.0 ** -8
+FINE = 2.0 ** -14
+
+
+def attention(*args, **kwargs):
+    import fused_gemm_a2a
+    return fused_gemm_a2a.packed_attention(*args, **kwargs)
+
+
+def offsets(lengths):
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    return cu
+
+
+# ----------------------------------------------------------------------------------------- CPU
+def test_refusals():
+    bf = torch.bfloat16
+    q, k = torch.zeros(6, 4, 128, dtype=bf), torch.zeros(6, 2, 128, dtype=bf)
+    cu = torch.tensor([0, 2, 6], dtype=torch.int32)
+    for message, change in (
+            ('BF16', dict(q=q.float())), ('BF16', dict(q=q.half())), ('BF16', dict(k=k[..., :64])), ('BF16', dict(v=k[0])),
+            ('head', dict(k=k[:, :0], v=k[:, :0])), ('one shape', dict(v=q)), ('tokens', dict(k=k[:5], v=k[:5])),
+            ('multiple', dict(k=q[:, :3], v=q[:, :3])), ('scale', dict(scale=0.0)), ('scale', dict(scale=-1.0)),
+            ('scale', dict(scale=math.inf)), ('scale', dict(scale=math.nan)),
+            ('strides', dict(q=torch.zeros(6, 4, 256, dtype=bf)[..., ::2])),
+            ('strides', dict(v=torch.zeros(6, 1, 128, dtype=bf).expand(6, 2, 128))),
+            ('strides', dict(q=torch.zeros(6 * 4 * 128 + 4, dtype=bf)[4:].view(6, 4, 128))),
+            ('cu_seqlens', dict(cu_seqlens=cu.long())), ('cu_seqlens', dict(cu_seqlens=cu[:1])),
+            ('cu_seqlens', dict(cu_seqlens=cu.view(3, 1))),
+            ('65535', dict(cu_seqlens=torch.zeros(65537, dtype=torch.int32))), ('CUDA', {})):
+        with pytest.raises(ValueError, match=message):
+            attention(**(dict(q=q, k=k, v=k, cu_seqlens=cu) | change))
+
+
+def test_the_c_entry_refuses_what_the_kernels_cannot_do(native):
+    import ctypes
+
+    import _fga_native as api
+    args = api.FgaAttention(16, 16, 16, 16, 16, tokens=4, heads=4, kv_heads=2, samples=1, scale=0.1, status=16)
+    for i in range(3):
+        args.token_stride[i], args.head_stride[i] = 512, 128
+    assert native.fga_attention_forward(None, None) == -1 and b'null' in native.fga_last_error()
+    for field, value, message in (('tokens', 0, b'tokens'), ('tokens', 1 << 31, b'tokens'), ('kv_heads', 3, b'multiple'),
+                                  ('kv_heads', 0, b'multiple'), ('samples', 0, b'sequences'), ('samples', 2, b'cu_seqlens'),
+                                  ('scale', 0.0, b'scale'), ('scale', math.nan, b'scale'), ('q', 8, b'aligned'),
+                                  ('v', None, b'null'), ('status', None, b'null')):
+        broken = api.FgaAttention.from_buffer_copy(args)
+        setattr(broken, field, value)
+        assert native.fga_attention_forward(ctypes.byref(broken), None) == -1, field
+        assert message in native.fga_last_error(), (field, native.fga_last_error())
+    broken = api.FgaAttention.from_buffer_copy(args)
+    broken.head_stride[1] = 130
+    assert native.fga_attention_forward(ctypes.byref(broken), None) == -1 and b'strides' in native.fga_last_error()
+
+
+def test_gradient_of_the_plain_form_against_differences():
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(5, h, 8, generator=g, dtype=torch.float64).requires_grad_() for h in (4, 2, 2))
+    for causal in (False, True):
+        assert torch.autograd.gradcheck(lambda *t: plain.attention(*t, [0, 3, 3, 4], causal)[0], (q, k, v))
+
+
+# ----------------------------------------------------------------------------------------- GPU
+def normal(gen, *shape, std=1.0):
+    return (torch.randn(*shape, generator=gen, device='cuda') * std).bfloat16()
+
+
+def within(got, want, bound, label):
+    got = got.double()
+    assert got.shape == want.shape, label
+    assert torch.isfinite(got).all(), f'{label}: not finite'
+    excess = (got - want).abs() - bound
+    assert bool((excess <= 0).all()), f'{label}: over its bound by {excess.max().item():.3g} of {want.abs().max().item():.3g}'
+
+
+def expected(q, k, v, cu, causal, scale=None, do=None):
+    """o, lse and the gradients in 64 bits with the bounds of the kernels' errors."""
+    tokens, heads, dim = q.shape
+    group = heads // k.shape[1]
+    scale = dim ** -0.5 if scale is None else scale
+    zeros = lambda t: torch.zeros(t.shape, dtype=torch.float64, device=t.device)        # noqa: E731
+    o, eo, lse = zeros(q), zeros(q), torch.full((heads, tokens), -math.inf, dtype=torch.float64, device=q.device)
+    grads = {n: (zeros(t), zeros(t)) for n, t in (('q', q), ('k', k), ('v', v))}
+    for a, b in plain.segments(cu, tokens):
+        if a == b:
+            continue
+        mask = torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).triu(1) if causal else None
+        for h in range(heads):
+            g = h // group
+            qq, kk, vv = q[a:b, h].double(), k[a:b, g].double(), v[a:b, g].double()
+            s = qq @ kk.T * scale
+            if causal:
+                s = s.masked_fill(mask, -math.inf)
+            top = s.abs().masked_fill(s.isinf(), 0).amax()
+            fine = FINE + top.item() * 2.0 ** -21
+            p = s.softmax(-1)
+            lse[h, a:b] = torch.logsumexp(s, -1)
+            out = p @ vv
+            reach = p @ vv.abs()
+            o[a:b, h], eo[a:b, h] = out, (HALF * (1 + HALF) + fine) * reach + HALF * out.abs()
+            if do is None:
+                continue
+            d = do[a:b, h].double()
+            dp = d @ vv.T
+            delta = (d * out).sum(-1, keepdim=True)
+            edelta = (d.abs() * eo[a:b, h]).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            # dS: its own rounding, the exponential's and the products' error, and delta's
+            eds = HALF * (1 + HALF) * ds.abs() + p * ((1 + HALF) * edelta + fine * (dp.abs() + delta.abs() + d.abs() @ vv.abs().T))
+            for n, value, error in (('q', ds @ kk * scale, eds @ kk.abs() * scale),
+                                    ('k', ds.T @ qq * scale, eds.T @ qq.abs() * scale),
+                                    ('v', p.T @ d, (HALF + fine) * (p.T @ d.abs()))):
+                hh = h if n == 'q' else g
+                grads[n][0][a:b, hh] += value
+                grads[n][1][a:b, hh] += error * (1 + 2 * HALF) + fine * 2.0 ** -6 * value.abs()
+    for n in grads:
+        grads[n][1].add_(HALF * grads[n][0].abs())
+    return o, eo, lse, grads
+
+
+SHAPES = [
+    ([1], 0, 1, 1), ([1, 5, 17], 0, 8, 8), ([127], 0, 2, 1), ([128], 0, 2, 2), ([129], 0, 3, 1), ([255, 1], 0, 4, 2),
+    ([256], 5, 2, 1), ([257, 0, 0, 383], 130, 6, 3), ([0], 7, 2, 2), ([0, 3], 0, 1, 1), ([1000], 0, 5, 5),
+    ([700, 64, 65, 1, 640], 3, 4, 1), ([2049], 0, 2, 2),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lengths,pad,heads,kv_heads', SHAPES)
+@pytest.mark.parametrize('causal', [False, True])
+def test_forward_matches_the_plain_form(native, lengths, pad, heads, kv_heads, causal):
+    gen = torch.Generator(device='cuda').manual_seed(sum(lengths) + heads)
+    tokens, cu = sum(lengths) + pad, offsets(lengths)
+    q, k, v = normal(gen, tokens, heads, 128, std=1.5), normal(gen, tokens, kv_heads, 128), normal(gen, tokens, kv_heads, 128)
+    o, eo, lse, _ = expected(q, k, v, cu, causal)
+    if pad:                              # what padding rows hold must not matter
+        for t in (q, k, v):
+            t[-pad:] = float('nan')
+    got, got_lse = attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device='cuda'), causal=causal, return_lse=True)
+    within(got, o, eo + 1e-30, 'o')
+    live = cu[-1]
+    assert torch.isneginf(got_lse[:, live:]).all()
+    within(got_lse[:, :live], lse[:, :live], 1e-5 * (1 + lse[:, :live].abs()), 'lse')
+    if pad:
+        assert got[live:].abs().max() == 0
