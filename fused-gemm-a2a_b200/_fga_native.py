@@ -100,6 +100,7 @@ def _declare(l):
     l.fga_rotary_scratch_floats.restype = i64
     l.fga_norm_forward.argtypes = [vp, vp]
     l.fga_attention_forward.argtypes = [vp, vp]
+    l.fga_attention_backward.argtypes = [vp, vp]
     l.fga_norm_backward.argtypes = [vp, vp]
     l.fga_norm_scratch_floats.argtypes = [i64, i, i, i, i]
     l.fga_norm_scratch_floats.restype = i64
@@ -109,7 +110,7 @@ def _declare(l):
                  'fga_gemm_local', 'fga_gemm_local_mx', 'fga_gemm_push_mx', 'fga_gemm_recv_mx',
                  'fga_gemm_push_gqa_mx', 'fga_gemm_recv_gqa_mx', 'fga_copy_rank_rows', 'fga_bias_grad', 'fga_bias_grad_static',
                  'fga_mx_quantize', 'fga_rotary_forward', 'fga_rotary_backward', 'fga_norm_forward',
-                 'fga_norm_backward', 'fga_attention_forward'):
+                 'fga_norm_backward', 'fga_attention_forward', 'fga_attention_backward'):
         getattr(l, name).restype = i
 
 
@@ -120,7 +121,8 @@ EXPORTS = ('fga_version', 'fga_last_error', 'fga_sm_count', 'fga_launch_count', 
            'fga_gemm_push_gqa_mx', 'fga_gemm_recv_gqa_mx', 'fga_copy_rank_rows', 'fga_bias_grad_scratch_floats',
            'fga_bias_grad', 'fga_bias_grad_static_capacity_floats', 'fga_bias_grad_static', 'fga_mx_quantize',
            'fga_rotary_forward', 'fga_rotary_backward', 'fga_rotary_scratch_floats', 'fga_norm_forward',
-           'fga_norm_backward', 'fga_norm_scratch_floats', 'fga_attention_forward')
+           'fga_norm_backward', 'fga_norm_scratch_floats', 'fga_attention_forward',
+           'fga_attention_backward')
 
 
 def check(rc, exc=FgaError):

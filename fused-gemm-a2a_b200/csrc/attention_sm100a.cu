@@ -39,6 +39,10 @@ struct AttentionParams {
   float scale_log2;                             // scale * log2(e)
   uint16_t* o;                                  // forward: [tokens, heads, 128]
   float* lse;                                   // [heads, tokens], natural logarithm
+  const uint16_t* d_o;                          // backward: gradient of o, contiguous
+  uint16_t *dq, *dk, *dv;
+  float* delta;                                 // [heads, tokens]: rowwise sums of d_o * o
+  float scale;
   int tiles;                                    // work tiles per head in the grid (an upper bound)
   int* status;
   unsigned long long timeout_ns;
@@ -64,11 +68,14 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_tile, uint32_t b
     mma_bf16(d, a + step, b + step, kIdesc, k != 0);
   }
 }
-// D[128, 128] (+)= A B over the 128 rows of B: A from TMEM (BF16, 64 columns), B a tile read MN-major.
-__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a_tmem, uint32_t b_tile, bool accumulate) {
+// D[128, 128] (+)= A B over the 128 rows of B: A from TMEM (BF16, 64 columns, of which the second half may
+// lie `gap` columns further on), B a tile read MN-major.
+__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a_tmem, uint32_t b_tile, bool accumulate,
+                                             uint32_t gap = 0) {
   const uint64_t b = desc_mn_major(b_tile);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) mma_bf16_ta(d, a_tmem + k * 8, b + k * 128, kIdescMn, accumulate || k != 0);
+  for (int k = 0; k < 8; ++k)
+    mma_bf16_ta(d, a_tmem + k * 8 + (k >= 4 ? gap : 0), b + k * 128, kIdescMn, accumulate || k != 0);
 }
 
 // Work tile `t` of `rows` rows: tiles are numbered sequence by sequence, the rows behind the last
@@ -148,37 +155,38 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return r;
 }
 
-// Rows of a 128 x 128 FP32 accumulator, times `factor`, as BF16 to global memory: thread = row. Each
-// 64-column piece is staged in the thread's own 144-byte slot (a skew of 16 bytes keeps 16-byte stores free
-// of bank conflicts) and leaves with one bulk copy.
+// 64 columns of a row of an FP32 accumulator, times `factor`, as BF16 to global memory: thread = row. They
+// are staged in the thread's own 144-byte slot (a skew of 16 bytes keeps 16-byte stores free of bank
+// conflicts) and leave with one bulk copy. Whole warps.
 constexpr uint32_t kSlotPitch = 144;
-__device__ __forceinline__ void store_row(uint32_t tmem, uint32_t slot, uint16_t* dst, float factor, bool valid) {
+__device__ __forceinline__ void store_piece(uint32_t tmem, uint32_t slot, uint16_t* dst, float factor, bool valid) {
 #pragma unroll
-  for (int piece = 0; piece < 2; ++piece) {
-    if (piece) bulk_wait_read_all();
+  for (int c = 0; c < 2; ++c) {
+    uint32_t r[32];
+    tmem_ld_32x32(tmem + c * 32, r);
+    tmem_ld_wait();
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint32_t r[32];
-      tmem_ld_32x32(tmem + piece * 64 + c * 32, r);
-      tmem_ld_wait();
+    for (int v = 0; v < 4; ++v) {
+      uint32_t p[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        uint32_t p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          p[e] = pack_pair(__uint_as_float(r[v * 8 + 2 * e]) * factor, __uint_as_float(r[v * 8 + 2 * e + 1]) * factor);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + c * 64 + v * 16), "r"(p[0]), "r"(p[1]),
-                     "r"(p[2]), "r"(p[3])
-                     : "memory");
-      }
+      for (int e = 0; e < 4; ++e)
+        p[e] = pack_pair(__uint_as_float(r[v * 8 + 2 * e]) * factor, __uint_as_float(r[v * 8 + 2 * e + 1]) * factor);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + c * 64 + v * 16), "r"(p[0]), "r"(p[1]),
+                   "r"(p[2]), "r"(p[3])
+                   : "memory");
     }
-    fence_proxy_async_shared();
-    if (valid) {
-      bulk_store(dst + piece * 64, slot, 128);
-      bulk_commit();
-    }
-    __syncwarp();
   }
+  fence_proxy_async_shared();
+  if (valid) {
+    bulk_store(dst, slot, 128);
+    bulk_commit();
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void store_row(uint32_t tmem, uint32_t slot, uint16_t* dst, float factor, bool valid) {
+  store_piece(tmem, slot, dst, factor, valid);
+  bulk_wait_read_all();
+  store_piece(tmem + 64, slot, dst + 64, factor, valid);
 }
 
 // Every thread of the block: zero rows [row, end) of one head.
@@ -459,6 +467,503 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
 }
 
+// =============================================================================================
+// Backward. With P = exp(scale S - lse) and delta = rowsum(dO * O):
+//   dV = P^T dO,   dS = P * (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q.
+// Two kernels recompute S and dP: one owns key/value rows and walks over the queries (of all query heads
+// that share them, so a shared head's gradient is one sum in one accumulator), one owns query rows and
+// walks over the keys. That is 7 tile products where a single kernel would need 5, but dQ is then not
+// summed by atomics across blocks: every run gives the same bits, and no FP32 copy of dQ is kept.
+//
+// In both kernels two warpgroups share a 128 x 128 tile of scores, thread = row, 64 columns each. They
+// write their halves of P or dS as BF16 over their own halves of the scores, 64 columns apart.
+// =============================================================================================
+constexpr int kBwdThreads = 384;
+
+// delta[h, row]: half a warp per row, 8 elements a lane.
+__global__ void __launch_bounds__(256) attention_delta_kernel(const uint16_t* o, const uint16_t* d_o, float* delta,
+                                                              int tokens, int heads) {
+  const long long rows = static_cast<long long>(tokens) * heads;
+  const int sub = threadIdx.x & 15;
+  for (long long first = static_cast<long long>(blockIdx.x) * 16; first < rows;
+       first += static_cast<long long>(gridDim.x) * 16) {  // the whole block goes round together
+    const long long row = first + (threadIdx.x >> 4);
+    const bool on = row < rows;
+    float sum = 0.f;
+    if (on) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(o + row * kDim) + sub);
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(d_o + row * kDim) + sub);
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), sum);
+        sum = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), sum);
+      }
+    }
+#pragma unroll
+    for (int m = 8; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if (on && sub == 0) {
+      const int token = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<long long>(token) * heads);
+      delta[static_cast<long long>(head) * tokens + token] = sum;
+    }
+  }
+}
+
+// ---- dK, dV: S^T and dP^T tiles, rows = keys, columns = queries. TMEM: S^T (then P^T) 0, dP^T (then
+// dS^T) 128, dV 256, dK 384. The tensor cores run dV(i) and S(i+1) while the warps compute dS(i), and
+// dK(i) and dP(i+1) while they compute P(i+1).
+constexpr int kDkvStages = 2;
+constexpr uint32_t kDkvStageBytes = 2 * kTileBytes;
+constexpr uint32_t kDkvSmem = 2 * kTileBytes + kDkvStages * (kDkvStageBytes + 1024) + 256 + 1024;
+
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                         const __grid_constant__ AttentionParams P) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t k_smem = base, v_smem = base + kTileBytes, ring = base + 2 * kTileBytes;
+  const uint32_t rows_smem = ring + kDkvStages * kDkvStageBytes;  // per stage: -lse * log2(e) [128], delta [128]
+  const uint32_t bars = rows_smem + kDkvStages * 1024;
+  const uint32_t kv_full = bars, full = bars + 8, empty = full + 8 * kDkvStages, s_full = empty + 8 * kDkvStages,
+                 dp_full = s_full + 8, p_full = dp_full + 8, ds_full = p_full + 8, acc_done = ds_full + 8,
+                 own_bar = acc_done + 8, tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
+  static_assert(8 + 16 * kDkvStages + 48 + 16 <= 256, "barrier area");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int kv_head = blockIdx.x % P.kv_heads;
+  WorkTile wt;
+  // the first tiles first: under a causal mask they have the most queries behind them
+  if (!find_tile(P, kTile, static_cast<int>(blockIdx.x / P.kv_heads), wt)) return;
+  if (wt.padding) {
+    const int row = wt.first + wt.row0, end = min(row + kTile, wt.first + wt.len);
+    zero_rows(P.dk, P.kv_heads, kv_head, row, end);
+    zero_rows(P.dv, P.kv_heads, kv_head, row, end);
+    return;
+  }
+  const int q_tiles = (wt.len + kTile - 1) / kTile;
+  const int q_first = P.causal ? wt.row0 / kTile : 0;
+  const int per_head = q_tiles - q_first, total = per_head * P.group;
+
+  WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < kDkvStages; ++i) {
+      mbar_init(full + 8 * i, 3);  // Q, dO, and the row values
+      mbar_init(empty + 8 * i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_full, 8);
+    mbar_init(ds_full, 8);
+    mbar_init(acc_done, 1);
+    mbar_init(own_bar, 1);
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+
+  if (warp == 8) {
+    // ------------------------------------------------------------------ loads
+    if (lane == 0 && !w.dead) {
+      mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
+      load_tile(k_smem, &map_k, kv_full, kv_head, wt.first + wt.row0);
+      load_tile(v_smem, &map_v, kv_full, kv_head, wt.first + wt.row0);
+    }
+    int st = 0;
+    uint32_t phase = 0, own_phase = 0;
+    for (int i = 0; i < total && !w.dead; ++i) {
+      const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
+      const int valid = min(kTile, wt.len - row);
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(empty + 8 * st, phase ^ 1, w, 80);
+      if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
+        w.dead = true;
+        break;
+      }
+      const uint32_t q_dst = ring + st * kDkvStageBytes, do_dst = q_dst + kTileBytes, bar = full + 8 * st;
+      if (valid == kTile) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, kTileBytes);
+          load_tile(q_dst, &map_q, bar, head, wt.first + row);
+          mbar_arrive_expect_tx(bar, kTileBytes);
+          load_tile(do_dst, &map_do, bar, head, wt.first + row);
+        }
+      } else {
+        // rows behind the sequence are operands of the sums over queries here
+        if (!load_tail(q_dst, &map_q, bar, own_bar, own_phase, head, wt.first + row, valid, lane, w)) break;
+        if (!load_tail(do_dst, &map_do, bar, own_bar, own_phase, head, wt.first + row, valid, lane, w)) break;
+      }
+      const long long at = static_cast<long long>(head) * P.tokens + wt.first + row;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int q = c * 32 + lane;
+        float neg = -INFINITY, delta = 0.f;  // a probability of 0 behind the sequence
+        if (q < valid) {
+          neg = -kLog2e * __ldg(P.lse + at + q);
+          delta = __ldg(P.delta + at + q);
+        }
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows_smem + st * 1024 + q * 4), "f"(neg) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows_smem + st * 1024 + 512 + q * 4), "f"(delta) : "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(bar);
+      if (++st == kDkvStages) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ products
+    if (lane == 0 && mbar_wait(kv_full, 0, w, 81) && mbar_wait(full, 0, w, 82)) {
+      tc_fence_after();
+      mma_rows(tmem, k_smem, ring);
+      tc_commit(s_full);
+      mma_rows(tmem + 128, v_smem, ring + kTileBytes);
+      tc_commit(dp_full);
+      int st = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < total; ++i) {
+        const uint32_t q_tile = ring + st * kDkvStageBytes, do_tile = q_tile + kTileBytes;
+        const int cur = st;
+        if (++st == kDkvStages) {
+          st = 0;
+          phase ^= 1;
+        }
+        const uint32_t next_q = ring + st * kDkvStageBytes;
+        const bool more = i + 1 < total;
+        if (!mbar_wait(p_full, i & 1, w, 83)) break;
+        tc_fence_after();
+        mma_weighted(tmem + 256, tmem, do_tile, i > 0, 32);
+        if (more) {
+          if (!mbar_wait(full + 8 * st, phase, w, 84)) break;
+          tc_fence_after();
+          mma_rows(tmem, k_smem, next_q);
+          tc_commit(s_full);
+        }
+        if (!mbar_wait(ds_full, i & 1, w, 85)) break;
+        tc_fence_after();
+        mma_weighted(tmem + 384, tmem + 128, q_tile, i > 0, 32);
+        if (i + kDkvStages < total) tc_commit(empty + 8 * cur);
+        if (more) {
+          mma_rows(tmem + 128, v_smem, next_q + kTileBytes);
+          tc_commit(dp_full);
+        }
+      }
+      if (!w.dead) tc_commit(acc_done);
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ P and dS
+    const int g = warp >> 2, key = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + lanes + g * 64, dp_tmem = s_tmem + 128;
+    const float c = P.scale_log2;
+    int st = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    for (int i = 0; i < total; ++i) {
+      // the stage's own barrier orders this thread behind the stores of the row values
+      if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, phase, w, 89) && mbar_wait(s_full, i & 1, w, 86))) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      float p[64];
+      {
+        uint32_t s[2][32];
+        tmem_ld_32x32(s_tmem, s[0]);
+        tmem_ld_32x32(s_tmem + 32, s[1]);
+        tmem_ld_wait();
+        const uint32_t neg = rows_smem + st * 1024 + g * 256;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          float n[4];
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(n[0]), "=f"(n[1]), "=f"(n[2]), "=f"(n[3])
+                       : "r"(neg + v * 16));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            p[v * 4 + e] = exp2_approx(fmaf(__uint_as_float(s[v >> 3][(v & 7) * 4 + e]), c, n[e]));
+        }
+      }
+      if (P.causal && i % per_head == 0) {  // the diagonal tile: queries in front of the key do not see it
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (g * 64 + e < key) p[e] = 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t b[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) b[e] = pack_pair(p[h * 32 + 2 * e], p[h * 32 + 2 * e + 1]);
+        tmem_st_32x16(s_tmem + h * 16, b);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(p_full);
+      if (!__all_sync(0xffffffffu, mbar_wait(dp_full, i & 1, w, 87))) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t delta = rows_smem + st * 1024 + 512 + g * 256;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t d[32], b[16];
+        tmem_ld_32x32(dp_tmem + h * 32, d);
+        tmem_ld_wait();
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          float n[4];
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(n[0]), "=f"(n[1]), "=f"(n[2]), "=f"(n[3])
+                       : "r"(delta + h * 128 + v * 16));
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = p[h * 32 + v * 4 + e] * (__uint_as_float(d[v * 4 + e]) - n[e]);
+          b[2 * v] = pack_pair(x[0], x[1]);
+          b[2 * v + 1] = pack_pair(x[2], x[3]);
+        }
+        // columns [0, 32) of this warpgroup's half have been read when h = 1 is stored to [16, 32), and
+        // h = 0 goes to [0, 16), which it has just read itself
+        tmem_st_32x16(dp_tmem + h * 16, b);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(ds_full);
+      if (++st == kDkvStages) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+    if (alive && __all_sync(0xffffffffu, mbar_wait(acc_done, 0, w, 88))) {
+      tc_fence_after();
+      const bool valid = wt.row0 + key < wt.len;
+      const long long at = (static_cast<long long>(wt.first + wt.row0 + key) * P.kv_heads + kv_head) * kDim;
+      // one warpgroup stores dV, the other dK; K and V have been read for the last time
+      store_row(tmem + lanes + 256 + g * 128, (g ? k_smem : v_smem) + key * kSlotPitch, (g ? P.dk : P.dv) + at,
+                g ? P.scale : 1.f, valid);
+      bulk_wait_all();
+    }
+  }
+  settle(w);
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- dQ: S and dP tiles, rows = queries, columns = keys. TMEM: S (then dS) in two buffers 0 and 128, dP
+// 256, dQ 384. The tensor cores run S(j+1) and dP(j+1) while the warps compute dS(j).
+constexpr int kDqStages = 2;
+constexpr uint32_t kDqStageBytes = 2 * kTileBytes;
+constexpr uint32_t kDqSmem = 2 * kTileBytes + kDqStages * kDqStageBytes + 256 + 1024;
+
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                        const __grid_constant__ AttentionParams P) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_smem = base, do_smem = base + kTileBytes, ring = base + 2 * kTileBytes;
+  const uint32_t bars = ring + kDqStages * kDqStageBytes;
+  const uint32_t q_full = bars, full = bars + 8, empty = full + 8 * kDqStages, s_full = empty + 8 * kDqStages,
+                 dp_full = s_full + 16, dp_read = dp_full + 8, ds_full = dp_read + 8, acc_done = ds_full + 8,
+                 own_bar = acc_done + 8, tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
+  static_assert(8 + 16 * kDqStages + 56 + 16 <= 256, "barrier area");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int head = blockIdx.x % P.heads;
+  WorkTile wt;
+  if (!find_tile(P, kTile, P.tiles - 1 - static_cast<int>(blockIdx.x / P.heads), wt)) return;
+  if (wt.padding) {
+    const int row = wt.first + wt.row0;
+    zero_rows(P.dq, P.heads, head, row, min(row + kTile, wt.first + wt.len));
+    return;
+  }
+  const int all_tiles = (wt.len + kTile - 1) / kTile;
+  const int n = P.causal ? min(all_tiles, wt.row0 / kTile + 1) : all_tiles;
+
+  WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < kDqStages; ++i) {
+      mbar_init(full + 8 * i, 2);  // K and V
+      mbar_init(empty + 8 * i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_full + 8, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(dp_read, 8);
+    mbar_init(ds_full, 8);
+    mbar_init(acc_done, 1);
+    mbar_init(own_bar, 1);
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+
+  if (warp == 8) {
+    // ------------------------------------------------------------------ loads
+    const int kv_head = head / P.group;
+    if (lane == 0 && !w.dead) {
+      mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+      load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
+      load_tile(do_smem, &map_do, q_full, head, wt.first + wt.row0);
+    }
+    int st = 0;
+    uint32_t phase = 0, own_phase = 0;
+    for (int j = 0; j < n && !w.dead; ++j) {
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(empty + 8 * st, phase ^ 1, w, 90);
+      if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
+        w.dead = true;
+        break;
+      }
+      const int row = j * kTile, valid = wt.len - row;
+      const uint32_t k_dst = ring + st * kDqStageBytes, bar = full + 8 * st;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, kTileBytes);
+        load_tile(k_dst + kTileBytes, &map_v, bar, kv_head, wt.first + row);
+      }
+      if (valid < kTile) {  // K is also summed over, V only makes scores that are masked
+        if (!load_tail(k_dst, &map_k, bar, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
+      } else if (lane == 0) {
+        mbar_arrive_expect_tx(bar, kTileBytes);
+        load_tile(k_dst, &map_k, bar, kv_head, wt.first + row);
+      }
+      if (++st == kDqStages) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ products
+    if (lane == 0 && mbar_wait(q_full, 0, w, 91) && mbar_wait(full, 0, w, 92)) {
+      tc_fence_after();
+      mma_rows(tmem, q_smem, ring);
+      tc_commit(s_full);
+      mma_rows(tmem + 256, do_smem, ring + kTileBytes);
+      tc_commit(dp_full);
+      int st = 0;
+      uint32_t phase = 0;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t k_tile = ring + st * kDqStageBytes;
+        const int cur = st;
+        if (++st == kDqStages) {
+          st = 0;
+          phase ^= 1;
+        }
+        const uint32_t next_k = ring + st * kDqStageBytes;
+        if (j + 1 < n) {
+          if (!mbar_wait(full + 8 * st, phase, w, 93)) break;
+          tc_fence_after();
+          mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, next_k);
+          tc_commit(s_full + 8 * ((j + 1) & 1));
+          if (!mbar_wait(dp_read, j & 1, w, 94)) break;
+          tc_fence_after();
+          mma_rows(tmem + 256, do_smem, next_k + kTileBytes);
+          tc_commit(dp_full);
+        }
+        if (!mbar_wait(ds_full, j & 1, w, 95)) break;
+        tc_fence_after();
+        mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_tile, j > 0, 32);
+        if (j + kDqStages < n) tc_commit(empty + 8 * cur);
+      }
+      if (!w.dead) tc_commit(acc_done);
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ dS
+    const int g = warp >> 2, row_in_tile = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int row = wt.row0 + row_in_tile;
+    const bool valid = row < wt.len;
+    const long long at = wt.first + (valid ? row : 0);
+    const float c = P.scale_log2;
+    const float neg = -kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at);
+    const float delta = __ldg(P.delta + static_cast<long long>(head) * P.tokens + at);
+    bool alive = true;
+    for (int j = 0; j < n; ++j) {
+      const uint32_t s_tmem = tmem + lanes + (j & 1) * 128 + g * 64, dp_tmem = tmem + lanes + 256 + g * 64;
+      if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * (j & 1), (j >> 1) & 1, w, 96))) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      float p[64];
+      {
+        uint32_t s[2][32];
+        tmem_ld_32x32(s_tmem, s[0]);
+        tmem_ld_32x32(s_tmem + 32, s[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 64; ++e) p[e] = exp2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), c, neg));
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(dp_full, j & 1, w, 97))) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t d[2][32];
+      tmem_ld_32x32(dp_tmem, d[0]);
+      tmem_ld_32x32(dp_tmem + 32, d[1]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(dp_read);
+#pragma unroll
+      for (int e = 0; e < 64; ++e) p[e] *= __uint_as_float(d[e >> 5][e & 31]) - delta;
+      if (j == n - 1) {
+        const int limit = min(wt.len, P.causal ? row + 1 : wt.len) - j * kTile - g * 64;
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e >= limit) p[e] = 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t b[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) b[e] = pack_pair(p[h * 32 + 2 * e], p[h * 32 + 2 * e + 1]);
+        tmem_st_32x16(s_tmem + h * 16, b);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(ds_full);
+    }
+    if (alive && __all_sync(0xffffffffu, mbar_wait(acc_done, 0, w, 98))) {
+      tc_fence_after();
+      // each warpgroup stores half of the columns; Q and dO have been read for the last time
+      store_piece(tmem + lanes + 384 + g * 64, (g ? do_smem : q_smem) + row_in_tile * kSlotPitch,
+                  P.dq + (static_cast<long long>(wt.first + row) * P.heads + head) * kDim + g * 64, P.scale, valid);
+      bulk_wait_all();
+    }
+  }
+  settle(w);
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 }  // namespace
 
 // 3-D map [tokens, heads, 128] with boxes of 128 tokens x one head x 64 columns, 128-byte swizzle.
@@ -489,6 +994,7 @@ static int check_attention(const FgaAttention* a, AttentionParams& P) {
   P.group = a->heads / a->kv_heads;
   P.causal = a->causal;
   P.scale_log2 = a->scale * kLog2e;
+  P.scale = a->scale;
   P.o = static_cast<uint16_t*>(a->o);
   P.lse = a->lse;
   P.status = a->status;
@@ -522,6 +1028,41 @@ int fga_attention_forward(const FgaAttention* args, void* stream) {
   P.tiles = static_cast<int>(tiles);
   FGA_CUDA(cudaFuncSetAttribute(attention_forward_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdSmem));
   attention_forward_kernel<<<static_cast<unsigned>(blocks), kFwdThreads, kFwdSmem, static_cast<cudaStream_t>(stream)>>>(q, k, v, P);
+  FGA_LAUNCHED();
+  return kSuccess;
+}
+
+int fga_attention_backward(const FgaAttention* args, void* stream) {
+  AttentionParams P = {};
+  int rc = check_attention(args, P);
+  if (rc != kSuccess) return rc;
+  FGA_REQUIRE(args->d_o && args->dq && args->dk && args->dv && args->delta, "attention: null pointer");
+  for (const void* p : {args->d_o, const_cast<const void*>(args->dq), const_cast<const void*>(args->dk),
+                        const_cast<const void*>(args->dv)})
+    FGA_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "attention: pointers must be 16-byte aligned");
+  P.d_o = static_cast<const uint16_t*>(args->d_o);
+  P.dq = static_cast<uint16_t*>(args->dq);
+  P.dk = static_cast<uint16_t*>(args->dk);
+  P.dv = static_cast<uint16_t*>(args->dv);
+  P.delta = args->delta;
+  CUtensorMap q, k, v, d;
+  if ((rc = encode_heads(&q, args->q, P.tokens, P.heads, args->token_stride[0], args->head_stride[0])) != kSuccess) return rc;
+  if ((rc = encode_heads(&k, args->k, P.tokens, P.kv_heads, args->token_stride[1], args->head_stride[1])) != kSuccess) return rc;
+  if ((rc = encode_heads(&v, args->v, P.tokens, P.kv_heads, args->token_stride[2], args->head_stride[2])) != kSuccess) return rc;
+  if ((rc = encode_heads(&d, args->d_o, P.tokens, P.heads, static_cast<int64_t>(P.heads) * kDim, kDim)) != kSuccess) return rc;
+  const long long tiles = tile_bound(P, kTile), blocks = tiles * P.heads;
+  FGA_REQUIRE(blocks <= 0x7fffffff, "attention: too many heads and sequences for one launch");
+  P.tiles = static_cast<int>(tiles);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long row_blocks = (static_cast<long long>(P.tokens) * P.heads + 15) / 16, most = 16ll * sm_count();
+  attention_delta_kernel<<<static_cast<unsigned>(row_blocks < most ? row_blocks : most), 256, 0, st>>>(P.o, P.d_o, P.delta,
+                                                                                                      P.tokens, P.heads);
+  FGA_LAUNCHED();
+  FGA_CUDA(cudaFuncSetAttribute(attention_dkv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDkvSmem));
+  attention_dkv_kernel<<<static_cast<unsigned>(tiles * P.kv_heads), kBwdThreads, kDkvSmem, st>>>(q, k, v, d, P);
+  FGA_LAUNCHED();
+  FGA_CUDA(cudaFuncSetAttribute(attention_dq_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem));
+  attention_dq_kernel<<<static_cast<unsigned>(blocks), kBwdThreads, kDqSmem, st>>>(q, k, v, d, P);
   FGA_LAUNCHED();
   return kSuccess;
 }

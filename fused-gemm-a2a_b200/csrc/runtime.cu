@@ -54,6 +54,18 @@ static PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
   return fn;
 }
 
+// Encoding needs a current context. A thread that has made no runtime call yet (autograd's, in its first
+// backward pass) has none; selecting the device it is on makes the primary context current.
+template <typename Encode>
+static CUresult with_context(Encode encode) {
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
+  return r;
+}
+
 int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes,
                    uint64_t rows, uint64_t cols, uint64_t row_pitch_elems, uint32_t box_rows,
                    uint32_t box_cols, bool swizzle128) {
@@ -67,10 +79,11 @@ int encode_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
   cuuint64_t strides[1] = {row_pitch_elems * elem_bytes};
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = with_context([&] {
+    return enc(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   if (r != CUDA_SUCCESS)
     return set_error(kCudaError, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%llu cols=%llu)",
                      static_cast<int>(r), static_cast<unsigned long long>(rows),
@@ -86,9 +99,11 @@ int encode_tmap_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t p
   cuuint64_t strides[2] = {plane_pitch_elems * 2, row_pitch_elems * 2};
   cuuint32_t box[3] = {box_cols, 1, box_rows};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = with_context([&] {
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   if (r != CUDA_SUCCESS)
     return set_error(kCudaError, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%llu planes=%llu)",
                      static_cast<int>(r), static_cast<unsigned long long>(rows),

@@ -12,7 +12,9 @@ tensors; a weight with a Megatron `main_grad` gets its gradient accumulated ther
 described by `cu_seqlens`, an int32 device tensor [samples + 1] of ascending offsets into the token axis
 that starts at 0 and is never read by the host; rows from its last offset on belong to no sequence.
 All device work is one or a few launches of libfga.so on the current stream of the tensors' device; there
-is no CPU or PyTorch fallback. Calls may be captured into CUDA graphs.
+is no CPU or PyTorch fallback. Calls may be captured into CUDA graphs, backward passes included; as with any
+autograd code, no graph recorded outside the capture may then still hold the same leaves (autograd ties a
+leaf to the stream of the first graph that uses it and would wait on that stream from inside the capture).
 """
 from ctypes import byref
 
@@ -150,6 +152,21 @@ class _Attention(torch.autograd.Function):
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return o, lse
+
+    @staticmethod
+    def backward(ctx, d_o, _):
+        if d_o is None:
+            return (None,) * 6
+        q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
+        d_o = _grad_rows(d_o, o.shape)
+        grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
+        if q.shape[0]:
+            delta = torch.empty_like(lse)
+            args = _attention_args(q, k, v, o, lse, cu_seqlens, *ctx.rule)
+            args.d_o, args.delta = d_o.data_ptr(), delta.data_ptr()
+            args.dq, args.dk, args.dv = (t.data_ptr() for t in grads)
+            _launch(_native.lib().fga_attention_backward, args, q.device)
+        return (*grads, None, None, None)
 
 
 def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, return_lse=False):

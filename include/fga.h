@@ -320,6 +320,7 @@ typedef struct FgaAttention {
   float scale;
 } FgaAttention;
 int fga_attention_forward(const FgaAttention* args, void* stream);
+int fga_attention_backward(const FgaAttention* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -161,3 +161,96 @@ def test_forward_matches_the_plain_form(native, lengths, pad, heads, kv_heads, c
     within(got_lse[:, :live], lse[:, :live], 1e-5 * (1 + lse[:, :live].abs()), 'lse')
     if pad:
         assert got[live:].abs().max() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lengths,pad,heads,kv_heads', SHAPES)
+@pytest.mark.parametrize('causal', [False, True])
+def test_gradients_match_the_plain_form(native, lengths, pad, heads, kv_heads, causal):
+    gen = torch.Generator(device='cuda').manual_seed(sum(lengths) + heads)
+    tokens, cu = sum(lengths) + pad, offsets(lengths)
+    q, k, v = normal(gen, tokens, heads, 128, std=1.5), normal(gen, tokens, kv_heads, 128), normal(gen, tokens, kv_heads, 128)
+    do = normal(gen, tokens, heads, 128)
+    _, _, _, grads = expected(q, k, v, cu, causal, do=do)
+    if pad:
+        for t in (q, k, v, do):
+            t[-pad:] = float('nan')
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = attention(*leaves, torch.tensor(cu, dtype=torch.int32, device='cuda'), causal=causal)
+    for name, got in zip('qkv', torch.autograd.grad(o, leaves, do)):
+        within(got, grads[name][0], grads[name][1] + 1e-30, 'd' + name)
+        if pad:
+            assert got[cu[-1]:].abs().max() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('scale,std', [(1.0, 0.5), (0.02, 4.0), (0.3, 3.0)])
+def test_other_scales_and_peaked_rows(native, scale, std):
+    """Scores that reach the hundreds: the running maximum moves, and most probabilities vanish."""
+    gen = torch.Generator(device='cuda').manual_seed(7)
+    q, k, v, do = (normal(gen, 900, h, 128, std=s) for h, s in ((4, std), (2, std), (2, 1.0), (4, 1.0)))
+    ramp = torch.linspace(0.1, 3.0, 900, device='cuda')[:, None, None]       # later keys weigh more: maxima keep rising
+    k = (k.float() * ramp).bfloat16()
+    o, eo, lse, grads = expected(q, k, v, None, False, scale, do)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got, got_lse = attention(*leaves, scale=scale, return_lse=True)
+    within(got.detach(), o, eo + 1e-30, 'o')
+    within(got_lse, lse, 1e-5 * (1 + lse.abs()), 'lse')
+    for name, g in zip('qkv', torch.autograd.grad(got, leaves, do)):
+        within(g, grads[name][0], grads[name][1] + 1e-30, 'd' + name)
+
+
+@pytest.mark.gpu
+def test_strided_heads_and_expanded_gradients(native):
+    gen = torch.Generator(device='cuda').manual_seed(8)
+    packed = normal(gen, 300, 8, 128)
+    q, k = packed[:, 2:6], packed[:, 6:]
+    v = normal(gen, 2, 300, 128).transpose(0, 1)
+    views = [t.detach().requires_grad_() for t in (q, k, v)]
+    whole = [t.detach().contiguous().requires_grad_() for t in (q, k, v)]
+    outs = [attention(*t, causal=True) for t in (views, whole)]
+    assert torch.equal(*outs)
+    grads = [torch.autograd.grad(o.float().sum(), t) for o, t in zip(outs, (views, whole))]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.gpu
+def test_the_same_bits_on_side_streams_and_in_a_graph(native):
+    gen = torch.Generator(device='cuda').manual_seed(9)
+    cu = torch.tensor([0, 700, 701, 1500], dtype=torch.int32, device='cuda')
+    q, k, v, do = (normal(gen, 1500, h, 128) for h in (8, 2, 2, 8))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = attention(*leaves, cu, causal=True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    first = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            results.append(step())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        captured = step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for other in (*results, captured):
+        assert all(torch.equal(a, b) for a, b in zip(first, other))
+    with torch.no_grad():
+        q.normal_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+@pytest.mark.gpu
+def test_no_tokens(native):
+    q = torch.zeros(0, 4, 128, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+    o = attention(q, q, q)
+    assert o.shape == q.shape
+    assert torch.autograd.grad(o.sum(), q)[0].shape == q.shape
