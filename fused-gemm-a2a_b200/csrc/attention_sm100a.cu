@@ -1002,6 +1002,19 @@ static int check_attention(const FgaAttention* a, AttentionParams& P) {
   return kSuccess;
 }
 
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device, once per device and kernel.
+template <typename Kernel>
+static int allow_smem(Kernel kernel, uint32_t bytes, uint64_t& done) {
+  int dev = 0;
+  FGA_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit) return kSuccess;
+  FGA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+  return kSuccess;
+}
+static uint64_t g_smem_forward, g_smem_dkv, g_smem_dq;
+
 // Upper bound of the work tiles of `rows` rows: each sequence, and the rows behind the last, ends in one
 // that may be short.
 static long long tile_bound(const AttentionParams& P, int rows) {
@@ -1026,7 +1039,7 @@ int fga_attention_forward(const FgaAttention* args, void* stream) {
   const long long tiles = tile_bound(P, 2 * kTile), blocks = tiles * P.heads;
   FGA_REQUIRE(blocks <= 0x7fffffff, "attention: too many heads and sequences for one launch");
   P.tiles = static_cast<int>(tiles);
-  FGA_CUDA(cudaFuncSetAttribute(attention_forward_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdSmem));
+  if ((rc = allow_smem(attention_forward_kernel, kFwdSmem, g_smem_forward)) != kSuccess) return rc;
   attention_forward_kernel<<<static_cast<unsigned>(blocks), kFwdThreads, kFwdSmem, static_cast<cudaStream_t>(stream)>>>(q, k, v, P);
   FGA_LAUNCHED();
   return kSuccess;
@@ -1058,10 +1071,10 @@ int fga_attention_backward(const FgaAttention* args, void* stream) {
   attention_delta_kernel<<<static_cast<unsigned>(row_blocks < most ? row_blocks : most), 256, 0, st>>>(P.o, P.d_o, P.delta,
                                                                                                       P.tokens, P.heads);
   FGA_LAUNCHED();
-  FGA_CUDA(cudaFuncSetAttribute(attention_dkv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDkvSmem));
+  if ((rc = allow_smem(attention_dkv_kernel, kDkvSmem, g_smem_dkv)) != kSuccess) return rc;
   attention_dkv_kernel<<<static_cast<unsigned>(tiles * P.kv_heads), kBwdThreads, kDkvSmem, st>>>(q, k, v, d, P);
   FGA_LAUNCHED();
-  FGA_CUDA(cudaFuncSetAttribute(attention_dq_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem));
+  if ((rc = allow_smem(attention_dq_kernel, kDqSmem, g_smem_dq)) != kSuccess) return rc;
   attention_dq_kernel<<<static_cast<unsigned>(blocks), kBwdThreads, kDqSmem, st>>>(q, k, v, d, P);
   FGA_LAUNCHED();
   return kSuccess;

@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include "../../include/fga.h"
 #include "common.cuh"
+#include "ptx.cuh"
 #include "seq_bounds.cuh"
 
 namespace fga {
@@ -37,6 +38,21 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 __device__ __forceinline__ void store16(uint16_t* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
+
+// 16 bytes global -> shared without passing through registers; groups are per thread.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const uint16_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 
 // =============================================================================================
 // Rotary positions. Pair i of a head turns by angle pos[axis(i)] * inv_freq[i]; interleaved pairs are
@@ -142,39 +158,49 @@ __global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryP
     for (int i = 0; i < 8; ++i) dw[t][i] = 0.f;
     if (kNorm && P.w[t] != nullptr) unpack8(load16(P.w[t] + sub * 8), w[t]);
   }
-  const long long units = static_cast<long long>(P.tokens) * P.splits;
-  for (long long u = static_cast<long long>(blockIdx.x) * kRotaryWarps + warp; u < units;
-       u += static_cast<long long>(gridDim.x) * kRotaryWarps) {
-    const int token = static_cast<int>(u / P.splits), split = static_cast<int>(u % P.splits);
-    warp_rotation(P, turns, token, lane, tables[warp]);
+  // A trip takes two head rows of q, or two of k, so the weight is the same for a whole warp. The loads of
+  // four trips are in flight before the first is used.
+  constexpr int kAhead = 4;
+  const int units = P.tokens * P.splits;  // below 2^31: there is more than one split only with few tokens
+  const int q_trips = (P.heads[0] + 1) >> 1, trips = q_trips + ((P.heads[1] + 1) >> 1);
+  for (int u = blockIdx.x * kRotaryWarps + warp; u < units; u += gridDim.x * kRotaryWarps) {
+    const int token = P.splits == 1 ? u : u / P.splits, split = u - token * P.splits;
+    bool fresh = true;
     float c[8], s[8];
+    for (int trip0 = split; trip0 < trips; trip0 += kAhead * P.splits) {
+      uint4 raw[kAhead], xraw[kAhead];
 #pragma unroll
-    for (int i = 0; i < (kInterleaved ? 4 : 8); ++i) {
-      const float2 e = tables[warp][kInterleaved ? sub * 4 + i : (sub & 7) * 8 + i];
-      c[i] = e.x;
-      s[i] = e.y;
-    }
-    __syncwarp();  // the table is rewritten for the next token
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int heads = P.heads[t];
-      const bool normed = kNorm && P.w[t] != nullptr;
-      const uint16_t* xp = P.x[t] + token * P.x_tok[t] + sub * 8;
-      const uint16_t* gp = kBackward ? P.dy[t] + token * P.dy_tok[t] + sub * 8 : nullptr;
-      uint16_t* op = P.out[t] + static_cast<long long>(token) * heads * kHeadDim + sub * 8;
-#pragma unroll 4
-      for (int h0 = 2 * split; h0 < heads; h0 += 2 * P.splits) {  // the same trips for all lanes
-        const int h = h0 + half;
-        const bool active = h < heads;
-        uint4 raw = make_uint4(0, 0, 0, 0), xraw = make_uint4(0, 0, 0, 0);
-        if constexpr (kBackward) {
-          if (active) raw = load16(gp + h * P.dy_head[t]);
-          if (normed && active) xraw = load16(xp + h * P.x_head[t]);
-        } else {
-          if (active) raw = load16(xp + h * P.x_head[t]);
+      for (int n = 0; n < kAhead; ++n) {
+        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 2 * (trip - (t ? q_trips : 0)) + half;
+        raw[n] = xraw[n] = make_uint4(0, 0, 0, 0);
+        if (trip < trips && h < P.heads[t]) {
+          const uint16_t* xp = P.x[t] + token * P.x_tok[t] + h * P.x_head[t] + sub * 8;
+          if constexpr (kBackward) {
+            raw[n] = load16(P.dy[t] + token * P.dy_tok[t] + h * P.dy_head[t] + sub * 8);
+            if (kNorm && P.w[t] != nullptr) xraw[n] = load16(xp);
+          } else {
+            raw[n] = load16(xp);
+          }
         }
+      }
+      if (fresh) {  // behind the first loads, which it hides
+        fresh = false;
+        warp_rotation(P, turns, token, lane, tables[warp]);
+#pragma unroll
+        for (int i = 0; i < (kInterleaved ? 4 : 8); ++i) {
+          const float2 e = tables[warp][kInterleaved ? sub * 4 + i : (sub & 7) * 8 + i];
+          c[i] = e.x;
+          s[i] = e.y;
+        }
+        __syncwarp();  // the table is rewritten for the next token
+      }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 2 * (trip - (t ? q_trips : 0)) + half;
+        if (trip >= trips) break;  // the whole warp
+        const bool active = h < P.heads[t], normed = kNorm && P.w[t] != nullptr;
         float f[8];
-        unpack8(raw, f);
+        unpack8(raw[n], f);
         if constexpr (!kBackward) {
           if (normed) {
             float sq = 0.f;
@@ -182,31 +208,37 @@ __global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryP
             for (int i = 0; i < 8; ++i) sq += f[i] * f[i];
             const float rstd = rsqrtf(half_warp_sum(sq) * (1.f / kHeadDim) + P.eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * w[t][i];
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * (t ? w[1][i] : w[0][i]);
           }
           rotate8<kInterleaved>(f, c, s, upper, 1.f);
         } else {
           rotate8<kInterleaved>(f, c, s, upper, -1.f);
           if (normed) {
-            // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n))
+            // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n)).
+            // Rows that do not exist hold zeros and add nothing.
             float x[8], sq = 0.f, dot = 0.f;
-            unpack8(xraw, x);
+            unpack8(xraw[n], x);
+            float g[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+              g[i] = f[i] * (t ? w[1][i] : w[0][i]);
               sq += x[i] * x[i];
-              dot += f[i] * w[t][i] * x[i];
+              dot += g[i] * x[i];
             }
             const float rstd = rsqrtf(half_warp_sum(sq) * (1.f / kHeadDim) + P.eps);
             const float mean = half_warp_sum(dot) * rstd * (1.f / kHeadDim);
+            if (t == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float n = x[i] * rstd;
-              if (active) dw[t][i] += f[i] * n;
-              f[i] = rstd * (f[i] * w[t][i] - n * mean);
+              for (int i = 0; i < 8; ++i) dw[0][i] += f[i] * (x[i] * rstd);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) dw[1][i] += f[i] * (x[i] * rstd);
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = rstd * (g[i] - x[i] * rstd * mean);
           }
         }
-        if (active) store16(op + h * kHeadDim, pack8(f));
+        if (active) store16(P.out[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8, pack8(f));
       }
     }
   }
@@ -329,14 +361,17 @@ __device__ __forceinline__ RowRange range_of(const NormParams& P, int row) {
   return s;
 }
 
+constexpr int kForwardAhead = 4, kBackwardAhead = 3;  // rows in flight, see norm_smem()
+
 template <int kVec>
 __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormParams P) {
   __shared__ float buf[2][64];
+  extern __shared__ uint4 ring[];  // every thread's own pieces: [row][x, branch][kVec][thread]
   const int warps = blockDim.x >> 5;
   const int row0 = blockIdx.x * P.chunk_rows, row1 = min(row0 + P.chunk_rows, P.tokens);
   const int vecs = P.hidden >> 3;
   const float inv_h = 1.f / P.hidden;
-  uint4 wt[kVec], gt[kVec], sc[kVec], sh[kVec], xv[kVec], bv[kVec];
+  uint4 wt[kVec], gt[kVec], sc[kVec], sh[kVec];
   bool on[kVec];
   int col[kVec];
 #pragma unroll
@@ -344,19 +379,24 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
     const int v = threadIdx.x + k * blockDim.x;
     on[k] = v < vecs;
     col[k] = v * 8;
-    wt[k] = gt[k] = sc[k] = sh[k] = xv[k] = bv[k] = make_uint4(0, 0, 0, 0);
+    wt[k] = gt[k] = sc[k] = sh[k] = make_uint4(0, 0, 0, 0);
     if (on[k] && P.weight != nullptr) wt[k] = load16(P.weight + col[k]);
   }
-  auto fetch = [&](int row) {
+  const uint32_t mine = smem_u32(ring) + threadIdx.x * 16, piece = blockDim.x * 16;
+  auto fetch = [&](int row) {  // a group per row, also when there is none left
+    if (row < row1) {
+      const uint32_t at = mine + (row % kForwardAhead) * 2 * kVec * piece;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      if (on[k]) {
-        const long long at = static_cast<long long>(row) * P.hidden + col[k];
-        xv[k] = load16(P.x + at);
-        if (P.branch != nullptr) bv[k] = load16(P.branch + at);
-      }
+      for (int k = 0; k < kVec; ++k)
+        if (on[k]) {
+          const long long from = static_cast<long long>(row) * P.hidden + col[k];
+          copy16_async(at + k * piece, P.x + from);
+          if (P.branch != nullptr) copy16_async(at + (kVec + k) * piece, P.branch + from);
+        }
+    }
+    copy_commit();
   };
-  if (row0 < row1) fetch(row0);
+  for (int i = 0; i < kForwardAhead; ++i) fetch(row0 + i);
   RowRange s{0, 0};
   int parity = 0;
   for (int row = row0; row < row1; ++row) {
@@ -375,18 +415,19 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
     }
     const bool padding = s.sample >= P.samples;
     float r[kVec][8];
+    copy_wait<kForwardAhead - 1>();
+    const uint32_t slot = mine + (row % kForwardAhead) * 2 * kVec * piece;
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      unpack8(xv[k], r[k]);
-      if (P.branch != nullptr && !(padding && P.gate != nullptr)) {
+      unpack8(on[k] ? shared16(slot + k * piece) : make_uint4(0, 0, 0, 0), r[k]);
+      if (on[k] && P.branch != nullptr && !(padding && P.gate != nullptr)) {
         float b[8], g[8];
-        unpack8(bv[k], b);
+        unpack8(shared16(slot + (kVec + k) * piece), b);
         unpack8(gt[k], g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[k][i] += P.gate != nullptr ? g[i] * b[i] : b[i];
       }
     }
-    if (row + 1 < row1) fetch(row + 1);
     float mean = 0.f;
     if (P.center) {
       float t[1] = {0.f};
@@ -409,6 +450,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
         }
     block_sum(t, buf[parity], warps);
     parity ^= 1;
+    fetch(row + kForwardAhead);  // this row's pieces are in registers
     const float rstd = rsqrtf(t[0] * inv_h + P.eps);
     if (threadIdx.x == 0 && P.rstd != nullptr) {
       P.rstd[row] = rstd;
@@ -442,11 +484,13 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
 template <int kVec, bool kMod>
 __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormParams P) {
   __shared__ float buf[2][64];
+  extern __shared__ uint4 ring[];  // every thread's own pieces: [row][r, dy, dr, branch][kVec][thread]
+  constexpr int kParts = kMod ? 4 : 3;
   const int warps = blockDim.x >> 5;
   const int row0 = blockIdx.x * P.chunk_rows, row1 = min(row0 + P.chunk_rows, P.tokens);
   const int vecs = P.hidden >> 3;
   const float inv_h = 1.f / P.hidden;
-  uint4 wt[kVec], gt[kVec], sc[kVec], rv[kVec], bv[kVec], yv[kVec], dv[kVec];
+  uint4 wt[kVec], gt[kVec], sc[kVec];
   float sa[kVec][8], dg[kVec][8], dh[kVec][8];
   bool on[kVec];
   int col[kVec];
@@ -461,20 +505,25 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
     const int v = threadIdx.x + k * blockDim.x;
     on[k] = v < vecs;
     col[k] = v * 8;
-    wt[k] = gt[k] = sc[k] = rv[k] = bv[k] = yv[k] = dv[k] = make_uint4(0, 0, 0, 0);
+    wt[k] = gt[k] = sc[k] = make_uint4(0, 0, 0, 0);
     if (on[k] && P.weight != nullptr) wt[k] = load16(P.weight + col[k]);
   }
   clear();
-  auto fetch = [&](int row) {
+  const uint32_t mine = smem_u32(ring) + threadIdx.x * 16, piece = blockDim.x * 16;
+  auto fetch = [&](int row) {  // a group per row, also when there is none left
+    if (row < row1) {
+      const uint32_t at = mine + (row % kBackwardAhead) * kParts * kVec * piece;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      if (on[k]) {
-        const long long at = static_cast<long long>(row) * P.hidden + col[k];
-        rv[k] = load16(P.x + at);
-        if (kMod && P.gate != nullptr) bv[k] = load16(P.branch + at);
-        if (P.dy != nullptr) yv[k] = load16(P.dy + at);
-        if (P.dr != nullptr) dv[k] = load16(P.dr + at);
-      }
+      for (int k = 0; k < kVec; ++k)
+        if (on[k]) {
+          const long long from = static_cast<long long>(row) * P.hidden + col[k];
+          copy16_async(at + k * piece, P.x + from);
+          if (P.dy != nullptr) copy16_async(at + (kVec + k) * piece, P.dy + from);
+          if (P.dr != nullptr) copy16_async(at + (2 * kVec + k) * piece, P.dr + from);
+          if (kMod && P.gate != nullptr) copy16_async(at + (3 * kVec + k) * piece, P.branch + from);
+        }
+    }
+    copy_commit();
   };
   // Leaves the sums of the rows of `sample` behind. `fresh`: the first flush of this block.
   auto flush = [&](int sample, bool fresh) {
@@ -504,7 +553,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
       }
     clear();
   };
-  if (row0 < row1) fetch(row0);
+  for (int i = 0; i < kBackwardAhead; ++i) fetch(row0 + i);
   RowRange s{P.samples, 0};
   int parity = 0;
   bool fresh = true;
@@ -528,18 +577,17 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
     const bool padding = s.sample >= P.samples;
     const float rstd = __ldg(P.rstd + row), mean = P.mean != nullptr ? __ldg(P.mean + row) : 0.f;
     float n[kVec][8], dn[kVec][8];
-    uint4 b0[kVec], d0[kVec];
     float t[2] = {0.f, 0.f};
+    copy_wait<kBackwardAhead - 1>();
+    const uint32_t slot = mine + (row % kBackwardAhead) * kParts * kVec * piece;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      b0[k] = bv[k];
-      d0[k] = dv[k];
-      float w[8], a[8];
-      unpack8(rv[k], n[k]);
-      unpack8(yv[k], dn[k]);
-      unpack8(wt[k], w);
-      unpack8(sc[k], a);
-      if (!padding && on[k])
+    for (int k = 0; k < kVec; ++k)
+      if (!padding && on[k]) {
+        float w[8], a[8];
+        unpack8(shared16(slot + k * piece), n[k]);
+        unpack8(P.dy != nullptr ? shared16(slot + (kVec + k) * piece) : make_uint4(0, 0, 0, 0), dn[k]);
+        unpack8(wt[k], w);
+        unpack8(sc[k], a);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           n[k][i] = (n[k][i] - mean) * rstd;
@@ -550,8 +598,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
           t[0] += dn[k][i] * n[k][i];
           t[1] += dn[k][i];
         }
-    }
-    if (row + 1 < row1) fetch(row + 1);
+      }
     block_sum(t, buf[parity], warps);
     parity ^= 1;
     const float dot = t[0] * inv_h, avg = P.center ? t[1] * inv_h : 0.f;
@@ -560,14 +607,14 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
       if (on[k]) {
         const long long at = static_cast<long long>(row) * P.hidden + col[k];
         float d[8];
-        unpack8(d0[k], d);
+        unpack8(P.dr != nullptr ? shared16(slot + (2 * kVec + k) * piece) : make_uint4(0, 0, 0, 0), d);
         if (!padding)
 #pragma unroll
           for (int i = 0; i < 8; ++i) d[i] += rstd * (dn[k][i] - avg - n[k][i] * dot);
         store16(P.dx + at, pack8(d));
         if (kMod && P.dbranch != nullptr) {
           float b[8], g[8];
-          unpack8(b0[k], b);
+          unpack8(shared16(slot + (3 * kVec + k) * piece), b);
           unpack8(gt[k], g);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -577,6 +624,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
           store16(P.dbranch + at, pack8(g));
         }
       }
+    fetch(row + kBackwardAhead);  // what it overwrites this thread has read and used
   }
   if (row0 < row1) {
     if (s.sample < P.samples) {
@@ -591,8 +639,11 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Rows a norm block walks: two resident blocks on every SM share the rows evenly; at least one row.
-int norm_chunk_rows(long long tokens, int sms) { return static_cast<int>(ceil_div(tokens, 2ll * sms)); }
+// Rows a norm block walks: the blocks that are resident at once (four on an SM up to 1024 columns, else
+// two) share the rows evenly; at least one row.
+int norm_chunk_rows(long long tokens, int hidden, int sms) {
+  return static_cast<int>(ceil_div(tokens, (hidden <= 1024 ? 4ll : 2ll) * sms));
+}
 
 struct NormShape {
   int vec, threads;
@@ -602,6 +653,16 @@ struct NormShape {
 NormShape norm_shape(int hidden) {
   const int vecs = hidden / 8, vec = hidden <= 2048 ? 1 : 2;
   return {vec, static_cast<int>(ceil_div(ceil_div(vecs, vec), 32) * 32)};
+}
+
+// Bytes of the rows in flight: `ahead` rows of `parts` tensors, 16 bytes a thread and vector.
+uint32_t norm_smem(NormShape s, int ahead, int parts) { return 16u * s.vec * s.threads * ahead * parts; }
+
+int run_norm(void (*kernel)(NormParams), int grid, NormShape shape, uint32_t smem, const NormParams& P, cudaStream_t st) {
+  if (smem > 40 * 1024)  // beside the static arrays, 48 KiB need no leave
+    FGA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<grid, shape.threads, smem, st>>>(P);
+  return kSuccess;
 }
 
 int rotary_grid(long long units, bool sums, int sms) {
@@ -711,7 +772,7 @@ int check_norm(const FgaNorm* a, NormParams& P) {
   P.tokens = static_cast<int>(a->tokens);
   P.hidden = a->hidden;
   P.samples = a->samples;
-  P.chunk_rows = norm_chunk_rows(a->tokens, sm_count());
+  P.chunk_rows = norm_chunk_rows(a->tokens, a->hidden, sm_count());
   return kSuccess;
 }
 
@@ -773,17 +834,17 @@ int fga_norm_forward(const FgaNorm* args, void* stream) {
   const NormShape shape = norm_shape(P.hidden);
   const int grid = static_cast<int>(ceil_div(P.tokens, P.chunk_rows));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (shape.vec == 1)
-    norm_forward_kernel<1><<<grid, shape.threads, 0, st>>>(P);
-  else
-    norm_forward_kernel<2><<<grid, shape.threads, 0, st>>>(P);
+  const uint32_t smem = norm_smem(shape, kForwardAhead, 2);
+  const int rc2 = shape.vec == 1 ? run_norm(norm_forward_kernel<1>, grid, shape, smem, P, st)
+                                 : run_norm(norm_forward_kernel<2>, grid, shape, smem, P, st);
+  if (rc2 != kSuccess) return rc2;
   FGA_LAUNCHED();
   return kSuccess;
 }
 
 int64_t fga_norm_scratch_floats(int64_t tokens, int hidden, int samples, int has_weight, int modulated) {
   if (tokens < 1 || hidden < 1 || samples < 1) return 0;
-  const int64_t chunks = ceil_div(tokens, norm_chunk_rows(tokens, sm_count()));
+  const int64_t chunks = ceil_div(tokens, norm_chunk_rows(tokens, hidden, sm_count()));
   return (has_weight ? chunks * hidden : 0) + (modulated ? (chunks + samples) * 3 * hidden : 0);
 }
 
@@ -804,13 +865,14 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = static_cast<int>(chunks);
   const bool mod = P.gate || P.scale || modulated;
-  if (shape.vec == 1) {
-    if (mod) norm_backward_kernel<1, true><<<grid, shape.threads, 0, st>>>(P);
-    else norm_backward_kernel<1, false><<<grid, shape.threads, 0, st>>>(P);
-  } else {
-    if (mod) norm_backward_kernel<2, true><<<grid, shape.threads, 0, st>>>(P);
-    else norm_backward_kernel<2, false><<<grid, shape.threads, 0, st>>>(P);
-  }
+  const uint32_t smem = norm_smem(shape, kBackwardAhead, mod ? 4 : 3);
+  if (shape.vec == 1)
+    rc = mod ? run_norm(norm_backward_kernel<1, true>, grid, shape, smem, P, st)
+             : run_norm(norm_backward_kernel<1, false>, grid, shape, smem, P, st);
+  else
+    rc = mod ? run_norm(norm_backward_kernel<2, true>, grid, shape, smem, P, st)
+             : run_norm(norm_backward_kernel<2, false>, grid, shape, smem, P, st);
+  if (rc != kSuccess) return rc;
   FGA_LAUNCHED();
   const int blocks = static_cast<int>(ceil_div(P.hidden, 32));
   if (args->dweight != nullptr) {

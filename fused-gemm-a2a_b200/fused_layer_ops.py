@@ -41,11 +41,31 @@ def _same_device(first, *others):
 
 def _launch(entry, args, device):
     """Call a libfga entry point on the current stream of `device`, whichever device is current."""
-    if torch.cuda.current_device() == device.index:
-        _native.check(entry(byref(args), torch.cuda.current_stream().cuda_stream))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = entry(byref(args), torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            _native.check(rc)
         return
     with torch.cuda.device(device):
-        _native.check(entry(byref(args), torch.cuda.current_stream().cuda_stream))
+        _native.check(entry(byref(args), torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _floats(entry, device, *sizes):
+    """FP32 scratch of the size the library asks for on `device`."""
+    if torch.cuda.current_device() == device.index:
+        return torch.empty(entry(*sizes), device=device, dtype=torch.float32)
+    with torch.cuda.device(device):
+        return torch.empty(entry(*sizes), device=device, dtype=torch.float32)
+
+
+def _fresh(t):
+    """Contiguous, uninitialised storage for a tensor like `t`."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _differentiable(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _head_tensor(t, label):
@@ -138,15 +158,19 @@ def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale):
     return args
 
 
+def _attend(q, k, v, cu_seqlens, causal, scale):
+    tokens, heads, _ = q.shape
+    o = _fresh(q)
+    lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32)
+    if tokens:
+        _launch(_native.lib().fga_attention_forward, _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale), q.device)
+    return o, lse
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, causal, scale):
-        tokens, heads, _ = q.shape
-        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32)
-        if tokens:
-            _launch(_native.lib().fga_attention_forward, _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale),
-                    q.device)
+        o, lse = _attend(q, k, v, cu_seqlens, causal, scale)
         ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
         ctx.rule = (causal, scale)
         ctx.mark_non_differentiable(lse)
@@ -159,7 +183,7 @@ class _Attention(torch.autograd.Function):
             return (None,) * 6
         q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
         d_o = _grad_rows(d_o, o.shape)
-        grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
+        grads = [_fresh(t) for t in (q, k, v)]
         if q.shape[0]:
             delta = torch.empty_like(lse)
             args = _attention_args(q, k, v, o, lse, cu_seqlens, *ctx.rule)
@@ -200,7 +224,8 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
         if cu_seqlens.shape[0] > 65536:
             raise ValueError('at most 65535 packed sequences')
     _same_device(q, k, v, cu_seqlens)
-    o, lse = _Attention.apply(q, k, v, cu_seqlens, bool(causal), scale)
+    attend = _Attention.apply if _differentiable(q, k, v) else _attend
+    o, lse = attend(q, k, v, cu_seqlens, bool(causal), scale)
     return (o, lse) if return_lse else o
 
 
@@ -224,14 +249,18 @@ def _rotary_args(xs, outs, weights, positions, inv_freq, sections, interleaved, 
     return args
 
 
+def _rotate(q, k, q_weight, k_weight, positions, inv_freq, sections, interleaved, eps):
+    outs = _fresh(q), _fresh(k)
+    if q.shape[0]:
+        _launch(_native.lib().fga_rotary_forward,
+                _rotary_args((q, k), outs, (q_weight, k_weight), positions, inv_freq, sections, interleaved, eps), q.device)
+    return outs
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, sections, interleaved, eps):
-        outs = tuple(torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
-        if q.shape[0]:
-            _launch(_native.lib().fga_rotary_forward,
-                    _rotary_args((q, k), outs, (q_weight, k_weight), positions, inv_freq, sections, interleaved, eps),
-                    q.device)
+        outs = _rotate(q, k, q_weight, k_weight, positions, inv_freq, sections, interleaved, eps)
         # without a head norm the rotation's gradient does not need its input
         ctx.save_for_backward(q if q_weight is not None else None, k if k_weight is not None else None, q_weight,
                               k_weight, positions, inv_freq)
@@ -244,7 +273,7 @@ class _Rotary(torch.autograd.Function):
         q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
         sections, interleaved, eps = ctx.rule
         grads = [_grad_rows(g, shape) for g, shape in zip((dq_out, dk_out), ctx.shapes)]
-        outs = [torch.empty(shape, device=positions.device, dtype=torch.bfloat16) for shape in ctx.shapes]
+        outs = [_fresh(g) for g in grads]
         targets = [_weight_target(w, needed) for w, needed in zip(ctx.owners, ctx.needs_input_grad[2:4])]
         tokens = outs[0].shape[0]
         if tokens:
@@ -256,9 +285,7 @@ class _Rotary(torch.autograd.Function):
                 args.dweight_f32[t] = target is not None and target.dtype == torch.float32
                 args.dweight_accumulate[t] = accumulate
             if q_weight is not None or k_weight is not None:
-                with torch.cuda.device(positions.device):
-                    floats = lib.fga_rotary_scratch_floats(tokens, args.heads[0], args.heads[1])
-                scratch = torch.empty(floats, device=positions.device, dtype=torch.float32)
+                scratch = _floats(lib.fga_rotary_scratch_floats, positions.device, tokens, args.heads[0], args.heads[1])
                 args.scratch = scratch.data_ptr()
             _launch(lib.fga_rotary_backward, args, positions.device)
         else:
@@ -301,34 +328,37 @@ def rotary_embedding(q, k, positions, inv_freq, sections=None, *, interleaved=Tr
     _vector(q_weight, HEAD_DIM, 'q_weight')
     _vector(k_weight, HEAD_DIM, 'k_weight')
     _same_device(q, k, positions, inv_freq, q_weight, k_weight)
-    return _Rotary.apply(q, k, q_weight, k_weight, positions, inv_freq, sections, bool(interleaved), float(eps))
+    rotate = _Rotary.apply if _differentiable(q, k, q_weight, k_weight) else _rotate
+    return rotate(q, k, q_weight, k_weight, positions, inv_freq, sections, bool(interleaved), float(eps))
 
 
 # ----------------------------------------------------------------------------------------------
 # Norm around a block
 # ----------------------------------------------------------------------------------------------
+def _normalise(x, branch, weight, gate, scale, shift, cu_seqlens, samples, eps, center, rstd=None, mean=None):
+    tokens, hidden = x.shape
+    y = torch.empty_like(x)
+    r = None if branch is None else torch.empty_like(x)
+    if tokens:
+        args = _native.FgaNorm(_address(x), _address(branch), _address(weight), _address(gate), _address(scale),
+                               _address(shift), _address(cu_seqlens), _address(y), _address(r), _address(rstd),
+                               _address(mean))
+        args.tokens, args.hidden, args.samples, args.center, args.eps = tokens, hidden, samples, center, eps
+        _launch(_native.lib().fga_norm_forward, args, x.device)
+    return y, x if r is None else r
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, weight, gate, scale, shift, cu_seqlens, samples, eps, center):
-        tokens, hidden = x.shape
-        keep = any(ctx.needs_input_grad)
-        y = torch.empty_like(x)
-        r = None if branch is None else torch.empty_like(x)
-        rstd = torch.empty(tokens, device=x.device, dtype=torch.float32) if keep else None
-        mean = torch.empty(tokens, device=x.device, dtype=torch.float32) if keep and center else None
-        if tokens:
-            args = _native.FgaNorm(_address(x), _address(branch), _address(weight), _address(gate), _address(scale),
-                                   _address(shift), _address(cu_seqlens), _address(y), _address(r), _address(rstd),
-                                   _address(mean))
-            args.tokens, args.hidden, args.samples, args.center, args.eps = tokens, hidden, samples, center, eps
-            _launch(_native.lib().fga_norm_forward, args, x.device)
+        rstd = torch.empty(x.shape[0], device=x.device, dtype=torch.float32)
+        mean = torch.empty_like(rstd) if center else None
+        y, r = _normalise(x, branch, weight, gate, scale, shift, cu_seqlens, samples, eps, center, rstd, mean)
         ctx.set_materialize_grads(False)
-        if keep:
-            ctx.save_for_backward(x if r is None else r, branch if gate is not None else None, weight, gate, scale,
-                                  cu_seqlens, rstd, mean)
+        ctx.save_for_backward(r, branch if gate is not None else None, weight, gate, scale, cu_seqlens, rstd, mean)
         ctx.owner, ctx.has_branch, ctx.has_shift = weight, branch is not None, shift is not None
         ctx.rule = (samples, eps, center)
-        return y, x if r is None else r
+        return y, r
 
     @staticmethod
     def backward(ctx, dy, dr):
@@ -348,9 +378,8 @@ class _ResidualNorm(torch.autograd.Function):
             modulated = any(t is not None for t in rows)
             scratch = None
             if target is not None or modulated:
-                with torch.cuda.device(r.device):
-                    floats = lib.fga_norm_scratch_floats(tokens, hidden, samples, target is not None, modulated)
-                scratch = torch.empty(floats, device=r.device, dtype=torch.float32)
+                scratch = _floats(lib.fga_norm_scratch_floats, r.device, tokens, hidden, samples, target is not None,
+                                  modulated)
             args = _native.FgaNorm(None, _address(branch), _address(weight), _address(gate), _address(scale), None,
                                    _address(cu_seqlens), None, _address(r), _address(rstd), _address(mean),
                                    _address(dy), _address(dr), _address(dx), _address(dbranch), _address(target),
@@ -405,4 +434,5 @@ def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=N
             raise ValueError(f'{label} must be a contiguous, 16-byte aligned BF16 tensor [{samples}, {hidden}]')
         rows.append(t)
     _same_device(x, branch, weight, cu_seqlens, *rows)
-    return _ResidualNorm.apply(x, branch, weight, *rows, cu_seqlens, samples, float(eps), bool(center))
+    normalise = _ResidualNorm.apply if _differentiable(x, branch, weight, *rows) else _normalise
+    return normalise(x, branch, weight, *rows, cu_seqlens, samples, float(eps), bool(center))
