@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include "../../include/fga.h"
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "ptx.cuh"
 #include "seq_bounds.cuh"
 
@@ -18,23 +19,14 @@ namespace {
 
 constexpr int kHeadDim = 128;
 
-__device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = lo_f32(w[i]);
-    f[2 * i + 1] = hi_f32(w[i]);
-  }
+__device__ __forceinline__ void unpack8(uint4 v, F2 (&f)[4]) {
+  f[0] = f2_of_bf16(v.x);
+  f[1] = f2_of_bf16(v.y);
+  f[2] = f2_of_bf16(v.z);
+  f[3] = f2_of_bf16(v.w);
 }
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+__device__ __forceinline__ uint4 pack8(const F2 (&f)[4]) {
+  return make_uint4(bf16_of_f2(f[0]), bf16_of_f2(f[1]), bf16_of_f2(f[2]), bf16_of_f2(f[3]));
 }
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 __device__ __forceinline__ void store16(uint16_t* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
@@ -65,16 +57,20 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
 // become a float: the error is below 2^-25 turns at every position below 2^31.
 //
 // Mapping: one warp per token (several when tokens are few), which computes the token's 64 sines and
-// cosines once for all heads; a half-warp holds one head row, 8 elements a lane.
+// cosines once for all heads. Eight lanes hold a head row, each 8 elements of its lower and 8 of its upper
+// half, so both kinds of pairs turn inside a lane; a warp takes four head rows at a time. The first version
+// (16 lanes a row, scalar arithmetic) issued 870 instructions per token of 8 heads and was bound by that, at
+// 3.7 TB/s.
 // =============================================================================================
 constexpr int kRotaryWarps = 8;
 
 struct RotaryParams {
   const uint16_t* x[2];       // forward: inputs; backward: the forward's inputs (only read where w is set)
-  const uint16_t* dy[2];      // backward: incoming gradients
-  uint16_t* out[2];           // forward: outputs; backward: gradients of x
+  const uint16_t* dy[2];      // backward: incoming gradients, contiguous
+  uint16_t* out[2];           // forward: outputs; backward: gradients of x; contiguous
   const uint16_t* w[2];       // [128] or null
-  long long x_tok[2], x_head[2], dy_tok[2], dy_head[2];  // strides in elements; out is contiguous
+  long long x_tok[2];         // strides in elements
+  int x_head[2];
   int heads[2];
   const void* pos;            // [tokens, axes]
   int pos64;
@@ -88,157 +84,198 @@ struct RotaryParams {
   float* partial;             // backward with weights: [grid][2][128]
 };
 
-__device__ __forceinline__ void warp_rotation(const RotaryParams& P, const unsigned long long* turns, int token, int lane,
-                                              float2* table) {
+// A lane's share of the angles: pairs lane and lane + 32.
+struct LaneAngle {
+  unsigned long long turns[2];  // 2^-64 turns per position
+  int axis[2];
+};
+__device__ __forceinline__ LaneAngle lane_angle(const RotaryParams& P, int lane) {
+  LaneAngle a;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int pair = lane + 32 * i;
-    int axis = 0;
-    while (axis + 1 < P.axes && pair >= P.ends[axis]) ++axis;
-    const long long at = static_cast<long long>(token) * P.axes + axis;
+    const double f = P.freq64 ? __ldg(static_cast<const double*>(P.freq) + pair)
+                              : static_cast<double>(__ldg(static_cast<const float*>(P.freq) + pair));
+    const double t = f * 0.15915494309189533577;  // turns per position
+    a.turns[i] = static_cast<unsigned long long>((t - floor(t)) * 18446744073709551616.0);
+    a.axis[i] = (P.axes > 1 && pair >= P.ends[0]) + (P.axes > 2 && pair >= P.ends[1]) + (P.axes > 3 && pair >= P.ends[2]);
+  }
+  return a;
+}
+__device__ __forceinline__ void warp_rotation(const RotaryParams& P, const LaneAngle& a, int token, int lane,
+                                              float* cosines, float* sines) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const long long at = static_cast<long long>(token) * P.axes + a.axis[i];
     const long long pos = P.pos64 ? __ldg(static_cast<const long long*>(P.pos) + at)
                                   : static_cast<long long>(__ldg(static_cast<const int*>(P.pos) + at));
-    const unsigned long long phase = turns[pair] * static_cast<unsigned long long>(pos);
+    const unsigned long long phase = a.turns[i] * static_cast<unsigned long long>(pos);
     // top 32 bits as a signed fraction of a turn; sincospi takes half turns
     const float half_turns = static_cast<float>(static_cast<int>(phase >> 32)) * 4.656612873077393e-10f;  // 2^-31
     float s, c;
     sincospif(half_turns, &s, &c);
-    table[pair] = make_float2(c, s);
+    cosines[lane + 32 * i] = c;
+    sines[lane + 32 * i] = s;
   }
   __syncwarp();
 }
 
-// Rotation of a lane's 8 elements; `sign` -1 turns back. Half-split rows exchange their halves between
-// lanes l and l ^ 8.
+// Turns a lane's 16 elements (f[0..3] from the lower half of the head, f[4..7] from the upper). Interleaved:
+// pair i of f is (lo, hi) of f[i], with cosine c[i>>1] half i&1. Half-split: f[i] turns with f[i + 4], with
+// cosines c[i].
 template <bool kInterleaved>
-__device__ __forceinline__ void rotate8(float (&f)[8], const float (&c)[8], const float (&s)[8], bool upper, float sign) {
+__device__ __forceinline__ void rotate16(F2 (&f)[8], const F2 (&c)[4], const F2 (&s)[4]) {
   if constexpr (kInterleaved) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = f[2 * i], b = f[2 * i + 1], sn = sign * s[i];
-      f[2 * i] = a * c[i] - b * sn;
-      f[2 * i + 1] = b * c[i] + a * sn;
+    for (int i = 0; i < 8; ++i) {
+      float a, b, c0, c1, s0, s1;
+      split(f[i], a, b);
+      split(c[i >> 1], c0, c1);
+      split(s[i >> 1], s0, s1);
+      const float cc = i & 1 ? c1 : c0, ss = i & 1 ? s1 : s0;
+      f[i] = f2(a * cc - b * ss, b * cc + a * ss);
     }
   } else {
-    const float flip = upper ? sign : -sign;
+    const F2 minus = f2(-1.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, f[i], 8);
-      f[i] = f[i] * c[i] + other * (flip * s[i]);
+    for (int i = 0; i < 4; ++i) {
+      const F2 a = f[i], b = f[i + 4];
+      f[i] = fma2(b * minus, s[i], a * c[i]);
+      f[i + 4] = fma2(a, s[i], b * c[i]);
     }
   }
 }
 
-__device__ __forceinline__ float half_warp_sum(float v) {
+__device__ __forceinline__ float eight_lane_sum(float v) {
 #pragma unroll
-  for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+__device__ __forceinline__ void unpack16(uint4 lower, uint4 upper, F2 (&f)[8]) {
+  F2 a[4], b[4];
+  unpack8(lower, a);
+  unpack8(upper, b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = a[i];
+    f[i + 4] = b[i];
+  }
 }
 
 template <bool kInterleaved, bool kBackward, bool kNorm>
-__global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryParams P) {
-  __shared__ unsigned long long turns[64];
-  __shared__ float2 tables[kRotaryWarps][64];
+__global__ void __launch_bounds__(32 * kRotaryWarps, kNorm ? 2 : 3) rotary_kernel(const RotaryParams P) {
+  __shared__ float tables[kRotaryWarps][2][64];
   __shared__ float reduce[kBackward && kNorm ? kRotaryWarps : 1][2][kHeadDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x < 64) {
-    const double f = P.freq64 ? __ldg(static_cast<const double*>(P.freq) + threadIdx.x)
-                              : static_cast<double>(__ldg(static_cast<const float*>(P.freq) + threadIdx.x));
-    const double t = f * 0.15915494309189533577;  // turns per position
-    turns[threadIdx.x] = static_cast<unsigned long long>((t - floor(t)) * 18446744073709551616.0);
-  }
-  __syncthreads();
-  const int sub = lane & 15, half = lane >> 4;
-  const bool upper = sub >= 8;
-  float w[2][8];
-  float dw[2][8];
+  const int sub = lane & 7, quarter = lane >> 3;
+  const LaneAngle angle = lane_angle(P, lane);
+  uint4 w[2][2];
+  F2 dw[2][8];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[t][i] = 0.f;
-    if (kNorm && P.w[t] != nullptr) unpack8(load16(P.w[t] + sub * 8), w[t]);
+    for (int i = 0; i < 8; ++i) dw[t][i] = f2(0.f);
+    if (kNorm && P.w[t] != nullptr) {
+      w[t][0] = load16(P.w[t] + sub * 8);
+      w[t][1] = load16(P.w[t] + 64 + sub * 8);
+    }
   }
-  // A trip takes two head rows of q, or two of k, so the weight is the same for a whole warp. The loads of
-  // four trips are in flight before the first is used.
-  constexpr int kAhead = 4;
+  // A trip takes four head rows of q, or four of k, so the weight is the same for a whole warp. Four 16-byte
+  // loads of a lane are in flight before the first is used: two trips, or one that reads two tensors.
+  constexpr int kAhead = kBackward && kNorm ? 1 : 2;
   const int units = P.tokens * P.splits;  // below 2^31: there is more than one split only with few tokens
-  const int q_trips = (P.heads[0] + 1) >> 1, trips = q_trips + ((P.heads[1] + 1) >> 1);
+  const int q_trips = (P.heads[0] + 3) >> 2, trips = q_trips + ((P.heads[1] + 3) >> 2);
   for (int u = blockIdx.x * kRotaryWarps + warp; u < units; u += gridDim.x * kRotaryWarps) {
-    const int token = P.splits == 1 ? u : u / P.splits, split = u - token * P.splits;
+    const int token = P.splits == 1 ? u : u / P.splits, split_at = u - token * P.splits;
     bool fresh = true;
-    float c[8], s[8];
-    for (int trip0 = split; trip0 < trips; trip0 += kAhead * P.splits) {
-      uint4 raw[kAhead], xraw[kAhead];
+    F2 c[4], s[4];
+    for (int trip0 = split_at; trip0 < trips; trip0 += kAhead * P.splits) {
+      uint4 raw[kAhead][2], xraw[kAhead][2];
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) {
-        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 2 * (trip - (t ? q_trips : 0)) + half;
-        raw[n] = xraw[n] = make_uint4(0, 0, 0, 0);
+        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 4 * (trip - (t ? q_trips : 0)) + quarter;
+        raw[n][0] = raw[n][1] = xraw[n][0] = xraw[n][1] = make_uint4(0, 0, 0, 0);
         if (trip < trips && h < P.heads[t]) {
-          const uint16_t* xp = P.x[t] + token * P.x_tok[t] + h * P.x_head[t] + sub * 8;
+          const uint16_t* xp = P.x[t] + token * P.x_tok[t] + static_cast<long long>(h) * P.x_head[t] + sub * 8;
           if constexpr (kBackward) {
-            raw[n] = load16(P.dy[t] + token * P.dy_tok[t] + h * P.dy_head[t] + sub * 8);
-            if (kNorm && P.w[t] != nullptr) xraw[n] = load16(xp);
+            const uint16_t* gp = P.dy[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8;
+            raw[n][0] = load16(gp);
+            raw[n][1] = load16(gp + 64);
+            if (kNorm && P.w[t] != nullptr) {
+              xraw[n][0] = load16(xp);
+              xraw[n][1] = load16(xp + 64);
+            }
           } else {
-            raw[n] = load16(xp);
+            raw[n][0] = load16(xp);
+            raw[n][1] = load16(xp + 64);
           }
         }
       }
       if (fresh) {  // behind the first loads, which it hides
         fresh = false;
-        warp_rotation(P, turns, token, lane, tables[warp]);
+        float *ct = tables[warp][0], *st = tables[warp][1];
+        warp_rotation(P, angle, token, lane, ct, st);
 #pragma unroll
-        for (int i = 0; i < (kInterleaved ? 4 : 8); ++i) {
-          const float2 e = tables[warp][kInterleaved ? sub * 4 + i : (sub & 7) * 8 + i];
-          c[i] = e.x;
-          s[i] = e.y;
+        for (int i = 0; i < 4; ++i) {
+          // interleaved: pairs sub*4 .. +3 of the lower half, 32 + sub*4 .. +3 of the upper; else sub*8 .. +7
+          const int at = kInterleaved ? sub * 4 + (i & 1) * 2 + (i >> 1) * 32 : sub * 8 + 2 * i;
+          c[i] = f2(ct[at], ct[at + 1]);
+          s[i] = kBackward ? f2(-st[at], -st[at + 1]) : f2(st[at], st[at + 1]);
         }
         __syncwarp();  // the table is rewritten for the next token
       }
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) {
-        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 2 * (trip - (t ? q_trips : 0)) + half;
+        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 4 * (trip - (t ? q_trips : 0)) + quarter;
         if (trip >= trips) break;  // the whole warp
         const bool active = h < P.heads[t], normed = kNorm && P.w[t] != nullptr;
-        float f[8];
-        unpack8(raw[n], f);
+        F2 f[8];
+        unpack16(raw[n][0], raw[n][1], f);
         if constexpr (!kBackward) {
           if (normed) {
-            float sq = 0.f;
+            F2 sq = f[0] * f[0], wt[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sq += f[i] * f[i];
-            const float rstd = rsqrtf(half_warp_sum(sq) * (1.f / kHeadDim) + P.eps);
+            for (int i = 1; i < 8; ++i) sq = fma2(f[i], f[i], sq);
+            unpack16(t ? w[1][0] : w[0][0], t ? w[1][1] : w[0][1], wt);
+            const F2 rstd = f2(rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * (t ? w[1][i] : w[0][i]);
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * wt[i];
           }
-          rotate8<kInterleaved>(f, c, s, upper, 1.f);
+          rotate16<kInterleaved>(f, c, s);
         } else {
-          rotate8<kInterleaved>(f, c, s, upper, -1.f);
+          rotate16<kInterleaved>(f, c, s);
           if (normed) {
             // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n)).
             // Rows that do not exist hold zeros and add nothing.
-            float x[8], sq = 0.f, dot = 0.f;
-            unpack8(xraw[n], x);
-            float g[8];
+            F2 x[8], g[8], sq = f2(0.f), dot = f2(0.f);
+            unpack16(xraw[n][0], xraw[n][1], x);
+            unpack16(t ? w[1][0] : w[0][0], t ? w[1][1] : w[0][1], g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              g[i] = f[i] * (t ? w[1][i] : w[0][i]);
-              sq += x[i] * x[i];
-              dot += g[i] * x[i];
+              g[i] = g[i] * f[i];
+              sq = fma2(x[i], x[i], sq);
+              dot = fma2(g[i], x[i], dot);
             }
-            const float rstd = rsqrtf(half_warp_sum(sq) * (1.f / kHeadDim) + P.eps);
-            const float mean = half_warp_sum(dot) * rstd * (1.f / kHeadDim);
+            const float rstd = rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps);
+            const F2 r = f2(rstd), mean = f2(-eight_lane_sum(sum(dot)) * rstd * (1.f / kHeadDim));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * r;
             if (t == 0) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) dw[0][i] += f[i] * (x[i] * rstd);
+              for (int i = 0; i < 8; ++i) dw[0][i] = fma2(f[i], x[i], dw[0][i]);
             } else {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) dw[1][i] += f[i] * (x[i] * rstd);
+              for (int i = 0; i < 8; ++i) dw[1][i] = fma2(f[i], x[i], dw[1][i]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = rstd * (g[i] - x[i] * rstd * mean);
+            for (int i = 0; i < 8; ++i) f[i] = r * fma2(x[i], mean, g[i]);
           }
         }
-        if (active) store16(P.out[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8, pack8(f));
+        if (active) {
+          uint16_t* op = P.out[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8;
+          store16(op, make_uint4(bf16_of_f2(f[0]), bf16_of_f2(f[1]), bf16_of_f2(f[2]), bf16_of_f2(f[3])));
+          store16(op + 64, make_uint4(bf16_of_f2(f[4]), bf16_of_f2(f[5]), bf16_of_f2(f[6]), bf16_of_f2(f[7])));
+        }
       }
     }
   }
@@ -247,8 +284,14 @@ __global__ void __launch_bounds__(32 * kRotaryWarps) rotary_kernel(const RotaryP
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float v = dw[t][i] + __shfl_xor_sync(0xffffffffu, dw[t][i], 16);
-        if (half == 0) reduce[warp][t][sub * 8 + i] = v;
+        float v[2];
+        split(dw[t][i], v[0], v[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          v[e] += __shfl_xor_sync(0xffffffffu, v[e], 8);
+          v[e] += __shfl_xor_sync(0xffffffffu, v[e], 16);
+          if (quarter == 0) reduce[warp][t][(i >> 2) * 64 + sub * 8 + 2 * (i & 3) + e] = v[e];
+        }
       }
     __syncthreads();
     const int t = threadIdx.x >> 7, col = threadIdx.x & 127;
@@ -414,40 +457,45 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
       }
     }
     const bool padding = s.sample >= P.samples;
-    float r[kVec][8];
+    F2 r[kVec][4];
     copy_wait<kForwardAhead - 1>();
     const uint32_t slot = mine + (row % kForwardAhead) * 2 * kVec * piece;
+    F2 total = f2(0.f);
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      unpack8(on[k] ? shared16(slot + k * piece) : make_uint4(0, 0, 0, 0), r[k]);
+      unpack8(on[k] ? shared16(slot + k * piece) : make_uint4(0, 0, 0, 0), r[k]);  // columns beyond the row hold zeros
       if (on[k] && P.branch != nullptr && !(padding && P.gate != nullptr)) {
-        float b[8], g[8];
+        F2 b[4], g[4];
         unpack8(shared16(slot + (kVec + k) * piece), b);
         unpack8(gt[k], g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[k][i] += P.gate != nullptr ? g[i] * b[i] : b[i];
+        for (int i = 0; i < 4; ++i) r[k][i] = P.gate != nullptr ? fma2(g[i], b[i], r[k][i]) : r[k][i] + b[i];
+        store16(P.r + static_cast<long long>(row) * P.hidden + col[k], pack8(r[k]));
+      } else if (on[k] && P.r != nullptr) {
+        store16(P.r + static_cast<long long>(row) * P.hidden + col[k], pack8(r[k]));
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total = total + r[k][i];
     }
     float mean = 0.f;
     if (P.center) {
-      float t[1] = {0.f};
-#pragma unroll
-      for (int k = 0; k < kVec; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t[0] += r[k][i];  // columns beyond the row hold zeros
+      float t[1] = {sum(total)};
       block_sum(t, buf[parity], warps);
       parity ^= 1;
       mean = t[0] * inv_h;
+      const F2 minus = f2(-mean);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        if (on[k])
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[k][i] = r[k][i] + minus;
     }
-    float t[1] = {0.f};
+    total = f2(0.f);
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
-      if (on[k])
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = r[k][i] - mean;
-          t[0] += d * d;
-        }
+      for (int i = 0; i < 4; ++i) total = fma2(r[k][i], r[k][i], total);
+    float t[1] = {sum(total)};
     block_sum(t, buf[parity], warps);
     parity ^= 1;
     fetch(row + kForwardAhead);  // this row's pieces are in registers
@@ -456,23 +504,29 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
       P.rstd[row] = rstd;
       if (P.mean != nullptr) P.mean[row] = mean;
     }
+    const F2 scaled = f2(rstd);
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
       if (on[k]) {
-        const long long at = static_cast<long long>(row) * P.hidden + col[k];
-        if (P.r != nullptr) store16(P.r + at, pack8(r[k]));
-        float y[8], w[8], a[8], b[8];
-        unpack8(wt[k], w);
-        unpack8(sc[k], a);
-        unpack8(sh[k], b);
+        F2 y[4], e[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y[i] = (r[k][i] - mean) * rstd;
-          if (P.weight != nullptr) y[i] *= w[i];
-          if (P.scale != nullptr) y[i] *= 1.f + a[i];
-          if (P.shift != nullptr) y[i] += b[i];
+        for (int i = 0; i < 4; ++i) y[i] = r[k][i] * scaled;
+        if (P.weight != nullptr) {
+          unpack8(wt[k], e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = y[i] * e[i];
         }
-        store16(P.y + at, padding ? make_uint4(0, 0, 0, 0) : pack8(y));
+        if (P.scale != nullptr) {
+          unpack8(sc[k], e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = fma2(y[i], e[i], y[i]);
+        }
+        if (P.shift != nullptr) {
+          unpack8(sh[k], e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = y[i] + e[i];
+        }
+        store16(P.y + static_cast<long long>(row) * P.hidden + col[k], padding ? make_uint4(0, 0, 0, 0) : pack8(y));
       }
   }
 }
@@ -491,14 +545,14 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
   const int vecs = P.hidden >> 3;
   const float inv_h = 1.f / P.hidden;
   uint4 wt[kVec], gt[kVec], sc[kVec];
-  float sa[kVec][8], dg[kVec][8], dh[kVec][8];
+  F2 sa[kVec][4], dg[kVec][4], dh[kVec][4];
   bool on[kVec];
   int col[kVec];
   auto clear = [&]() {
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sa[k][i] = dg[k][i] = dh[k][i] = 0.f;
+      for (int i = 0; i < 4; ++i) sa[k][i] = dg[k][i] = dh[k][i] = f2(0.f);
   };
 #pragma unroll
   for (int k = 0; k < kVec; ++k) {
@@ -530,25 +584,35 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
       if (on[k]) {
-        float w[8], a[8];
+        F2 w[4], a[4];
         unpack8(wt[k], w);
         unpack8(sc[k], a);
+        auto put = [&](float* at, const F2(&v)[4], bool add) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float4 o, *p = reinterpret_cast<float4*>(at) + i;
+            split(v[2 * i], o.x, o.y);
+            split(v[2 * i + 1], o.z, o.w);
+            if (add) {
+              const float4 q = *p;
+              o = make_float4(o.x + q.x, o.y + q.y, o.z + q.z, o.w + q.w);
+            }
+            *p = o;
+          }
+        };
+        F2 v[4];
         if (kMod && P.part_mod != nullptr) {
           float* base = P.part_mod + static_cast<long long>(blockIdx.x + sample) * 3 * P.hidden + col[k];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            base[i] = dg[k][i];
-            base[P.hidden + i] = P.weight != nullptr ? sa[k][i] * w[i] : sa[k][i];
-            base[2 * P.hidden + i] = dh[k][i];
-          }
+          for (int i = 0; i < 4; ++i) v[i] = P.weight != nullptr ? sa[k][i] * w[i] : sa[k][i];
+          put(base, dg[k], false);
+          put(base + P.hidden, v, false);
+          put(base + 2 * P.hidden, dh[k], false);
         }
         if (P.part_weight != nullptr) {
-          float* base = P.part_weight + static_cast<long long>(blockIdx.x) * P.hidden + col[k];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = kMod && P.scale != nullptr ? sa[k][i] * (1.f + a[i]) : sa[k][i];
-            base[i] = fresh ? v : base[i] + v;
-          }
+          for (int i = 0; i < 4; ++i) v[i] = kMod && P.scale != nullptr ? fma2(sa[k][i], a[i], sa[k][i]) : sa[k][i];
+          put(P.part_weight + static_cast<long long>(blockIdx.x) * P.hidden + col[k], v, !fresh);
         }
       }
     clear();
@@ -576,52 +640,62 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
     }
     const bool padding = s.sample >= P.samples;
     const float rstd = __ldg(P.rstd + row), mean = P.mean != nullptr ? __ldg(P.mean + row) : 0.f;
-    float n[kVec][8], dn[kVec][8];
-    float t[2] = {0.f, 0.f};
+    F2 n[kVec][4], dn[kVec][4], dot2 = f2(0.f), sum2 = f2(0.f);
     copy_wait<kBackwardAhead - 1>();
     const uint32_t slot = mine + (row % kBackwardAhead) * kParts * kVec * piece;
+    const F2 scaled = f2(rstd), offset = f2(-mean * rstd);
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
       if (!padding && on[k]) {
-        float w[8], a[8];
+        F2 e[4];
         unpack8(shared16(slot + k * piece), n[k]);
         unpack8(P.dy != nullptr ? shared16(slot + (kVec + k) * piece) : make_uint4(0, 0, 0, 0), dn[k]);
-        unpack8(wt[k], w);
-        unpack8(sc[k], a);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          n[k][i] = (n[k][i] - mean) * rstd;
-          sa[k][i] += dn[k][i] * n[k][i];
-          if (kMod) dh[k][i] += dn[k][i];
-          if (kMod && P.scale != nullptr) dn[k][i] *= 1.f + a[i];
-          if (P.weight != nullptr) dn[k][i] *= w[i];
-          t[0] += dn[k][i] * n[k][i];
-          t[1] += dn[k][i];
+        for (int i = 0; i < 4; ++i) {
+          n[k][i] = fma2(n[k][i], scaled, offset);
+          sa[k][i] = fma2(dn[k][i], n[k][i], sa[k][i]);
+          if (kMod) dh[k][i] = dh[k][i] + dn[k][i];
+        }
+        if (kMod && P.scale != nullptr) {
+          unpack8(sc[k], e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dn[k][i] = fma2(dn[k][i], e[i], dn[k][i]);
+        }
+        if (P.weight != nullptr) {
+          unpack8(wt[k], e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dn[k][i] = dn[k][i] * e[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dot2 = fma2(dn[k][i], n[k][i], dot2);
+          sum2 = sum2 + dn[k][i];
         }
       }
+    float t[2] = {sum(dot2), sum(sum2)};
     block_sum(t, buf[parity], warps);
     parity ^= 1;
-    const float dot = t[0] * inv_h, avg = P.center ? t[1] * inv_h : 0.f;
+    const F2 dot = f2(-t[0] * inv_h), avg = f2(P.center ? -t[1] * inv_h : 0.f);
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
       if (on[k]) {
         const long long at = static_cast<long long>(row) * P.hidden + col[k];
-        float d[8];
+        F2 d[4];
         unpack8(P.dr != nullptr ? shared16(slot + (2 * kVec + k) * piece) : make_uint4(0, 0, 0, 0), d);
         if (!padding)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] += rstd * (dn[k][i] - avg - n[k][i] * dot);
+          for (int i = 0; i < 4; ++i) d[i] = fma2(scaled, fma2(n[k][i], dot, dn[k][i] + avg), d[i]);
         store16(P.dx + at, pack8(d));
         if (kMod && P.dbranch != nullptr) {
-          float b[8], g[8];
+          F2 b[4], g[4];
           unpack8(shared16(slot + (3 * kVec + k) * piece), b);
           unpack8(gt[k], g);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (!padding) dg[k][i] += d[i] * b[i];
-            g[i] = padding ? 0.f : g[i] * d[i];
+          for (int i = 0; i < 4; ++i) {
+            if (!padding) dg[k][i] = fma2(d[i], b[i], dg[k][i]);
+            g[i] = g[i] * d[i];
           }
-          store16(P.dbranch + at, pack8(g));
+          store16(P.dbranch + at, padding ? make_uint4(0, 0, 0, 0) : pack8(g));
         }
       }
     fetch(row + kBackwardAhead);  // what it overwrites this thread has read and used
@@ -673,7 +747,7 @@ int rotary_grid(long long units, bool sums, int sms) {
 
 // Warps a token's heads are spread over: as many as it takes to give every SM 16 warps.
 int rotary_splits(long long tokens, int heads, int sms) {
-  const long long want = ceil_div(16ll * sms, tokens), most = (heads + 1) / 2;
+  const long long want = ceil_div(16ll * sms, tokens), most = (heads + 3) / 4;
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -726,9 +800,8 @@ int check_rotary(const FgaRotary* a, bool backward, RotaryParams& P) {
     P.out[t] = static_cast<uint16_t*>(a->out[t]);
     P.w[t] = static_cast<const uint16_t*>(a->weight[t]);
     P.x_tok[t] = a->x_token_stride[t];
-    P.x_head[t] = a->x_head_stride[t];
-    P.dy_tok[t] = static_cast<long long>(a->heads[t]) * kHeadDim;
-    P.dy_head[t] = kHeadDim;
+    FGA_REQUIRE(a->x_head_stride[t] >= 0 && a->x_head_stride[t] <= 0x7fffffff, "rotary: head stride out of range");
+    P.x_head[t] = static_cast<int>(a->x_head_stride[t]);
     P.heads[t] = a->heads[t];
   }
   P.pos = a->positions;
