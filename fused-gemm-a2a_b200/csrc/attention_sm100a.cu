@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include "../../include/fga.h"
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "ptx.cuh"
 #include "seq_bounds.cuh"
 #include "wait.cuh"
@@ -48,34 +49,41 @@ struct AttentionParams {
   unsigned long long timeout_ns;
 };
 
-// Shared-memory matrix descriptors of a tile (128-byte swizzle, 8-row groups 1024 bytes apart).
-constexpr uint64_t kDescHigh = static_cast<uint64_t>(64u | (1u << 14) | (2u << 29)) << 32;
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) { return kDescHigh | ((addr >> 4) & 0x3fffu) | (1u << 16); }
-// MN-major: the 64-column halves are 16384 bytes apart.
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
-  return kDescHigh | ((addr >> 4) & 0x3fffu) | ((kHalfBytes >> 4) << 16);
+// Shared-memory matrix descriptors of a tile (128-byte swizzle, 8-row groups 1024 bytes apart): a constant
+// high word and a low word of address and leading stride. K-major, and MN-major with the 64-column halves
+// 16384 bytes apart.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t addr) {
+  return ((addr >> 4) & 0x3fffu) | ((kHalfBytes >> 4) << 16);
 }
 // Instruction descriptors: BF16 x BF16 -> FP32, M = N = 128, B K-major or MN-major.
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);
 constexpr uint32_t kIdescMn = kIdesc | (1u << 16);
 
+// The products below are issued by one elected lane of a converged warp.
 // D[128, 128] = A B^T over the 128 columns of two K-major tiles.
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile) {
-  const uint64_t a = desc_k_major(a_tile), b = desc_k_major(b_tile);
+  const uint32_t a = desc_k_major(a_tile), b = desc_k_major(b_tile);
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const uint32_t step = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
-    mma_bf16(d, a + step, b + step, kIdesc, k != 0);
+    mma_bf16<kDescHigh, kIdesc>(d, a + step, b + step, k != 0);
   }
 }
-// D[128, 128] (+)= A B over the 128 rows of B: A from TMEM (BF16, 64 columns, of which the second half may
-// lie `gap` columns further on), B a tile read MN-major.
-__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a_tmem, uint32_t b_tile, bool accumulate,
-                                             uint32_t gap = 0) {
-  const uint64_t b = desc_mn_major(b_tile);
+// D[128, 128] (+)= A B over 16 * kSteps rows of B from row 16 * step on: A from TMEM (BF16, 8 columns a
+// step), B a tile read MN-major.
+template <int kSteps>
+__device__ __forceinline__ void mma_weighted_part(uint32_t d, uint32_t a_tmem, uint32_t b_tile, int step, bool accumulate) {
+  const uint32_t b = desc_mn_major(b_tile) + step * 128;
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    mma_bf16_ta(d, a_tmem + k * 8 + (k >= 4 ? gap : 0), b + k * 128, kIdescMn, accumulate || k != 0);
+  for (int k = 0; k < kSteps; ++k)
+    mma_bf16_ta<kDescHigh, kIdescMn>(d, a_tmem + k * 8, b + k * 128, k != 0 ? 1u : accumulate);
+}
+// Over all 128 rows, with the halves of A 64 columns apart.
+__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a_tmem, uint32_t b_tile, bool accumulate) {
+  mma_weighted_part<4>(d, a_tmem, b_tile, 0, accumulate);
+  mma_weighted_part<4>(d, a_tmem + 64, b_tile, 4, true);
 }
 
 // Work tile `t` of `rows` rows: tiles are numbered sequence by sequence, the rows behind the last
@@ -130,7 +138,7 @@ __device__ __forceinline__ bool load_tail(uint32_t dst, const CUtensorMap* map, 
   if (lane == 0) {
     mbar_arrive_expect_tx(own, kTileBytes);
     load_tile(dst, map, own, head, row);
-    ok = mbar_wait(own, phase, w, 62);
+    ok = wait_small(own, phase, w, 62);
   }
   phase ^= 1;
   ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -189,6 +197,46 @@ __device__ __forceinline__ void store_row(uint32_t tmem, uint32_t slot, uint16_t
   store_piece(tmem + 64, slot, dst + 64, factor, valid);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void shared_pairs(uint32_t at, F2 (&v)[2]) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[0].v), "=l"(v[1].v) : "r"(at) : "memory");
+}
+__device__ __forceinline__ F2 f2_of_bits(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
+// 2^x of both halves without the special function unit, whose 16 results per cycle bound a softmax that
+// feeds tensor cores of this rate. x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
+// bits of the sum) and |f| <= 1/2; 2^f by the polynomial 1 + c1 f + .. + c4 f^4 of least relative error on that
+// interval (2.8e-6, fitted by iteratively reweighted least squares, constant term fixed), n added to the
+// exponent field. x below -127 gives 0; a NaN stays one.
+__device__ __forceinline__ F2 exp2_poly(F2 x) {
+  float lo, hi;
+  split(x, lo, hi);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
+  x = f2(lo, hi);
+  const F2 magic = f2(12582912.f), minus = f2(-12582912.f);
+  const F2 t = x + magic, n = t + minus, f = fma2(n, f2(-1.f), x);
+  F2 y = fma2(f, f2(0.009582854876057492f), f2(0.05590643239793828f));
+  y = fma2(y, f, f2(0.24024098625996076f));
+  y = fma2(y, f, f2(0.6931241925312817f));
+  y = fma2(y, f, f2(1.f));
+  float tl, th, yl, yh;
+  split(t, tl, th);
+  split(y, yl, yh);
+  const F2 r = f2(__uint_as_float(__float_as_uint(yl) + (__float_as_uint(tl) << 23)),
+                  __uint_as_float(__float_as_uint(yh) + (__float_as_uint(th) << 23)));
+  return fma2(x, f2(0.f), r);
+}
+// 2^x of both halves.
+__device__ __forceinline__ F2 exp2_pair(F2 x) {
+  float lo, hi;
+  split(x, lo, hi);
+  return f2(exp2_approx(lo), exp2_approx(hi));
+}
+
 // Every thread of the block: zero rows [row, end) of one head.
 __device__ __forceinline__ void zero_rows(uint16_t* base, int heads, int head, int row, int end) {
   for (int i = threadIdx.x; i < (end - row) * 16; i += blockDim.x)
@@ -219,21 +267,20 @@ __device__ __forceinline__ void settle(WaitCtx& w) {
 // probabilities are at most 2^8 too large, which the final division by the equally scaled sum undoes, and
 // the output accumulator need not be touched.
 // =============================================================================================
-constexpr int kFwdSlots = 5;
 constexpr int kFwdThreads = 384;
-constexpr uint32_t kFwdSmem = 2 * kTileBytes + kFwdSlots * kTileBytes + 256 + 1024;
+constexpr uint32_t kFwdStageBytes = 2 * kTileBytes;  // V(j) and K(j + 1): the operands of one iteration
+constexpr uint32_t kFwdSmem = 3 * kTileBytes + 2 * kFwdStageBytes + 256 + 1024;
 
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attention_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttentionParams P) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_smem = base, ring = base + 2 * kTileBytes;
-  const uint32_t bars = ring + kFwdSlots * kTileBytes;
-  const uint32_t q_full = bars, kv_full = bars + 16, kv_empty = kv_full + 8 * kFwdSlots,
-                 s_full = kv_empty + 8 * kFwdSlots, p_full = s_full + 16, pv_done = p_full + 16, own_bar = pv_done + 16,
+  const uint32_t q_smem = base, k0_smem = base + 2 * kTileBytes, ring = base + 3 * kTileBytes;
+  const uint32_t bars = ring + 2 * kFwdStageBytes;
+  const uint32_t q_full = bars, k0_full = bars + 16, full = k0_full + 8, empty = full + 16, s_full = empty + 16,
+                 p_full = s_full + 16 /* [tile][part] */, pv_done = p_full + 32, own_bar = pv_done + 16,
                  tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
-  static_assert(16 + 16 * kFwdSlots + 48 + 8 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int head = blockIdx.x % P.heads;
@@ -249,23 +296,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
   // key tiles of the two query tiles; a second tile that starts behind the sequence has none
   const int all_tiles = (wt.len + kTile - 1) / kTile;
-  int n[2];
-  n[0] = P.causal ? min(all_tiles, wt.row0 / kTile + 1) : all_tiles;
-  n[1] = wt.row0 + kTile >= wt.len ? 0 : P.causal ? min(all_tiles, wt.row0 / kTile + 2) : all_tiles;
-  const int n_max = max(n[0], n[1]);
+  const int n0 = P.causal ? min(all_tiles, wt.row0 / kTile + 1) : all_tiles;
+  const int n1 = wt.row0 + kTile >= wt.len ? 0 : P.causal ? min(all_tiles, wt.row0 / kTile + 2) : all_tiles;
+  const int n_max = max(n0, n1);
 
   WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 1);
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 4);
+      mbar_init(p_full + 16 * i, 4);
+      mbar_init(p_full + 16 * i + 8, 4);
       mbar_init(pv_done + 8 * i, 1);
     }
-    for (int i = 0; i < kFwdSlots; ++i) {
-      mbar_init(kv_full + 8 * i, 1);
-      mbar_init(kv_empty + 8 * i, 1);
-    }
+    mbar_init(k0_full, 1);
     mbar_init(own_bar, 1);
     asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
     fence_mbar_init();
@@ -283,88 +329,75 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp >= 8) {
     regs_down<80>();
     if (warp == 8) {
-      // ---------------------------------------------------------------- loads: Q, then K0 V0 K1 V1 ...
+      // ---------------------------------------------------------------- loads: Q, K(0), then V(j) with K(j + 1)
       const int kv_head = head / P.group;
-      if (lane == 0 && !w.dead)
-        for (int i = 0; i < 2; ++i)
-          if (n[i] > 0) {
-            mbar_arrive_expect_tx(q_full + 8 * i, kTileBytes);
-            load_tile(q_smem + i * kTileBytes, &map_q, q_full + 8 * i, head, wt.first + wt.row0 + i * kTile);
-          }
-      int slot = 0;
-      uint32_t phase = 0, own_phase = 0;
-      for (int j = 0; j < 2 * n_max && !w.dead; ++j) {
-        bool ok = true;
-        if (lane == 0) ok = mbar_wait(kv_empty + 8 * slot, phase ^ 1, w, 60);
-        if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
-          w.dead = true;
-          break;
-        }
-        const int row = (j >> 1) * kTile, valid = wt.len - row;
-        const uint32_t dst = ring + slot * kTileBytes, full = kv_full + 8 * slot;
-        if ((j & 1) && valid < kTile) {
-          if (!load_tail(dst, &map_v, full, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
-        } else if (lane == 0) {
-          mbar_arrive_expect_tx(full, kTileBytes);
-          load_tile(dst, (j & 1) ? &map_v : &map_k, full, kv_head, wt.first + row);
-        }
-        if (++slot == kFwdSlots) {
-          slot = 0;
-          phase ^= 1;
+      if (lane == 0 && !w.dead) {
+        mbar_arrive_expect_tx(q_full, kTileBytes);
+        load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
+        mbar_arrive_expect_tx(k0_full, kTileBytes);
+        load_tile(k0_smem, &map_k, k0_full, kv_head, wt.first);
+        if (n1 > 0) {
+          mbar_arrive_expect_tx(q_full + 8, kTileBytes);
+          load_tile(q_smem + kTileBytes, &map_q, q_full + 8, head, wt.first + wt.row0 + kTile);
         }
       }
-    } else if (warp == 9 && lane == 0) {
-      // ---------------------------------------------------------------- products
-      int k_slot = 0;                 // slot of K(j); V(j) is in the next one
-      uint32_t k_phase = 0;
-      auto advance = [](int& slot, uint32_t& phase) {
-        if (++slot == kFwdSlots) {
-          slot = 0;
-          phase ^= 1;
-        }
-      };
-      if (mbar_wait(kv_full, 0, w, 63)) {
-        for (int i = 0; i < 2; ++i)
-          if (n[i] > 0) {
-            if (!mbar_wait(q_full + 8 * i, 0, w, 64)) break;
-            tc_fence_after();
-            mma_rows(tmem + i * 128, q_smem + i * kTileBytes, ring);
-            tc_commit(s_full + 8 * i);
-          }
-        if (kFwdSlots < 2 * n_max) tc_commit(kv_empty);
-      }
+      uint32_t own_phase = 0;
       for (int j = 0; j < n_max && !w.dead; ++j) {
-        int v_slot = k_slot;
-        uint32_t v_phase = k_phase;
-        advance(v_slot, v_phase);
-        int next = v_slot;
-        uint32_t next_phase = v_phase;
-        advance(next, next_phase);
-        if (!mbar_wait(kv_full + 8 * v_slot, v_phase, w, 65)) break;
-        bool have_next = false;
-        for (int i = 0; i < 2; ++i) {
-          if (j < n[i]) {
-            if (!mbar_wait(p_full + 8 * i, j & 1, w, 66)) break;
-            tc_fence_after();
-            mma_weighted(tmem + 256 + i * 128, tmem + i * 128, ring + v_slot * kTileBytes, j > 0);
-            tc_commit(pv_done + 8 * i);
-          }
-          if (j + 1 < n[i]) {
-            if (!have_next) {
-              if (!mbar_wait(kv_full + 8 * next, next_phase, w, 67)) break;
-              tc_fence_after();
-              have_next = true;
-            }
-            mma_rows(tmem + i * 128, q_smem + i * kTileBytes, ring + next * kTileBytes);
-            tc_commit(s_full + 8 * i);
-          }
+        if (j >= 2 && !warp_wait(empty + 8 * (j & 1), ((j >> 1) & 1) ^ 1, w, 60)) break;
+        const int row = j * kTile, valid = wt.len - row;
+        const uint32_t dst = ring + (j & 1) * kFwdStageBytes, bar = full + 8 * (j & 1);
+        if (valid < kTile) {  // the last tile: no K follows
+          if (!load_tail(dst, &map_v, bar, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
+        } else if (lane == 0) {
+          const bool more = j + 1 < n_max;
+          mbar_arrive_expect_tx(bar, more ? 2 * kTileBytes : kTileBytes);
+          load_tile(dst, &map_v, bar, kv_head, wt.first + row);
+          if (more) load_tile(dst + kTileBytes, &map_k, bar, kv_head, wt.first + row + kTile);
         }
-        if (w.dead) break;
-        // A slot is only released to a load that will take it, so that no arrival is in flight at the end.
-        if (2 * j + 1 + kFwdSlots < 2 * n_max) tc_commit(kv_empty + 8 * v_slot);
-        if (2 * j + 2 + kFwdSlots < 2 * n_max) tc_commit(kv_empty + 8 * next);
-        k_slot = next;
-        k_phase = next_phase;
+        __syncwarp();
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------------- products
+      auto scores = [&](int i, uint32_t k_tile) {
+        if (elect_one()) {
+          mma_rows(tmem + i * 128, q_smem + i * kTileBytes, k_tile);
+          tc_commit(s_full + 8 * i);
+        }
+        __syncwarp();
+      };
+      // P(j) V(j) of tile i, the first 96 keys and the last 32, as its warpgroup hands them over
+      auto weighted = [&](int i, uint32_t v, int j, bool last) {
+        const uint32_t o = tmem + 256 + i * 128, p = tmem + i * 128;
+        if (!warp_wait(p_full + 16 * i, j & 1, w, 66)) return;
+        tc_fence_after();
+        if (elect_one()) mma_weighted_part<6>(o, p, v, 0, j > 0);
+        __syncwarp();
+        if (!warp_wait(p_full + 16 * i + 8, j & 1, w, 66)) return;
+        tc_fence_after();
+        if (elect_one()) {
+          mma_weighted_part<2>(o, p + 48, v, 6, true);
+          if (last) tc_commit(pv_done + 8 * i);
+        }
+        __syncwarp();
+      };
+      if (warp_wait(k0_full, 0, w, 63) && warp_wait(q_full, 0, w, 64)) {
+        tc_fence_after();
+        scores(0, k0_smem);
+        if (n1 > 0 && warp_wait(q_full + 8, 0, w, 64)) {
+          tc_fence_after();
+          scores(1, k0_smem);
+        }
+      }
+#pragma unroll 1
+      for (int j = 0; j < n_max && !w.dead; ++j) {
+        if (!warp_wait(full + 8 * (j & 1), (j >> 1) & 1, w, 65)) break;
+        const uint32_t v = ring + (j & 1) * kFwdStageBytes;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int n = i ? n1 : n0;
+          if (j < n && !w.dead) weighted(i, v, j, j + 1 == n);
+          if (j + 1 < n && !w.dead) scores(i, v + kTileBytes);
+        }
       }
     }
   } else {
@@ -375,16 +408,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint32_t s_tmem = tmem + i * 128 + lanes, o_tmem = tmem + 256 + i * 128 + lanes;
     const int row = wt.row0 + i * kTile + row_in_tile;  // within the sequence
     const float c = P.scale_log2;
-    const int tiles = n[i];
+    const int tiles = i ? n1 : n0;
+    const bool releases = warp == (n1 > 0 ? 4 : 0);
     float m = 0.f, l = 0.f;
     bool alive = true;
     for (int j = 0; j < tiles; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * i, j & 1, w, 70))) {
+      if (!warp_wait(s_full + 8 * i, j & 1, w, 70)) {
         w.dead = true;
         alive = false;
         break;
       }
       tc_fence_after();
+      // The scores of the tile that has the most keys are the last product of an iteration to be issued:
+      // their arrival frees the operands of the iteration before.
+      if (releases && lane == 0 && j > 0) mbar_arrive_local(empty + 8 * ((j - 1) & 1));
       uint32_t s[4][32];
 #pragma unroll
       for (int q = 0; q < 4; ++q) tmem_ld_32x32(s_tmem + q * 32, s[q]);
@@ -397,23 +434,47 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           for (int e = 0; e < 32; ++e)
             if (q * 32 + e >= limit) s[q][e] = 0xff800000u;  // -inf
       }
-      float mx[4];
+      auto row_max = [&]() {
+        float mx[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        mx[q] = __uint_as_float(s[q][0]);
+        for (int q = 0; q < 4; ++q) mx[q] = fmaxf(__uint_as_float(s[q][0]), __uint_as_float(s[q][1]));
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mx[q] = fmaxf(mx[q], __uint_as_float(s[q][e]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (j == 0) {
-        m = top == -INFINITY ? 0.f : top;
-      } else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
-        if (!__all_sync(0xffffffffu, mbar_wait(pv_done + 8 * i, (j - 1) & 1, w, 71))) {
-          w.dead = true;
-          alive = false;
-          break;
+        for (int e = 2; e < 32; e += 2)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
+        return max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+      };
+      const F2 c2 = f2(c);
+      uint32_t p[2][16];
+      // 32 probabilities; one pair in four by polynomial. One rounding to BF16, the type the products take;
+      // their sum stays FP32 and unrounded.
+      auto probabilities = [&](int q, F2 shift, F2& total, uint32_t (&out)[16]) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const F2 x = fma2(f2_of_bits(s[q][2 * e], s[q][2 * e + 1]), c2, shift);
+          const F2 y = (e & 3) == 3 ? exp2_poly(x) : exp2_pair(x);
+          total = total + y;
+          out[e] = bf16_of_f2(y);
         }
-        tc_fence_after();
+      };
+      auto hand_over = [&](int part) {
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(p_full + 16 * i + 8 * part);
+      };
+      if (j == 0) {
+        const float top = row_max();
+        m = top == -INFINITY ? 0.f : top;
+      }
+      // The first half goes ahead with the maximum of the tiles before, while this tile's is still being
+      // found; only a row that outgrows it by 2^8 has to start again.
+      F2 shift = f2(-m * c), sum2[2] = {f2(0.f), f2(0.f)};
+      probabilities(0, shift, sum2[0], p[0]);
+      probabilities(1, shift, sum2[1], p[1]);
+      const float top = row_max();
+      if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {  // never in the first tile
+        // S(j) was issued behind the product that last wrote the output: its arrival covers both
         const float up = fmaxf(m, top), f = exp2_approx((m - up) * c);
         m = up;
         l *= f;
@@ -426,30 +487,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
           tmem_st_32x32(o_tmem + q * 32, o);
         }
+        shift = f2(-m * c);
+        sum2[0] = sum2[1] = f2(0.f);
+        probabilities(0, shift, sum2[0], p[0]);
+        probabilities(1, shift, sum2[1], p[1]);
       }
-      const float shift = -m * c;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float a = exp2_approx(fmaf(__uint_as_float(s[q][2 * e]), c, shift));
-          const float b = exp2_approx(fmaf(__uint_as_float(s[q][2 * e + 1]), c, shift));
-          sum[(2 * e) & 3] += a;
-          sum[(2 * e + 1) & 3] += b;
-          // One rounding of the probabilities to BF16, the type the products take; their sum stays FP32.
-          p[e] = pack_pair(a, b);
-        }
-        tmem_st_32x16(s_tmem + q * 16, p);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_local(p_full + 8 * i);
+      tmem_st_32x16(s_tmem, p[0]);
+      tmem_st_32x16(s_tmem + 16, p[1]);
+      probabilities(2, shift, sum2[0], p[0]);
+      tmem_st_32x16(s_tmem + 32, p[0]);
+      hand_over(0);
+      probabilities(3, shift, sum2[1], p[1]);
+      tmem_st_32x16(s_tmem + 48, p[1]);
+      hand_over(1);
+      l += sum(sum2[0] + sum2[1]);
     }
-    if (alive && tiles > 0 && __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * i, (tiles - 1) & 1, w, 72))) {
+    if (alive && tiles > 0 && warp_wait(pv_done + 8 * i, 0, w, 72)) {
       tc_fence_after();
       const bool valid = row < wt.len;
       const long long at = wt.first + row;
@@ -584,7 +637,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
       const int valid = min(kTile, wt.len - row);
       bool ok = true;
-      if (lane == 0) ok = mbar_wait(empty + 8 * st, phase ^ 1, w, 80);
+      if (lane == 0) ok = wait_small(empty + 8 * st, phase ^ 1, w, 80);
       if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
         w.dead = true;
         break;
@@ -623,12 +676,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
-    if (lane == 0 && mbar_wait(kv_full, 0, w, 81) && mbar_wait(full, 0, w, 82)) {
+    if (warp_wait(kv_full, 0, w, 81) && warp_wait(full, 0, w, 82)) {
       tc_fence_after();
-      mma_rows(tmem, k_smem, ring);
-      tc_commit(s_full);
-      mma_rows(tmem + 128, v_smem, ring + kTileBytes);
-      tc_commit(dp_full);
+      if (elect_one()) {
+        mma_rows(tmem, k_smem, ring);
+        tc_commit(s_full);
+        mma_rows(tmem + 128, v_smem, ring + kTileBytes);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
       int st = 0;
       uint32_t phase = 0;
       for (int i = 0; i < total; ++i) {
@@ -640,25 +696,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         const uint32_t next_q = ring + st * kDkvStageBytes;
         const bool more = i + 1 < total;
-        if (!mbar_wait(p_full, i & 1, w, 83)) break;
+        if (more && !warp_wait(full + 8 * st, phase, w, 84)) break;
+        if (!warp_wait(p_full, i & 1, w, 83)) break;
         tc_fence_after();
-        mma_weighted(tmem + 256, tmem, do_tile, i > 0, 32);
-        if (more) {
-          if (!mbar_wait(full + 8 * st, phase, w, 84)) break;
-          tc_fence_after();
-          mma_rows(tmem, k_smem, next_q);
-          tc_commit(s_full);
+        if (elect_one()) {
+          mma_weighted(tmem + 256, tmem, do_tile, i > 0);
+          if (more) {
+            mma_rows(tmem, k_smem, next_q);
+            tc_commit(s_full);
+          }
         }
-        if (!mbar_wait(ds_full, i & 1, w, 85)) break;
+        __syncwarp();
+        if (!warp_wait(ds_full, i & 1, w, 85)) break;
         tc_fence_after();
-        mma_weighted(tmem + 384, tmem + 128, q_tile, i > 0, 32);
-        if (i + kDkvStages < total) tc_commit(empty + 8 * cur);
-        if (more) {
-          mma_rows(tmem + 128, v_smem, next_q + kTileBytes);
-          tc_commit(dp_full);
+        if (elect_one()) {
+          mma_weighted(tmem + 384, tmem + 128, q_tile, i > 0);
+          if (i + kDkvStages < total) tc_commit(empty + 8 * cur);
+          if (more) {
+            mma_rows(tmem + 128, v_smem, next_q + kTileBytes);
+            tc_commit(dp_full);
+          }
         }
+        __syncwarp();
       }
-      if (!w.dead) tc_commit(acc_done);
+      if (!w.dead && elect_one()) tc_commit(acc_done);
+      __syncwarp();
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------------ P and dS
@@ -671,12 +733,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     bool alive = true;
     for (int i = 0; i < total; ++i) {
       // the stage's own barrier orders this thread behind the stores of the row values
-      if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * st, phase, w, 89) && mbar_wait(s_full, i & 1, w, 86))) {
+      if (!warp_wait(full + 8 * st, phase, w, 89) || !warp_wait(s_full, i & 1, w, 86)) {
         alive = false;
         break;
       }
       tc_fence_after();
-      float p[64];
+      F2 p[32];
+      const F2 c2 = f2(c);
       {
         uint32_t s[2][32];
         tmem_ld_32x32(s_tmem, s[0]);
@@ -685,37 +748,41 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t neg = rows_smem + st * 1024 + g * 256;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          float n[4];
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(n[0]), "=f"(n[1]), "=f"(n[2]), "=f"(n[3])
-                       : "r"(neg + v * 16));
+          F2 n[2];
+          shared_pairs(neg + v * 16, n);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            p[v * 4 + e] = exp2_approx(fmaf(__uint_as_float(s[v >> 3][(v & 7) * 4 + e]), c, n[e]));
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t* x = &s[v >> 3][(v & 7) * 4 + 2 * e];
+            p[v * 2 + e] = exp2_pair(fma2(f2_of_bits(x[0], x[1]), c2, n[e]));
+          }
         }
       }
       if (P.causal && i % per_head == 0) {  // the diagonal tile: queries in front of the key do not see it
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (g * 64 + e < key) p[e] = 0.f;
+        for (int e = 0; e < 32; ++e) {
+          float lo, hi;
+          split(p[e], lo, hi);
+          p[e] = f2(g * 64 + 2 * e < key ? 0.f : lo, g * 64 + 2 * e + 1 < key ? 0.f : hi);
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t b[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) b[e] = pack_pair(p[h * 32 + 2 * e], p[h * 32 + 2 * e + 1]);
+        for (int e = 0; e < 16; ++e) b[e] = bf16_of_f2(p[h * 16 + e]);
         tmem_st_32x16(s_tmem + h * 16, b);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_local(p_full);
-      if (!__all_sync(0xffffffffu, mbar_wait(dp_full, i & 1, w, 87))) {
+      if (!warp_wait(dp_full, i & 1, w, 87)) {
         alive = false;
         break;
       }
       tc_fence_after();
       const uint32_t delta = rows_smem + st * 1024 + 512 + g * 256;
+      const F2 minus = f2(-1.f);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t d[32], b[16];
@@ -723,15 +790,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld_wait();
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
-          float n[4];
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(n[0]), "=f"(n[1]), "=f"(n[2]), "=f"(n[3])
-                       : "r"(delta + h * 128 + v * 16));
-          float x[4];
+          F2 n[2];
+          shared_pairs(delta + h * 128 + v * 16, n);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = p[h * 32 + v * 4 + e] * (__uint_as_float(d[v * 4 + e]) - n[e]);
-          b[2 * v] = pack_pair(x[0], x[1]);
-          b[2 * v + 1] = pack_pair(x[2], x[3]);
+          for (int e = 0; e < 2; ++e)
+            b[2 * v + e] = bf16_of_f2(p[h * 16 + v * 2 + e] *
+                                      fma2(n[e], minus, f2_of_bits(d[v * 4 + 2 * e], d[v * 4 + 2 * e + 1])));
         }
         // columns [0, 32) of this warpgroup's half have been read when h = 1 is stored to [16, 32), and
         // h = 0 goes to [0, 16), which it has just read itself
@@ -746,7 +810,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         phase ^= 1;
       }
     }
-    if (alive && __all_sync(0xffffffffu, mbar_wait(acc_done, 0, w, 88))) {
+    if (alive && warp_wait(acc_done, 0, w, 88)) {
       tc_fence_after();
       const bool valid = wt.row0 + key < wt.len;
       const long long at = (static_cast<long long>(wt.first + wt.row0 + key) * P.kv_heads + kv_head) * kDim;
@@ -833,7 +897,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     uint32_t phase = 0, own_phase = 0;
     for (int j = 0; j < n && !w.dead; ++j) {
       bool ok = true;
-      if (lane == 0) ok = mbar_wait(empty + 8 * st, phase ^ 1, w, 90);
+      if (lane == 0) ok = wait_small(empty + 8 * st, phase ^ 1, w, 90);
       if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
         w.dead = true;
         break;
@@ -857,12 +921,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
-    if (lane == 0 && mbar_wait(q_full, 0, w, 91) && mbar_wait(full, 0, w, 92)) {
+    if (warp_wait(q_full, 0, w, 91) && warp_wait(full, 0, w, 92)) {
       tc_fence_after();
-      mma_rows(tmem, q_smem, ring);
-      tc_commit(s_full);
-      mma_rows(tmem + 256, do_smem, ring + kTileBytes);
-      tc_commit(dp_full);
+      if (elect_one()) {
+        mma_rows(tmem, q_smem, ring);
+        tc_commit(s_full);
+        mma_rows(tmem + 256, do_smem, ring + kTileBytes);
+        tc_commit(dp_full);
+      }
+      __syncwarp();
       int st = 0;
       uint32_t phase = 0;
       for (int j = 0; j < n; ++j) {
@@ -874,21 +941,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         const uint32_t next_k = ring + st * kDqStageBytes;
         if (j + 1 < n) {
-          if (!mbar_wait(full + 8 * st, phase, w, 93)) break;
+          if (!warp_wait(full + 8 * st, phase, w, 93)) break;
           tc_fence_after();
-          mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, next_k);
-          tc_commit(s_full + 8 * ((j + 1) & 1));
-          if (!mbar_wait(dp_read, j & 1, w, 94)) break;
+          if (elect_one()) {
+            mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, next_k);
+            tc_commit(s_full + 8 * ((j + 1) & 1));
+          }
+          __syncwarp();
+          if (!warp_wait(dp_read, j & 1, w, 94)) break;
           tc_fence_after();
-          mma_rows(tmem + 256, do_smem, next_k + kTileBytes);
-          tc_commit(dp_full);
+          if (elect_one()) {
+            mma_rows(tmem + 256, do_smem, next_k + kTileBytes);
+            tc_commit(dp_full);
+          }
+          __syncwarp();
         }
-        if (!mbar_wait(ds_full, j & 1, w, 95)) break;
+        if (!warp_wait(ds_full, j & 1, w, 95)) break;
         tc_fence_after();
-        mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_tile, j > 0, 32);
-        if (j + kDqStages < n) tc_commit(empty + 8 * cur);
+        if (elect_one()) {
+          mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_tile, j > 0);
+          if (j + kDqStages < n) tc_commit(empty + 8 * cur);
+        }
+        __syncwarp();
       }
-      if (!w.dead) tc_commit(acc_done);
+      if (!w.dead && elect_one()) tc_commit(acc_done);
+      __syncwarp();
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------------ dS
@@ -897,27 +974,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int row = wt.row0 + row_in_tile;
     const bool valid = row < wt.len;
     const long long at = wt.first + (valid ? row : 0);
-    const float c = P.scale_log2;
-    const float neg = -kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at);
-    const float delta = __ldg(P.delta + static_cast<long long>(head) * P.tokens + at);
+    const F2 c2 = f2(P.scale_log2);
+    const F2 neg = f2(-kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at));
+    const F2 delta = f2(-__ldg(P.delta + static_cast<long long>(head) * P.tokens + at));
     bool alive = true;
     for (int j = 0; j < n; ++j) {
       const uint32_t s_tmem = tmem + lanes + (j & 1) * 128 + g * 64, dp_tmem = tmem + lanes + 256 + g * 64;
-      if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * (j & 1), (j >> 1) & 1, w, 96))) {
+      if (!warp_wait(s_full + 8 * (j & 1), (j >> 1) & 1, w, 96)) {
         alive = false;
         break;
       }
       tc_fence_after();
-      float p[64];
+      F2 p[32];
       {
         uint32_t s[2][32];
         tmem_ld_32x32(s_tmem, s[0]);
         tmem_ld_32x32(s_tmem + 32, s[1]);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 64; ++e) p[e] = exp2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), c, neg));
+        for (int e = 0; e < 32; ++e)
+          p[e] = exp2_pair(fma2(f2_of_bits(s[e >> 4][2 * (e & 15)], s[e >> 4][2 * (e & 15) + 1]), c2, neg));
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(dp_full, j & 1, w, 97))) {
+      if (!warp_wait(dp_full, j & 1, w, 97)) {
         alive = false;
         break;
       }
@@ -930,18 +1008,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_local(dp_read);
 #pragma unroll
-      for (int e = 0; e < 64; ++e) p[e] *= __uint_as_float(d[e >> 5][e & 31]) - delta;
+      for (int e = 0; e < 32; ++e)
+        p[e] = p[e] * (f2_of_bits(d[e >> 4][2 * (e & 15)], d[e >> 4][2 * (e & 15) + 1]) + delta);
       if (j == n - 1) {
         const int limit = min(wt.len, P.causal ? row + 1 : wt.len) - j * kTile - g * 64;
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (e >= limit) p[e] = 0.f;
+        for (int e = 0; e < 32; ++e) {
+          float lo, hi;
+          split(p[e], lo, hi);
+          p[e] = f2(2 * e >= limit ? 0.f : lo, 2 * e + 1 >= limit ? 0.f : hi);
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t b[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) b[e] = pack_pair(p[h * 32 + 2 * e], p[h * 32 + 2 * e + 1]);
+        for (int e = 0; e < 16; ++e) b[e] = bf16_of_f2(p[h * 16 + e]);
         tmem_st_32x16(s_tmem + h * 16, b);
       }
       tmem_st_wait();
@@ -949,7 +1031,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_local(ds_full);
     }
-    if (alive && __all_sync(0xffffffffu, mbar_wait(acc_done, 0, w, 98))) {
+    if (alive && warp_wait(acc_done, 0, w, 98)) {
       tc_fence_after();
       // each warpgroup stores half of the columns; Q and dO have been read for the last time
       store_piece(tmem + lanes + 384 + g * 64, (g ? do_smem : q_smem) + row_in_tile * kSlotPitch,

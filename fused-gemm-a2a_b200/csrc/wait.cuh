@@ -50,4 +50,31 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, WaitCtx
   return true;
 }
 
+// The same with as little as possible in front of and inside the spin: what a role executes once per tile has
+// to come from the instruction cache each time, beside the other roles' code.
+__device__ __forceinline__ bool wait_small(uint32_t bar, uint32_t parity, WaitCtx& w, int where) {
+  if (w.dead) return false;
+  uint64_t since = 0;
+#pragma unroll 1
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (__builtin_expect((it & 0x3ff) == 0, 0)) {
+      if (should_abort(w)) return false;
+      const uint64_t now = globaltimer_ns();
+      if (since == 0) {
+        since = now;
+      } else if (now - since > w.timeout_ns) {
+        report(w, kErrPipelineTimeout, where, static_cast<int>(bar));
+        return false;
+      }
+    }
+  }
+}
+// For a converged warp whose lanes must take the same way afterwards.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, WaitCtx& w, int where) {
+  const bool ok = __all_sync(0xffffffffu, wait_small(bar, parity, w, where));
+  w.dead = !ok;
+  return ok;
+}
+
 }  // namespace fga
