@@ -157,6 +157,19 @@ __device__ __forceinline__ bool load_tail(uint32_t dst, const CUtensorMap* map, 
   return true;
 }
 
+// A place in a ring of buffers and the parity of its barriers there.
+struct Slot {
+  int at;
+  uint32_t phase;
+  template <int kSlots>
+  __device__ __forceinline__ void next() {
+    if (++at == kSlots) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -565,23 +578,30 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const uint16_t* o,
 // ---- dK, dV: S^T and dP^T tiles, rows = keys, columns = queries. TMEM: S^T (then P^T) 0, dP^T (then
 // dS^T) 128, dV 256, dK 384. The tensor cores run dV(i) and S(i+1) while the warps compute dS(i), and
 // dK(i) and dP(i+1) while they compute P(i+1).
-constexpr int kDkvStages = 2;
-constexpr uint32_t kDkvStageBytes = 2 * kTileBytes;
-constexpr uint32_t kDkvSmem = 2 * kTileBytes + kDkvStages * (kDkvStageBytes + 1024) + 256 + 1024;
+//
+// Q(i + 1) is needed first and Q(i) is let go last, so Q has three slots and dO two: with two pairs the
+// products waited 2100 cycles per tile for Q. The row values (lse, delta) have a warp and a ring of their own.
+// All of an SM's shared memory is in use: row values and barriers lie in the 3 KiB in front of the tiles.
+constexpr int kQSlots = 3, kDoSlots = 2, kRowSlots = 2;
+constexpr uint32_t kDkvSmem = (2 + kQSlots + kDoSlots) * kTileBytes + 3072;
+static_assert(kDkvSmem <= 227 * 1024 && kRowSlots * 1024 + 256 <= 3072, "shared memory");
 
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                          const __grid_constant__ AttentionParams P) {
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t k_smem = base, v_smem = base + kTileBytes, ring = base + 2 * kTileBytes;
-  const uint32_t rows_smem = ring + kDkvStages * kDkvStageBytes;  // per stage: -lse * log2(e) [128], delta [128]
-  const uint32_t bars = rows_smem + kDkvStages * 1024;
-  const uint32_t kv_full = bars, full = bars + 8, empty = full + 8 * kDkvStages, s_full = empty + 8 * kDkvStages,
-                 dp_full = s_full + 8, p_full = dp_full + 8, ds_full = p_full + 8, acc_done = ds_full + 8,
-                 own_bar = acc_done + 8, tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
-  static_assert(8 + 16 * kDkvStages + 48 + 16 <= 256, "barrier area");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t front = smem_u32(smem_raw), base = front + 3072;
+  const uint32_t k_smem = base, v_smem = base + kTileBytes, q_ring = base + 2 * kTileBytes,
+                 do_ring = q_ring + kQSlots * kTileBytes;
+  const uint32_t rows_smem = front;  // per slot: -lse * log2(e) [128], delta [128]
+  const uint32_t bars = rows_smem + kRowSlots * 1024;
+  const uint32_t kv_full = bars, q_full = bars + 8, q_empty = q_full + 8 * kQSlots, do_full = q_empty + 8 * kQSlots,
+                 do_empty = do_full + 8 * kDoSlots, rows_full = do_empty + 8 * kDoSlots,
+                 rows_empty = rows_full + 8 * kRowSlots, s_full = rows_empty + 8 * kRowSlots, dp_full = s_full + 8,
+                 p_full = dp_full + 8, ds_full = p_full + 8, acc_done = ds_full + 8, own_bar = acc_done + 8,
+                 tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
+  static_assert(8 + 16 * (kQSlots + kDoSlots + kRowSlots) + 48 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int kv_head = blockIdx.x % P.kv_heads;
@@ -599,11 +619,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int per_head = q_tiles - q_first, total = per_head * P.group;
 
   WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
+  if ((front & 1023u) != 0) {  // the tiles would not be where their swizzle needs them
+    if (threadIdx.x == 0 && atomicCAS(P.status, 0, kErrPipelineTimeout) == 0) P.status[1] = 78;
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int i = 0; i < kDkvStages; ++i) {
-      mbar_init(full + 8 * i, 3);  // Q, dO, and the row values
-      mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < kQSlots; ++i) {
+      mbar_init(q_full + 8 * i, 1);
+      mbar_init(q_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kDoSlots; ++i) {
+      mbar_init(do_full + 8 * i, 1);
+      mbar_init(do_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kRowSlots; ++i) {
+      mbar_init(rows_full + 8 * i, 1);
+      mbar_init(rows_empty + 8 * i, 8);
     }
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
@@ -631,89 +663,94 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       load_tile(k_smem, &map_k, kv_full, kv_head, wt.first + wt.row0);
       load_tile(v_smem, &map_v, kv_full, kv_head, wt.first + wt.row0);
     }
-    int st = 0;
-    uint32_t phase = 0, own_phase = 0;
+    uint32_t own_phase = 0;
+    Slot qs{0, 0}, ds{0, 0};
+    // rows behind the sequence are operands of the sums over queries here, so short tiles are cleared
+    auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int head, int row) {
+      const int valid = wt.len - row;
+      if (valid < kTile) return load_tail(dst, map, full, own_bar, own_phase, head, wt.first + row, valid, lane, w);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full, kTileBytes);
+        load_tile(dst, map, full, head, wt.first + row);
+      }
+      __syncwarp();
+      return true;
+    };
     for (int i = 0; i < total && !w.dead; ++i) {
       const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
-      const int valid = min(kTile, wt.len - row);
-      bool ok = true;
-      if (lane == 0) ok = wait_small(empty + 8 * st, phase ^ 1, w, 80);
-      if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
-        w.dead = true;
-        break;
-      }
-      const uint32_t q_dst = ring + st * kDkvStageBytes, do_dst = q_dst + kTileBytes, bar = full + 8 * st;
-      if (valid == kTile) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, kTileBytes);
-          load_tile(q_dst, &map_q, bar, head, wt.first + row);
-          mbar_arrive_expect_tx(bar, kTileBytes);
-          load_tile(do_dst, &map_do, bar, head, wt.first + row);
-        }
-      } else {
-        // rows behind the sequence are operands of the sums over queries here
-        if (!load_tail(q_dst, &map_q, bar, own_bar, own_phase, head, wt.first + row, valid, lane, w)) break;
-        if (!load_tail(do_dst, &map_do, bar, own_bar, own_phase, head, wt.first + row, valid, lane, w)) break;
-      }
+      if (i >= kQSlots && !warp_wait(q_empty + 8 * qs.at, qs.phase ^ 1, w, 80)) break;
+      if (!load(&map_q, q_ring + qs.at * kTileBytes, q_full + 8 * qs.at, head, row)) break;
+      if (i >= kDoSlots && !warp_wait(do_empty + 8 * ds.at, ds.phase ^ 1, w, 80)) break;
+      if (!load(&map_do, do_ring + ds.at * kTileBytes, do_full + 8 * ds.at, head, row)) break;
+      qs.next<kQSlots>();
+      ds.next<kDoSlots>();
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------------ row values of the queries
+    Slot rs{0, 0};
+    for (int i = 0; i < total; ++i) {
+      const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
       const long long at = static_cast<long long>(head) * P.tokens + wt.first + row;
+      float neg[4], delta[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int q = c * 32 + lane;
-        float neg = -INFINITY, delta = 0.f;  // a probability of 0 behind the sequence
-        if (q < valid) {
-          neg = -kLog2e * __ldg(P.lse + at + q);
-          delta = __ldg(P.delta + at + q);
+        neg[c] = -INFINITY;  // a probability of 0 behind the sequence
+        delta[c] = 0.f;
+        if (row + q < wt.len) {
+          neg[c] = -kLog2e * __ldg(P.lse + at + q);
+          delta[c] = __ldg(P.delta + at + q);
         }
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows_smem + st * 1024 + q * 4), "f"(neg) : "memory");
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows_smem + st * 1024 + 512 + q * 4), "f"(delta) : "memory");
+      }
+      if (i >= kRowSlots && !warp_wait(rows_empty + 8 * rs.at, rs.phase ^ 1, w, 79)) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t to = rows_smem + rs.at * 1024 + (c * 32 + lane) * 4;
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(neg[c]) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512), "f"(delta[c]) : "memory");
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_local(bar);
-      if (++st == kDkvStages) {
-        st = 0;
-        phase ^= 1;
-      }
+      if (lane == 0) mbar_arrive_local(rows_full + 8 * rs.at);
+      rs.next<kRowSlots>();
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
-    if (warp_wait(kv_full, 0, w, 81) && warp_wait(full, 0, w, 82)) {
+    if (warp_wait(kv_full, 0, w, 81) && warp_wait(q_full, 0, w, 82) && warp_wait(do_full, 0, w, 82)) {
       tc_fence_after();
       if (elect_one()) {
-        mma_rows(tmem, k_smem, ring);
+        mma_rows(tmem, k_smem, q_ring);
         tc_commit(s_full);
-        mma_rows(tmem + 128, v_smem, ring + kTileBytes);
+        mma_rows(tmem + 128, v_smem, do_ring);
         tc_commit(dp_full);
       }
       __syncwarp();
-      int st = 0;
-      uint32_t phase = 0;
+      Slot qs{0, 0}, ds{0, 0};
+#pragma unroll 1
       for (int i = 0; i < total; ++i) {
-        const uint32_t q_tile = ring + st * kDkvStageBytes, do_tile = q_tile + kTileBytes;
-        const int cur = st;
-        if (++st == kDkvStages) {
-          st = 0;
-          phase ^= 1;
-        }
-        const uint32_t next_q = ring + st * kDkvStageBytes;
+        const int q_at = qs.at, do_at = ds.at;
+        qs.next<kQSlots>();
+        ds.next<kDoSlots>();
         const bool more = i + 1 < total;
-        if (more && !warp_wait(full + 8 * st, phase, w, 84)) break;
         if (!warp_wait(p_full, i & 1, w, 83)) break;
+        if (more && !warp_wait(q_full + 8 * qs.at, qs.phase, w, 84)) break;
         tc_fence_after();
         if (elect_one()) {
-          mma_weighted(tmem + 256, tmem, do_tile, i > 0);
+          mma_weighted(tmem + 256, tmem, do_ring + do_at * kTileBytes, i > 0);
+          if (i + kDoSlots < total) tc_commit(do_empty + 8 * do_at);
           if (more) {
-            mma_rows(tmem, k_smem, next_q);
+            mma_rows(tmem, k_smem, q_ring + qs.at * kTileBytes);
             tc_commit(s_full);
           }
         }
         __syncwarp();
         if (!warp_wait(ds_full, i & 1, w, 85)) break;
+        if (more && !warp_wait(do_full + 8 * ds.at, ds.phase, w, 84)) break;
         tc_fence_after();
         if (elect_one()) {
-          mma_weighted(tmem + 384, tmem + 128, q_tile, i > 0);
-          if (i + kDkvStages < total) tc_commit(empty + 8 * cur);
+          mma_weighted(tmem + 384, tmem + 128, q_ring + q_at * kTileBytes, i > 0);
+          if (i + kQSlots < total) tc_commit(q_empty + 8 * q_at);
           if (more) {
-            mma_rows(tmem + 128, v_smem, next_q + kTileBytes);
+            mma_rows(tmem + 128, v_smem, do_ring + ds.at * kTileBytes);
             tc_commit(dp_full);
           }
         }
@@ -728,12 +765,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + g * 64, dp_tmem = s_tmem + 128;
     const float c = P.scale_log2;
-    int st = 0;
-    uint32_t phase = 0;
+    Slot rs{0, 0};
     bool alive = true;
+#pragma unroll 1
     for (int i = 0; i < total; ++i) {
-      // the stage's own barrier orders this thread behind the stores of the row values
-      if (!warp_wait(full + 8 * st, phase, w, 89) || !warp_wait(s_full, i & 1, w, 86)) {
+      const uint32_t rows = rows_smem + rs.at * 1024 + g * 256;
+      if (!warp_wait(rows_full + 8 * rs.at, rs.phase, w, 89) || !warp_wait(s_full, i & 1, w, 86)) {
         alive = false;
         break;
       }
@@ -745,11 +782,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld_32x32(s_tmem, s[0]);
         tmem_ld_32x32(s_tmem + 32, s[1]);
         tmem_ld_wait();
-        const uint32_t neg = rows_smem + st * 1024 + g * 256;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           F2 n[2];
-          shared_pairs(neg + v * 16, n);
+          shared_pairs(rows + v * 16, n);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t* x = &s[v >> 3][(v & 7) * 4 + 2 * e];
@@ -781,7 +817,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         break;
       }
       tc_fence_after();
-      const uint32_t delta = rows_smem + st * 1024 + 512 + g * 256;
       const F2 minus = f2(-1.f);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -791,7 +826,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
           F2 n[2];
-          shared_pairs(delta + h * 128 + v * 16, n);
+          shared_pairs(rows + 512 + h * 128 + v * 16, n);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             b[2 * v + e] = bf16_of_f2(p[h * 16 + v * 2 + e] *
@@ -804,11 +839,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_local(ds_full);
-      if (++st == kDkvStages) {
-        st = 0;
-        phase ^= 1;
+      if (lane == 0) {
+        mbar_arrive_local(ds_full);
+        mbar_arrive_local(rows_empty + 8 * rs.at);
       }
+      rs.next<kRowSlots>();
     }
     if (alive && warp_wait(acc_done, 0, w, 88)) {
       tc_fence_after();
@@ -829,9 +864,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
 // ---- dQ: S and dP tiles, rows = queries, columns = keys. TMEM: S (then dS) in two buffers 0 and 128, dP
 // 256, dQ 384. The tensor cores run S(j+1) and dP(j+1) while the warps compute dS(j).
-constexpr int kDqStages = 2;
-constexpr uint32_t kDqStageBytes = 2 * kTileBytes;
-constexpr uint32_t kDqSmem = 2 * kTileBytes + kDqStages * kDqStageBytes + 256 + 1024;
+// K has three slots and V two for the same reason as above.
+constexpr int kKSlots = 3, kVSlots = 2;
+constexpr uint32_t kDqSmem = (2 + kKSlots + kVSlots) * kTileBytes + 256 + 1024;
 
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -839,12 +874,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         const __grid_constant__ AttentionParams P) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_smem = base, do_smem = base + kTileBytes, ring = base + 2 * kTileBytes;
-  const uint32_t bars = ring + kDqStages * kDqStageBytes;
-  const uint32_t q_full = bars, full = bars + 8, empty = full + 8 * kDqStages, s_full = empty + 8 * kDqStages,
-                 dp_full = s_full + 16, dp_read = dp_full + 8, ds_full = dp_read + 8, acc_done = ds_full + 8,
-                 own_bar = acc_done + 8, tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
-  static_assert(8 + 16 * kDqStages + 56 + 16 <= 256, "barrier area");
+  const uint32_t q_smem = base, do_smem = base + kTileBytes, k_ring = base + 2 * kTileBytes,
+                 v_ring = k_ring + kKSlots * kTileBytes;
+  const uint32_t bars = v_ring + kVSlots * kTileBytes;
+  const uint32_t q_full = bars, k_full = bars + 8, k_empty = k_full + 8 * kKSlots, v_full = k_empty + 8 * kKSlots,
+                 v_empty = v_full + 8 * kVSlots, s_full = v_empty + 8 * kVSlots, dp_full = s_full + 16,
+                 dp_read = dp_full + 8, ds_full = dp_read + 8, acc_done = ds_full + 8, own_bar = acc_done + 8,
+                 tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
+  static_assert(8 + 16 * (kKSlots + kVSlots) + 56 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int head = blockIdx.x % P.heads;
@@ -861,9 +898,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < kDqStages; ++i) {
-      mbar_init(full + 8 * i, 2);  // K and V
-      mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < kKSlots; ++i) {
+      mbar_init(k_full + 8 * i, 1);
+      mbar_init(k_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kVSlots; ++i) {
+      mbar_init(v_full + 8 * i, 1);
+      mbar_init(v_empty + 8 * i, 1);
     }
     mbar_init(s_full, 1);
     mbar_init(s_full + 8, 1);
@@ -893,74 +934,69 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
       load_tile(do_smem, &map_do, q_full, head, wt.first + wt.row0);
     }
-    int st = 0;
-    uint32_t phase = 0, own_phase = 0;
+    uint32_t own_phase = 0;
+    Slot ks{0, 0}, vs{0, 0};
     for (int j = 0; j < n && !w.dead; ++j) {
-      bool ok = true;
-      if (lane == 0) ok = wait_small(empty + 8 * st, phase ^ 1, w, 90);
-      if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) == 0) {
-        w.dead = true;
-        break;
-      }
       const int row = j * kTile, valid = wt.len - row;
-      const uint32_t k_dst = ring + st * kDqStageBytes, bar = full + 8 * st;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, kTileBytes);
-        load_tile(k_dst + kTileBytes, &map_v, bar, kv_head, wt.first + row);
-      }
+      const uint32_t k_dst = k_ring + ks.at * kTileBytes, k_bar = k_full + 8 * ks.at;
+      if (j >= kKSlots && !warp_wait(k_empty + 8 * ks.at, ks.phase ^ 1, w, 90)) break;
       if (valid < kTile) {  // K is also summed over, V only makes scores that are masked
-        if (!load_tail(k_dst, &map_k, bar, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
+        if (!load_tail(k_dst, &map_k, k_bar, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
       } else if (lane == 0) {
-        mbar_arrive_expect_tx(bar, kTileBytes);
-        load_tile(k_dst, &map_k, bar, kv_head, wt.first + row);
+        mbar_arrive_expect_tx(k_bar, kTileBytes);
+        load_tile(k_dst, &map_k, k_bar, kv_head, wt.first + row);
       }
-      if (++st == kDqStages) {
-        st = 0;
-        phase ^= 1;
+      __syncwarp();
+      if (j >= kVSlots && !warp_wait(v_empty + 8 * vs.at, vs.phase ^ 1, w, 90)) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(v_full + 8 * vs.at, kTileBytes);
+        load_tile(v_ring + vs.at * kTileBytes, &map_v, v_full + 8 * vs.at, kv_head, wt.first + row);
       }
+      __syncwarp();
+      ks.next<kKSlots>();
+      vs.next<kVSlots>();
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ products
-    if (warp_wait(q_full, 0, w, 91) && warp_wait(full, 0, w, 92)) {
+    if (warp_wait(q_full, 0, w, 91) && warp_wait(k_full, 0, w, 92) && warp_wait(v_full, 0, w, 92)) {
       tc_fence_after();
       if (elect_one()) {
-        mma_rows(tmem, q_smem, ring);
+        mma_rows(tmem, q_smem, k_ring);
         tc_commit(s_full);
-        mma_rows(tmem + 256, do_smem, ring + kTileBytes);
+        mma_rows(tmem + 256, do_smem, v_ring);
         tc_commit(dp_full);
+        if (kVSlots < n) tc_commit(v_empty);
       }
       __syncwarp();
-      int st = 0;
-      uint32_t phase = 0;
+      Slot ks{0, 0}, vs{0, 0};
+#pragma unroll 1
       for (int j = 0; j < n; ++j) {
-        const uint32_t k_tile = ring + st * kDqStageBytes;
-        const int cur = st;
-        if (++st == kDqStages) {
-          st = 0;
-          phase ^= 1;
-        }
-        const uint32_t next_k = ring + st * kDqStageBytes;
+        const int k_at = ks.at;
+        ks.next<kKSlots>();
+        vs.next<kVSlots>();
         if (j + 1 < n) {
-          if (!warp_wait(full + 8 * st, phase, w, 93)) break;
+          if (!warp_wait(k_full + 8 * ks.at, ks.phase, w, 93)) break;
           tc_fence_after();
           if (elect_one()) {
-            mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, next_k);
+            mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, k_ring + ks.at * kTileBytes);
             tc_commit(s_full + 8 * ((j + 1) & 1));
           }
           __syncwarp();
+          if (!warp_wait(v_full + 8 * vs.at, vs.phase, w, 93)) break;
           if (!warp_wait(dp_read, j & 1, w, 94)) break;
           tc_fence_after();
           if (elect_one()) {
-            mma_rows(tmem + 256, do_smem, next_k + kTileBytes);
+            mma_rows(tmem + 256, do_smem, v_ring + vs.at * kTileBytes);
             tc_commit(dp_full);
+            if (j + 1 + kVSlots < n) tc_commit(v_empty + 8 * vs.at);
           }
           __syncwarp();
         }
         if (!warp_wait(ds_full, j & 1, w, 95)) break;
         tc_fence_after();
         if (elect_one()) {
-          mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_tile, j > 0);
-          if (j + kDqStages < n) tc_commit(empty + 8 * cur);
+          mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_ring + k_at * kTileBytes, j > 0);
+          if (j + kKSlots < n) tc_commit(k_empty + 8 * k_at);
         }
         __syncwarp();
       }
