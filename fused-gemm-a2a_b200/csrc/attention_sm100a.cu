@@ -599,9 +599,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t kv_full = bars, q_full = bars + 8, q_empty = q_full + 8 * kQSlots, do_full = q_empty + 8 * kQSlots,
                  do_empty = do_full + 8 * kDoSlots, rows_full = do_empty + 8 * kDoSlots,
                  rows_empty = rows_full + 8 * kRowSlots, s_full = rows_empty + 8 * kRowSlots, dp_full = s_full + 8,
-                 p_full = dp_full + 8, ds_full = p_full + 8, acc_done = ds_full + 8, own_bar = acc_done + 8,
+                 p_full = dp_full + 8, ds_full = p_full + 16, acc_done = ds_full + 8, own_bar = acc_done + 8,
                  tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
-  static_assert(8 + 16 * (kQSlots + kDoSlots + kRowSlots) + 48 + 16 <= 256, "barrier area");
+  static_assert(8 + 16 * (kQSlots + kDoSlots + kRowSlots) + 56 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int kv_head = blockIdx.x % P.kv_heads;
@@ -640,6 +640,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
     mbar_init(p_full, 8);
+    mbar_init(p_full + 8, 8);
     mbar_init(ds_full, 8);
     mbar_init(acc_done, 1);
     mbar_init(own_bar, 1);
@@ -656,110 +657,123 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
 
-  if (warp == 8) {
+  if (warp >= 8) {
+    regs_down<80>();
     // ------------------------------------------------------------------ loads
-    if (lane == 0 && !w.dead) {
-      mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
-      load_tile(k_smem, &map_k, kv_full, kv_head, wt.first + wt.row0);
-      load_tile(v_smem, &map_v, kv_full, kv_head, wt.first + wt.row0);
-    }
-    uint32_t own_phase = 0;
-    Slot qs{0, 0}, ds{0, 0};
-    // rows behind the sequence are operands of the sums over queries here, so short tiles are cleared
-    auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int head, int row) {
-      const int valid = wt.len - row;
-      if (valid < kTile) return load_tail(dst, map, full, own_bar, own_phase, head, wt.first + row, valid, lane, w);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(full, kTileBytes);
-        load_tile(dst, map, full, head, wt.first + row);
+    if (warp == 8) {
+      if (lane == 0 && !w.dead) {
+        mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
+        load_tile(k_smem, &map_k, kv_full, kv_head, wt.first + wt.row0);
+        load_tile(v_smem, &map_v, kv_full, kv_head, wt.first + wt.row0);
       }
-      __syncwarp();
-      return true;
-    };
-    for (int i = 0; i < total && !w.dead; ++i) {
-      const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
-      if (i >= kQSlots && !warp_wait(q_empty + 8 * qs.at, qs.phase ^ 1, w, 80)) break;
-      if (!load(&map_q, q_ring + qs.at * kTileBytes, q_full + 8 * qs.at, head, row)) break;
-      if (i >= kDoSlots && !warp_wait(do_empty + 8 * ds.at, ds.phase ^ 1, w, 80)) break;
-      if (!load(&map_do, do_ring + ds.at * kTileBytes, do_full + 8 * ds.at, head, row)) break;
-      qs.next<kQSlots>();
-      ds.next<kDoSlots>();
-    }
-  } else if (warp == 10) {
-    // ------------------------------------------------------------------ row values of the queries
-    Slot rs{0, 0};
-    for (int i = 0; i < total; ++i) {
-      const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
-      const long long at = static_cast<long long>(head) * P.tokens + wt.first + row;
-      float neg[4], delta[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int q = c * 32 + lane;
-        neg[c] = -INFINITY;  // a probability of 0 behind the sequence
-        delta[c] = 0.f;
-        if (row + q < wt.len) {
-          neg[c] = -kLog2e * __ldg(P.lse + at + q);
-          delta[c] = __ldg(P.delta + at + q);
-        }
-      }
-      if (i >= kRowSlots && !warp_wait(rows_empty + 8 * rs.at, rs.phase ^ 1, w, 79)) break;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t to = rows_smem + rs.at * 1024 + (c * 32 + lane) * 4;
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(neg[c]) : "memory");
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512), "f"(delta[c]) : "memory");
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_local(rows_full + 8 * rs.at);
-      rs.next<kRowSlots>();
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ products
-    if (warp_wait(kv_full, 0, w, 81) && warp_wait(q_full, 0, w, 82) && warp_wait(do_full, 0, w, 82)) {
-      tc_fence_after();
-      if (elect_one()) {
-        mma_rows(tmem, k_smem, q_ring);
-        tc_commit(s_full);
-        mma_rows(tmem + 128, v_smem, do_ring);
-        tc_commit(dp_full);
-      }
-      __syncwarp();
+      uint32_t own_phase = 0;
       Slot qs{0, 0}, ds{0, 0};
-#pragma unroll 1
-      for (int i = 0; i < total; ++i) {
-        const int q_at = qs.at, do_at = ds.at;
+      // rows behind the sequence are operands of the sums over queries here, so short tiles are cleared
+      auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int head, int row) {
+        const int valid = wt.len - row;
+        if (valid < kTile) return load_tail(dst, map, full, own_bar, own_phase, head, wt.first + row, valid, lane, w);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full, kTileBytes);
+          load_tile(dst, map, full, head, wt.first + row);
+        }
+        __syncwarp();
+        return true;
+      };
+      for (int i = 0; i < total && !w.dead; ++i) {
+        const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
+        if (i >= kQSlots && !warp_wait(q_empty + 8 * qs.at, qs.phase ^ 1, w, 80)) break;
+        if (!load(&map_q, q_ring + qs.at * kTileBytes, q_full + 8 * qs.at, head, row)) break;
+        if (i >= kDoSlots && !warp_wait(do_empty + 8 * ds.at, ds.phase ^ 1, w, 80)) break;
+        if (!load(&map_do, do_ring + ds.at * kTileBytes, do_full + 8 * ds.at, head, row)) break;
         qs.next<kQSlots>();
         ds.next<kDoSlots>();
-        const bool more = i + 1 < total;
-        if (!warp_wait(p_full, i & 1, w, 83)) break;
-        if (more && !warp_wait(q_full + 8 * qs.at, qs.phase, w, 84)) break;
-        tc_fence_after();
-        if (elect_one()) {
-          mma_weighted(tmem + 256, tmem, do_ring + do_at * kTileBytes, i > 0);
-          if (i + kDoSlots < total) tc_commit(do_empty + 8 * do_at);
-          if (more) {
-            mma_rows(tmem, k_smem, q_ring + qs.at * kTileBytes);
-            tc_commit(s_full);
+      }
+    } else if (warp == 10) {
+      // ------------------------------------------------------------------ row values of the queries
+      Slot rs{0, 0};
+      for (int i = 0; i < total; ++i) {
+        const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
+        const long long at = static_cast<long long>(head) * P.tokens + wt.first + row;
+        float neg[4], delta[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int q = c * 32 + lane;
+          neg[c] = -INFINITY;  // a probability of 0 behind the sequence
+          delta[c] = 0.f;
+          if (row + q < wt.len) {
+            neg[c] = -kLog2e * __ldg(P.lse + at + q);
+            delta[c] = __ldg(P.delta + at + q);
           }
+        }
+        if (i >= kRowSlots && !warp_wait(rows_empty + 8 * rs.at, rs.phase ^ 1, w, 79)) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t to = rows_smem + rs.at * 1024 + (c * 32 + lane) * 4;
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(neg[c]) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512), "f"(delta[c]) : "memory");
         }
         __syncwarp();
-        if (!warp_wait(ds_full, i & 1, w, 85)) break;
-        if (more && !warp_wait(do_full + 8 * ds.at, ds.phase, w, 84)) break;
+        if (lane == 0) mbar_arrive_local(rows_full + 8 * rs.at);
+        rs.next<kRowSlots>();
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------ products
+      if (warp_wait(kv_full, 0, w, 81) && warp_wait(q_full, 0, w, 82) && warp_wait(do_full, 0, w, 82)) {
         tc_fence_after();
         if (elect_one()) {
-          mma_weighted(tmem + 384, tmem + 128, q_ring + q_at * kTileBytes, i > 0);
-          if (i + kQSlots < total) tc_commit(q_empty + 8 * q_at);
-          if (more) {
-            mma_rows(tmem + 128, v_smem, do_ring + ds.at * kTileBytes);
-            tc_commit(dp_full);
-          }
+          mma_rows(tmem, k_smem, q_ring);
+          tc_commit(s_full);
+          mma_rows(tmem + 128, v_smem, do_ring);
+          tc_commit(dp_full);
         }
+        __syncwarp();
+        Slot qs{0, 0}, ds{0, 0};
+#pragma unroll 1
+        for (int i = 0; i < total; ++i) {
+          const int q_at = qs.at, do_at = ds.at;
+          qs.next<kQSlots>();
+          ds.next<kDoSlots>();
+          const bool more = i + 1 < total;
+          const uint32_t do_tile = do_ring + do_at * kTileBytes;
+          if (more && !warp_wait(q_full + 8 * qs.at, qs.phase, w, 84)) break;
+          if (!warp_wait(p_full, i & 1, w, 83)) break;
+          tc_fence_after();
+          if (elect_one()) {
+            mma_weighted_part<2>(tmem + 256, tmem, do_tile, 0, i > 0);
+            mma_weighted_part<2>(tmem + 256, tmem + 64, do_tile, 4, true);
+          }
+          __syncwarp();
+          if (!warp_wait(p_full + 8, i & 1, w, 83)) break;
+          tc_fence_after();
+          if (elect_one()) {
+            mma_weighted_part<2>(tmem + 256, tmem + 16, do_tile, 2, true);
+            mma_weighted_part<2>(tmem + 256, tmem + 80, do_tile, 6, true);
+            if (i + kDoSlots < total) tc_commit(do_empty + 8 * do_at);
+            if (more) {
+              mma_rows(tmem, k_smem, q_ring + qs.at * kTileBytes);
+              tc_commit(s_full);
+            }
+          }
+          __syncwarp();
+          if (!warp_wait(ds_full, i & 1, w, 85)) break;
+          if (more && !warp_wait(do_full + 8 * ds.at, ds.phase, w, 84)) break;
+          tc_fence_after();
+          if (elect_one()) {
+            mma_weighted(tmem + 384, tmem + 128, q_ring + q_at * kTileBytes, i > 0);
+            if (i + kQSlots < total) tc_commit(q_empty + 8 * q_at);
+            if (more) {
+              mma_rows(tmem + 128, v_smem, do_ring + ds.at * kTileBytes);
+              tc_commit(dp_full);
+            }
+          }
+          __syncwarp();
+        }
+        if (!w.dead && elect_one()) tc_commit(acc_done);
         __syncwarp();
       }
-      if (!w.dead && elect_one()) tc_commit(acc_done);
-      __syncwarp();
     }
-  } else if (warp < 8) {
+  } else {
+    regs_up<208>();  // 2 * 128 * 208 + 128 * 80 of the 384 * 168 registers at launch
     // ------------------------------------------------------------------ P and dS
     const int g = warp >> 2, key = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -777,6 +791,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_after();
       F2 p[32];
       const F2 c2 = f2(c);
+      const bool diagonal = P.causal && i % per_head == 0;
+      // 32 columns as BF16 to TMEM; half of the queries at a time, so that their product may begin
+      auto hand_over = [&](int h) {
+        if (diagonal) {  // queries in front of the key do not see it
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int q = g * 64 + h * 32 + 2 * e;
+            float lo, hi;
+            split(p[h * 16 + e], lo, hi);
+            p[h * 16 + e] = f2(q < key ? 0.f : lo, q + 1 < key ? 0.f : hi);
+          }
+        }
+        uint32_t b[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) b[e] = bf16_of_f2(p[h * 16 + e]);
+        tmem_st_32x16(s_tmem + h * 16, b);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(p_full + 8 * h);
+      };
       {
         uint32_t s[2][32];
         tmem_ld_32x32(s_tmem, s[0]);
@@ -789,29 +824,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t* x = &s[v >> 3][(v & 7) * 4 + 2 * e];
-            p[v * 2 + e] = exp2_pair(fma2(f2_of_bits(x[0], x[1]), c2, n[e]));
+            const F2 y = fma2(f2_of_bits(x[0], x[1]), c2, n[e]);
+            p[v * 2 + e] = (v & 1) && e ? exp2_poly(y) : exp2_pair(y);
           }
+          if (v == 7) hand_over(0);
         }
+        hand_over(1);
       }
-      if (P.causal && i % per_head == 0) {  // the diagonal tile: queries in front of the key do not see it
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float lo, hi;
-          split(p[e], lo, hi);
-          p[e] = f2(g * 64 + 2 * e < key ? 0.f : lo, g * 64 + 2 * e + 1 < key ? 0.f : hi);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t b[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) b[e] = bf16_of_f2(p[h * 16 + e]);
-        tmem_st_32x16(s_tmem + h * 16, b);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_local(p_full);
       if (!warp_wait(dp_full, i & 1, w, 87)) {
         alive = false;
         break;
@@ -926,84 +945,88 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
 
-  if (warp == 8) {
+  if (warp >= 8) {
+    regs_down<80>();
     // ------------------------------------------------------------------ loads
-    const int kv_head = head / P.group;
-    if (lane == 0 && !w.dead) {
-      mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
-      load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
-      load_tile(do_smem, &map_do, q_full, head, wt.first + wt.row0);
-    }
-    uint32_t own_phase = 0;
-    Slot ks{0, 0}, vs{0, 0};
-    for (int j = 0; j < n && !w.dead; ++j) {
-      const int row = j * kTile, valid = wt.len - row;
-      const uint32_t k_dst = k_ring + ks.at * kTileBytes, k_bar = k_full + 8 * ks.at;
-      if (j >= kKSlots && !warp_wait(k_empty + 8 * ks.at, ks.phase ^ 1, w, 90)) break;
-      if (valid < kTile) {  // K is also summed over, V only makes scores that are masked
-        if (!load_tail(k_dst, &map_k, k_bar, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
-      } else if (lane == 0) {
-        mbar_arrive_expect_tx(k_bar, kTileBytes);
-        load_tile(k_dst, &map_k, k_bar, kv_head, wt.first + row);
+    if (warp == 8) {
+      const int kv_head = head / P.group;
+      if (lane == 0 && !w.dead) {
+        mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+        load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
+        load_tile(do_smem, &map_do, q_full, head, wt.first + wt.row0);
       }
-      __syncwarp();
-      if (j >= kVSlots && !warp_wait(v_empty + 8 * vs.at, vs.phase ^ 1, w, 90)) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(v_full + 8 * vs.at, kTileBytes);
-        load_tile(v_ring + vs.at * kTileBytes, &map_v, v_full + 8 * vs.at, kv_head, wt.first + row);
-      }
-      __syncwarp();
-      ks.next<kKSlots>();
-      vs.next<kVSlots>();
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ products
-    if (warp_wait(q_full, 0, w, 91) && warp_wait(k_full, 0, w, 92) && warp_wait(v_full, 0, w, 92)) {
-      tc_fence_after();
-      if (elect_one()) {
-        mma_rows(tmem, q_smem, k_ring);
-        tc_commit(s_full);
-        mma_rows(tmem + 256, do_smem, v_ring);
-        tc_commit(dp_full);
-        if (kVSlots < n) tc_commit(v_empty);
-      }
-      __syncwarp();
+      uint32_t own_phase = 0;
       Slot ks{0, 0}, vs{0, 0};
-#pragma unroll 1
-      for (int j = 0; j < n; ++j) {
-        const int k_at = ks.at;
-        ks.next<kKSlots>();
-        vs.next<kVSlots>();
-        if (j + 1 < n) {
-          if (!warp_wait(k_full + 8 * ks.at, ks.phase, w, 93)) break;
-          tc_fence_after();
-          if (elect_one()) {
-            mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, k_ring + ks.at * kTileBytes);
-            tc_commit(s_full + 8 * ((j + 1) & 1));
-          }
-          __syncwarp();
-          if (!warp_wait(v_full + 8 * vs.at, vs.phase, w, 93)) break;
-          if (!warp_wait(dp_read, j & 1, w, 94)) break;
-          tc_fence_after();
-          if (elect_one()) {
-            mma_rows(tmem + 256, do_smem, v_ring + vs.at * kTileBytes);
-            tc_commit(dp_full);
-            if (j + 1 + kVSlots < n) tc_commit(v_empty + 8 * vs.at);
-          }
-          __syncwarp();
-        }
-        if (!warp_wait(ds_full, j & 1, w, 95)) break;
-        tc_fence_after();
-        if (elect_one()) {
-          mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_ring + k_at * kTileBytes, j > 0);
-          if (j + kKSlots < n) tc_commit(k_empty + 8 * k_at);
+      for (int j = 0; j < n && !w.dead; ++j) {
+        const int row = j * kTile, valid = wt.len - row;
+        const uint32_t k_dst = k_ring + ks.at * kTileBytes, k_bar = k_full + 8 * ks.at;
+        if (j >= kKSlots && !warp_wait(k_empty + 8 * ks.at, ks.phase ^ 1, w, 90)) break;
+        if (valid < kTile) {  // K is also summed over, V only makes scores that are masked
+          if (!load_tail(k_dst, &map_k, k_bar, own_bar, own_phase, kv_head, wt.first + row, valid, lane, w)) break;
+        } else if (lane == 0) {
+          mbar_arrive_expect_tx(k_bar, kTileBytes);
+          load_tile(k_dst, &map_k, k_bar, kv_head, wt.first + row);
         }
         __syncwarp();
+        if (j >= kVSlots && !warp_wait(v_empty + 8 * vs.at, vs.phase ^ 1, w, 90)) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(v_full + 8 * vs.at, kTileBytes);
+          load_tile(v_ring + vs.at * kTileBytes, &map_v, v_full + 8 * vs.at, kv_head, wt.first + row);
+        }
+        __syncwarp();
+        ks.next<kKSlots>();
+        vs.next<kVSlots>();
       }
-      if (!w.dead && elect_one()) tc_commit(acc_done);
-      __syncwarp();
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------ products
+      if (warp_wait(q_full, 0, w, 91) && warp_wait(k_full, 0, w, 92) && warp_wait(v_full, 0, w, 92)) {
+        tc_fence_after();
+        if (elect_one()) {
+          mma_rows(tmem, q_smem, k_ring);
+          tc_commit(s_full);
+          mma_rows(tmem + 256, do_smem, v_ring);
+          tc_commit(dp_full);
+          if (kVSlots < n) tc_commit(v_empty);
+        }
+        __syncwarp();
+        Slot ks{0, 0}, vs{0, 0};
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+          const int k_at = ks.at;
+          ks.next<kKSlots>();
+          vs.next<kVSlots>();
+          if (j + 1 < n) {
+            if (!warp_wait(k_full + 8 * ks.at, ks.phase, w, 93)) break;
+            tc_fence_after();
+            if (elect_one()) {
+              mma_rows(tmem + ((j + 1) & 1) * 128, q_smem, k_ring + ks.at * kTileBytes);
+              tc_commit(s_full + 8 * ((j + 1) & 1));
+            }
+            __syncwarp();
+            if (!warp_wait(v_full + 8 * vs.at, vs.phase, w, 93)) break;
+            if (!warp_wait(dp_read, j & 1, w, 94)) break;
+            tc_fence_after();
+            if (elect_one()) {
+              mma_rows(tmem + 256, do_smem, v_ring + vs.at * kTileBytes);
+              tc_commit(dp_full);
+              if (j + 1 + kVSlots < n) tc_commit(v_empty + 8 * vs.at);
+            }
+            __syncwarp();
+          }
+          if (!warp_wait(ds_full, j & 1, w, 95)) break;
+          tc_fence_after();
+          if (elect_one()) {
+            mma_weighted(tmem + 384, tmem + (j & 1) * 128, k_ring + k_at * kTileBytes, j > 0);
+            if (j + kKSlots < n) tc_commit(k_empty + 8 * k_at);
+          }
+          __syncwarp();
+        }
+        if (!w.dead && elect_one()) tc_commit(acc_done);
+        __syncwarp();
+      }
     }
-  } else if (warp < 8) {
+  } else {
+    regs_up<208>();  // 2 * 128 * 208 + 128 * 80 of the 384 * 168 registers at launch
     // ------------------------------------------------------------------ dS
     const int g = warp >> 2, row_in_tile = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -1029,7 +1052,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; ++e)
-          p[e] = exp2_pair(fma2(f2_of_bits(s[e >> 4][2 * (e & 15)], s[e >> 4][2 * (e & 15) + 1]), c2, neg));
+        {
+          const F2 x = fma2(f2_of_bits(s[e >> 4][2 * (e & 15)], s[e >> 4][2 * (e & 15) + 1]), c2, neg);
+          p[e] = (e & 3) == 3 ? exp2_poly(x) : exp2_pair(x);
+        }
       }
       if (!warp_wait(dp_full, j & 1, w, 97)) {
         alive = false;
