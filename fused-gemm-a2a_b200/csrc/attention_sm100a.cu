@@ -45,6 +45,7 @@ struct AttentionParams {
   float* delta;                                 // [heads, tokens]: rowwise sums of d_o * o
   float scale;
   int tiles;                                    // work tiles per head in the grid (an upper bound)
+  int parts;                                    // dK/dV: blocks (one cluster) that share the queries of a tile
   int* status;
   unsigned long long timeout_ns;
 };
@@ -260,14 +261,27 @@ __device__ __forceinline__ void zero_rows(uint16_t* base, int heads, int head, i
 // Teardown shared by the kernels: copies that were issued but never consumed after an abort may still be
 // landing in this block's shared memory.
 __device__ __forceinline__ void settle(WaitCtx& w) {
-  __syncwarp();
-  if (should_abort(w)) {
+  uint32_t aborted;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(aborted) : "r"(w.abort_flag) : "memory");
+  if (aborted != 0 || w.dead) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) nanosleep(1000);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+}
+
+// First thing in a kernel: what takes a trip to global memory and is needed a little later.
+__device__ __forceinline__ bool begin(const AttentionParams& P, const CUtensorMap* a, const CUtensorMap* b,
+                                      const CUtensorMap* c, const CUtensorMap* d) {
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(a);
+    tma_prefetch_desc(b);
+    tma_prefetch_desc(c);
+    if (d != nullptr) tma_prefetch_desc(d);
+  }
+  return ld_relaxed_sys_s32(P.status) != 0;  // an error of an earlier kernel is sticky
 }
 
 // =============================================================================================
@@ -296,7 +310,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                  tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int head = blockIdx.x % P.heads;
+  const bool sticky = begin(P, &map_q, &map_k, &map_v, nullptr);
+  const int head = blockIdx.x % P.heads, kv_head = head / P.group;
   WorkTile wt;
   // the last tiles first: under a causal mask they are the longest
   if (!find_tile(P, 2 * kTile, P.tiles - 1 - static_cast<int>(blockIdx.x / P.heads), wt)) return;
@@ -313,8 +328,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int n1 = wt.row0 + kTile >= wt.len ? 0 : P.causal ? min(all_tiles, wt.row0 / kTile + 2) : all_tiles;
   const int n_max = max(n0, n1);
 
-  WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
-  if (threadIdx.x == 0) {
+  WaitCtx w{P.status, P.timeout_ns, abort_word, sticky};
+  if (warp == 8 && lane == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 1);
       mbar_init(full + 8 * i, 1);
@@ -328,7 +343,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     mbar_init(own_bar, 1);
     asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
     fence_mbar_init();
+    if (!w.dead) {  // Q and K(0) are on their way while the block sets up
+      mbar_arrive_expect_tx(q_full, kTileBytes);
+      load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
+      mbar_arrive_expect_tx(k0_full, kTileBytes);
+      load_tile(k0_smem, &map_k, k0_full, kv_head, wt.first);
+      if (n1 > 0) {
+        mbar_arrive_expect_tx(q_full + 8, kTileBytes);
+        load_tile(q_smem + kTileBytes, &map_q, q_full + 8, head, wt.first + wt.row0 + kTile);
+      }
+    }
   }
+  __syncwarp();
   if (warp == 9) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -342,18 +368,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp >= 8) {
     regs_down<80>();
     if (warp == 8) {
-      // ---------------------------------------------------------------- loads: Q, K(0), then V(j) with K(j + 1)
-      const int kv_head = head / P.group;
-      if (lane == 0 && !w.dead) {
-        mbar_arrive_expect_tx(q_full, kTileBytes);
-        load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
-        mbar_arrive_expect_tx(k0_full, kTileBytes);
-        load_tile(k0_smem, &map_k, k0_full, kv_head, wt.first);
-        if (n1 > 0) {
-          mbar_arrive_expect_tx(q_full + 8, kTileBytes);
-          load_tile(q_smem + kTileBytes, &map_q, q_full + 8, head, wt.first + wt.row0 + kTile);
-        }
-      }
+      // ---------------------------------------------------------------- loads: V(j) with K(j + 1)
       uint32_t own_phase = 0;
       for (int j = 0; j < n_max && !w.dead; ++j) {
         if (j >= 2 && !warp_wait(empty + 8 * (j & 1), ((j >> 1) & 1) ^ 1, w, 60)) break;
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       store_row(o_tmem, q_smem + i * kTileBytes + row_in_tile * kSlotPitch, P.o + (at * P.heads + head) * kDim,
                 l > 0.f || l != l ? 1.f / l : 0.f, valid);
       if (valid) P.lse[static_cast<long long>(head) * P.tokens + at] = (m * c + log2f(l)) * kLn2;
-      bulk_wait_all();
+      bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
     }
   }
   settle(w);
@@ -582,7 +597,13 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const uint16_t* o,
 // Q(i + 1) is needed first and Q(i) is let go last, so Q has three slots and dO two: with two pairs the
 // products waited 2100 cycles per tile for Q. The row values (lse, delta) have a warp and a ring of their own.
 // All of an SM's shared memory is in use: row values and barriers lie in the 3 KiB in front of the tiles.
+//
+// With few key/value tiles and heads, two or four blocks of a cluster share the (head, query tile) list of a
+// tile in equal consecutive pieces. Their sums meet in shared memory: of the four pieces of 128 x 64 values
+// (dV, dK, two halves each) every block finishes 4 / parts, adding what the others send it in the order of
+// their ranks, so the result does not depend on who is first.
 constexpr int kQSlots = 3, kDoSlots = 2, kRowSlots = 2;
+constexpr uint32_t kPiecePitch = 272;  // bytes of 64 FP32 values and a skew against bank conflicts
 constexpr uint32_t kDkvSmem = (2 + kQSlots + kDoSlots) * kTileBytes + 3072;
 static_assert(kDkvSmem <= 227 * 1024 && kRowSlots * 1024 + 256 <= 3072, "shared memory");
 
@@ -604,10 +625,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   static_assert(8 + 16 * (kQSlots + kDoSlots + kRowSlots) + 56 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int kv_head = blockIdx.x % P.kv_heads;
+  const bool sticky = begin(P, &map_q, &map_k, &map_v, &map_do);
+  const int part = P.parts > 1 ? static_cast<int>(cluster_ctarank()) : 0, unit = blockIdx.x / P.parts;
+  const int kv_head = unit % P.kv_heads;
   WorkTile wt;
   // the first tiles first: under a causal mask they have the most queries behind them
-  if (!find_tile(P, kTile, static_cast<int>(blockIdx.x / P.kv_heads), wt)) return;
+  if (!find_tile(P, kTile, unit / P.kv_heads, wt)) return;  // the whole cluster
   if (wt.padding) {
     const int row = wt.first + wt.row0, end = min(row + kTile, wt.first + wt.len);
     zero_rows(P.dk, P.kv_heads, kv_head, row, end);
@@ -616,14 +639,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
   const int q_tiles = (wt.len + kTile - 1) / kTile;
   const int q_first = P.causal ? wt.row0 / kTile : 0;
-  const int per_head = q_tiles - q_first, total = per_head * P.group;
+  const int per_head = q_tiles - q_first, all = per_head * P.group;
+  const int begin_at = static_cast<int>(static_cast<long long>(all) * part / P.parts);
+  const int total = static_cast<int>(static_cast<long long>(all) * (part + 1) / P.parts) - begin_at;
 
-  WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
+  WaitCtx w{P.status, P.timeout_ns, abort_word, sticky};
   if ((front & 1023u) != 0) {  // the tiles would not be where their swizzle needs them
     if (threadIdx.x == 0 && atomicCAS(P.status, 0, kErrPipelineTimeout) == 0) P.status[1] = 78;
     return;
   }
-  if (threadIdx.x == 0) {
+  if (warp == 8 && lane == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < kQSlots; ++i) {
       mbar_init(q_full + 8 * i, 1);
@@ -646,7 +671,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(own_bar, 1);
     asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
     fence_mbar_init();
+    if (!w.dead && total > 0) {  // on their way while the block sets up
+      mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
+      load_tile(k_smem, &map_k, kv_full, kv_head, wt.first + wt.row0);
+      load_tile(v_smem, &map_v, kv_full, kv_head, wt.first + wt.row0);
+    }
   }
+  __syncwarp();
   if (warp == 9) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -661,11 +692,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     regs_down<80>();
     // ------------------------------------------------------------------ loads
     if (warp == 8) {
-      if (lane == 0 && !w.dead) {
-        mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
-        load_tile(k_smem, &map_k, kv_full, kv_head, wt.first + wt.row0);
-        load_tile(v_smem, &map_v, kv_full, kv_head, wt.first + wt.row0);
-      }
       uint32_t own_phase = 0;
       Slot qs{0, 0}, ds{0, 0};
       // rows behind the sequence are operands of the sums over queries here, so short tiles are cleared
@@ -680,7 +706,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         return true;
       };
       for (int i = 0; i < total && !w.dead; ++i) {
-        const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
+        const int head = kv_head * P.group + (begin_at + i) / per_head,
+                  row = (q_first + (begin_at + i) % per_head) * kTile;
         if (i >= kQSlots && !warp_wait(q_empty + 8 * qs.at, qs.phase ^ 1, w, 80)) break;
         if (!load(&map_q, q_ring + qs.at * kTileBytes, q_full + 8 * qs.at, head, row)) break;
         if (i >= kDoSlots && !warp_wait(do_empty + 8 * ds.at, ds.phase ^ 1, w, 80)) break;
@@ -692,7 +719,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // ------------------------------------------------------------------ row values of the queries
       Slot rs{0, 0};
       for (int i = 0; i < total; ++i) {
-        const int head = kv_head * P.group + i / per_head, row = (q_first + i % per_head) * kTile;
+        const int head = kv_head * P.group + (begin_at + i) / per_head,
+                  row = (q_first + (begin_at + i) % per_head) * kTile;
         const long long at = static_cast<long long>(head) * P.tokens + wt.first + row;
         float neg[4], delta[4];
 #pragma unroll
@@ -718,7 +746,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------------ products
-      if (warp_wait(kv_full, 0, w, 81) && warp_wait(q_full, 0, w, 82) && warp_wait(do_full, 0, w, 82)) {
+      if (total > 0 && warp_wait(kv_full, 0, w, 81) && warp_wait(q_full, 0, w, 82) && warp_wait(do_full, 0, w, 82)) {
         tc_fence_after();
         if (elect_one()) {
           mma_rows(tmem, k_smem, q_ring);
@@ -772,6 +800,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
       }
     }
+    if (P.parts > 1) {  // the block's part in the two meetings below
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     regs_up<208>();  // 2 * 128 * 208 + 128 * 80 of the 384 * 168 registers at launch
     // ------------------------------------------------------------------ P and dS
@@ -791,7 +824,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_after();
       F2 p[32];
       const F2 c2 = f2(c);
-      const bool diagonal = P.causal && i % per_head == 0;
+      const bool diagonal = P.causal && (begin_at + i) % per_head == 0;
       // 32 columns as BF16 to TMEM; half of the queries at a time, so that their product may begin
       auto hand_over = [&](int h) {
         if (diagonal) {  // queries in front of the key do not see it
@@ -864,14 +897,104 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       rs.next<kRowSlots>();
     }
-    if (alive && warp_wait(acc_done, 0, w, 88)) {
+    if (P.parts == 1 && alive && warp_wait(acc_done, 0, w, 88)) {
       tc_fence_after();
       const bool valid = wt.row0 + key < wt.len;
       const long long at = (static_cast<long long>(wt.first + wt.row0 + key) * P.kv_heads + kv_head) * kDim;
       // one warpgroup stores dV, the other dK; K and V have been read for the last time
       store_row(tmem + lanes + 256 + g * 128, (g ? k_smem : v_smem) + key * kSlotPitch, (g ? P.dk : P.dv) + at,
                 g ? P.scale : 1.f, valid);
-      bulk_wait_all();
+      bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
+    }
+    if (P.parts > 1) {
+      // Each warpgroup takes every second piece. A block without queries has sums of zero; one that gave up
+      // leaves its pieces unsent, and what is stored then is as invalid as the status word says.
+      const int mine = 4 / P.parts;
+      const bool worker = alive && !w.dead && (total == 0 || warp_wait(acc_done, 0, w, 88));
+      tc_fence_before();
+      __syncwarp();
+      cluster_sync();  // all products of all blocks are done: the tiles' memory is free
+      if (worker) {
+        tc_fence_after();
+        for (int piece = g; piece < 4; piece += 2) {
+          const int owner = piece / mine;
+          if (owner == part) continue;
+          // slot of this block among the owner's senders, and of the piece among the owner's
+          const int from = part - (part > owner ? 1 : 0);
+          const uint32_t to = mapa(k_smem, owner) + ((from * mine + piece % mine) * 128 + key) * kPiecePitch;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[32];
+            if (total > 0) {
+              tmem_ld_32x32(tmem + lanes + 256 + piece * 64 + c * 32, v);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + c * 128 + e * 16), "r"(v[4 * e]),
+                           "r"(v[4 * e + 1]), "r"(v[4 * e + 2]), "r"(v[4 * e + 3])
+                           : "memory");
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync();
+      if (worker) {
+        const bool valid = wt.row0 + key < wt.len;
+        const long long at = (static_cast<long long>(wt.first + wt.row0 + key) * P.kv_heads + kv_head) * kDim;
+        for (int piece = g; piece < 4; piece += 2) {
+          if (piece / mine != part) continue;
+          const uint32_t slot = q_ring + 2 * kTileBytes + (g * 128 + key) * kSlotPitch;  // behind what was received
+          bulk_wait_read_all();
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t own[32];
+            F2 v[16];
+            if (total > 0) {
+              tmem_ld_32x32(tmem + lanes + 256 + piece * 64 + c * 32, own);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) own[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = f2(0.f);
+            for (int rank = 0; rank < P.parts; ++rank) {
+              if (rank == part) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = v[e] + f2_of_bits(own[2 * e], own[2 * e + 1]);
+              } else {
+                const int from = rank - (rank > part ? 1 : 0);
+                const uint32_t at_smem = k_smem + ((from * mine + piece % mine) * 128 + key) * kPiecePitch + c * 128;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  F2 x[2];
+                  shared_pairs(at_smem + e * 16, x);
+                  v[2 * e] = v[2 * e] + x[0];
+                  v[2 * e + 1] = v[2 * e + 1] + x[1];
+                }
+              }
+            }
+            const F2 factor = f2(piece >= 2 ? P.scale : 1.f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + c * 64 + e * 16),
+                           "r"(bf16_of_f2(v[4 * e] * factor)), "r"(bf16_of_f2(v[4 * e + 1] * factor)),
+                           "r"(bf16_of_f2(v[4 * e + 2] * factor)), "r"(bf16_of_f2(v[4 * e + 3] * factor))
+                           : "memory");
+          }
+          fence_proxy_async_shared();
+          if (valid) {
+            bulk_store((piece >= 2 ? P.dk : P.dv) + at + (piece & 1) * 64, slot, 128);
+            bulk_commit();
+          }
+          __syncwarp();
+        }
+        bulk_wait_read_all();
+      }
     }
   }
   settle(w);
@@ -903,7 +1026,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   static_assert(8 + 16 * (kKSlots + kVSlots) + 56 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int head = blockIdx.x % P.heads;
+  const bool sticky = begin(P, &map_q, &map_k, &map_v, &map_do);
+  const int head = blockIdx.x % P.heads, kv_head = head / P.group;
   WorkTile wt;
   if (!find_tile(P, kTile, P.tiles - 1 - static_cast<int>(blockIdx.x / P.heads), wt)) return;
   if (wt.padding) {
@@ -914,8 +1038,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int all_tiles = (wt.len + kTile - 1) / kTile;
   const int n = P.causal ? min(all_tiles, wt.row0 / kTile + 1) : all_tiles;
 
-  WaitCtx w{P.status, P.timeout_ns, abort_word, ld_relaxed_sys_s32(P.status) != 0};
-  if (threadIdx.x == 0) {
+  WaitCtx w{P.status, P.timeout_ns, abort_word, sticky};
+  if (warp == 8 && lane == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < kKSlots; ++i) {
       mbar_init(k_full + 8 * i, 1);
@@ -934,7 +1058,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(own_bar, 1);
     asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
     fence_mbar_init();
+    if (!w.dead) {  // on their way while the block sets up
+      mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+      load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
+      load_tile(do_smem, &map_do, q_full, head, wt.first + wt.row0);
+    }
   }
+  __syncwarp();
   if (warp == 9) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -949,12 +1079,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     regs_down<80>();
     // ------------------------------------------------------------------ loads
     if (warp == 8) {
-      const int kv_head = head / P.group;
-      if (lane == 0 && !w.dead) {
-        mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
-        load_tile(q_smem, &map_q, q_full, head, wt.first + wt.row0);
-        load_tile(do_smem, &map_do, q_full, head, wt.first + wt.row0);
-      }
       uint32_t own_phase = 0;
       Slot ks{0, 0}, vs{0, 0};
       for (int j = 0; j < n && !w.dead; ++j) {
@@ -1098,7 +1222,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       // each warpgroup stores half of the columns; Q and dO have been read for the last time
       store_piece(tmem + lanes + 384 + g * 64, (g ? do_smem : q_smem) + row_in_tile * kSlotPitch,
                   P.dq + (static_cast<long long>(wt.first + row) * P.heads + head) * kDim + g * 64, P.scale, valid);
-      bulk_wait_all();
+      bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
     }
   }
   settle(w);
@@ -1166,6 +1290,18 @@ static long long tile_bound(const AttentionParams& P, int rows) {
                          : P.tokens / rows + static_cast<long long>(P.samples) + 1;
 }
 
+// Blocks of a cluster that share a key/value tile: four while there are fewer tiles than SMs, two while
+// there are fewer than four per SM, to fill the SMs and to even out tiles of unequal length, but only where
+// the mean tile has 16 query tiles or more to walk over (the lengths are not known here, their mean is): a
+// meeting costs about 8 us. 8191 causal tokens in five sequences, 32 heads on 4: 551 us alone, 466 us in
+// twos; 512 tokens, 8 heads, four query tiles each: 13.7 us alone, 19.4 us in fours.
+static int sharing_blocks(const AttentionParams& P, long long units) {
+  const long long sms = sm_count();
+  const long long walk = P.group * ((P.tokens / P.samples + kTile - 1ll) / kTile) / (P.causal ? 2 : 1);
+  if (walk < 16 || units >= 4 * sms) return 1;
+  return units < sms ? 4 : 2;
+}
+
 }  // namespace fga
 
 using namespace fga;
@@ -1216,7 +1352,21 @@ int fga_attention_backward(const FgaAttention* args, void* stream) {
                                                                                                       P.tokens, P.heads);
   FGA_LAUNCHED();
   if ((rc = allow_smem(attention_dkv_kernel, kDkvSmem, g_smem_dkv)) != kSuccess) return rc;
-  attention_dkv_kernel<<<static_cast<unsigned>(tiles * P.kv_heads), kBwdThreads, kDkvSmem, st>>>(q, k, v, d, P);
+  const long long units = tiles * P.kv_heads;
+  P.parts = sharing_blocks(P, units);
+  FGA_REQUIRE(units * P.parts <= 0x7fffffff, "attention: too many heads and sequences for one launch");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(units * P.parts));
+  config.blockDim = dim3(kBwdThreads);
+  config.dynamicSmemBytes = kDkvSmem;
+  config.stream = st;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = static_cast<unsigned>(P.parts);
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  FGA_CUDA(cudaLaunchKernelEx(&config, attention_dkv_kernel, q, k, v, d, P));
   FGA_LAUNCHED();
   if ((rc = allow_smem(attention_dq_kernel, kDqSmem, g_smem_dq)) != kSuccess) return rc;
   attention_dq_kernel<<<static_cast<unsigned>(blocks), kBwdThreads, kDqSmem, st>>>(q, k, v, d, P);

@@ -140,6 +140,8 @@ SHAPES = [
     ([1], 0, 1, 1), ([1, 5, 17], 0, 8, 8), ([127], 0, 2, 1), ([128], 0, 2, 2), ([129], 0, 3, 1), ([255, 1], 0, 4, 2),
     ([256], 5, 2, 1), ([257, 0, 0, 383], 130, 6, 3), ([0], 7, 2, 2), ([0, 3], 0, 1, 1), ([1000], 0, 5, 5),
     ([700, 64, 65, 1, 640], 3, 4, 1), ([2049], 0, 2, 2),
+    # one, two and four blocks that share a key/value tile, with and without a mask
+    ([1500, 549], 0, 32, 16), ([2100], 0, 40, 40), ([1500, 549], 0, 32, 4), ([2100], 0, 64, 16), ([130], 0, 32, 1),
 ]
 
 
