@@ -102,20 +102,35 @@ __device__ __forceinline__ LaneAngle lane_angle(const RotaryParams& P, int lane)
   }
   return a;
 }
+// Sine and cosine of both of a lane's angles. The nearest quarter turn is taken off the fixed-point angle,
+// which leaves |r| <= 1/8 turn; there sin(2 pi r) = r (s0 + s1 r^2 + s2 r^4 + s3 r^6) to a relative 3.3e-9 and
+// cos(2 pi r) = 1 + r^2 (c1 + c2 r^2 + c3 r^4) to 3.3e-8 (fitted by iteratively reweighted least squares), so
+// FP32 rounding dominates. Both angles go through as one packed pair; the general sincospif took a quarter
+// of the kernel's instructions.
 __device__ __forceinline__ void warp_rotation(const RotaryParams& P, const LaneAngle& a, int token, int lane,
                                               float* cosines, float* sines) {
+  float rest[2], c[2], s[2];
+  uint32_t quarter[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const long long at = static_cast<long long>(token) * P.axes + a.axis[i];
     const long long pos = P.pos64 ? __ldg(static_cast<const long long*>(P.pos) + at)
                                   : static_cast<long long>(__ldg(static_cast<const int*>(P.pos) + at));
-    const unsigned long long phase = a.turns[i] * static_cast<unsigned long long>(pos);
-    // top 32 bits as a signed fraction of a turn; sincospi takes half turns
-    const float half_turns = static_cast<float>(static_cast<int>(phase >> 32)) * 4.656612873077393e-10f;  // 2^-31
-    float s, c;
-    sincospif(half_turns, &s, &c);
-    cosines[lane + 32 * i] = c;
-    sines[lane + 32 * i] = s;
+    const uint32_t turn = static_cast<uint32_t>((a.turns[i] * static_cast<unsigned long long>(pos)) >> 32);
+    quarter[i] = (turn + 0x20000000u) >> 30;
+    rest[i] = static_cast<float>(static_cast<int>(turn - (quarter[i] << 30))) * 2.3283064365386963e-10f;  // 2^-32
+  }
+  const F2 r = f2(rest[0], rest[1]), u = r * r;
+  const F2 sine = r * fma2(fma2(fma2(u, f2(-75.3935558f), f2(81.59235342f)), u, f2(-41.34166145f)), u, f2(6.28318529f));
+  const F2 cosine = fma2(fma2(fma2(u, f2(-83.66591204f), f2(64.92322849f)), u, f2(-19.73916726f)), u, f2(1.f));
+  split(cosine, c[0], c[1]);
+  split(sine, s[0], s[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool odd = quarter[i] & 1;
+    const float cs = odd ? s[i] : c[i], sn = odd ? c[i] : s[i];
+    cosines[lane + 32 * i] = (quarter[i] + 1) & 2 ? -cs : cs;  // quarters 1 and 2
+    sines[lane + 32 * i] = quarter[i] & 2 ? -sn : sn;          // quarters 2 and 3
   }
   __syncwarp();
 }
@@ -163,26 +178,24 @@ __device__ __forceinline__ void unpack16(uint4 lower, uint4 upper, F2 (&f)[8]) {
 }
 
 template <bool kInterleaved, bool kBackward, bool kNorm>
-__global__ void __launch_bounds__(32 * kRotaryWarps, kNorm ? 2 : 3) rotary_kernel(const RotaryParams P) {
+__global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3) rotary_kernel(const RotaryParams P) {
   __shared__ float tables[kRotaryWarps][2][64];
   __shared__ float reduce[kBackward && kNorm ? kRotaryWarps : 1][2][kHeadDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane & 7, quarter = lane >> 3;
   const LaneAngle angle = lane_angle(P, lane);
-  uint4 w[2][2];
+  __shared__ uint4 weights[2][kHeadDim / 8];  // registers are short
   F2 dw[2][8];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[t][i] = f2(0.f);
-    if (kNorm && P.w[t] != nullptr) {
-      w[t][0] = load16(P.w[t] + sub * 8);
-      w[t][1] = load16(P.w[t] + 64 + sub * 8);
-    }
+    if (kNorm && P.w[t] != nullptr && threadIdx.x < kHeadDim / 8) weights[t][threadIdx.x] = load16(P.w[t] + threadIdx.x * 8);
   }
+  if (kNorm) __syncthreads();
   // A trip takes four head rows of q, or four of k, so the weight is the same for a whole warp. Four 16-byte
   // loads of a lane are in flight before the first is used: two trips, or one that reads two tensors.
-  constexpr int kAhead = kBackward && kNorm ? 1 : 2;
+  constexpr int kAhead = kNorm ? 1 : 2;
   const int units = P.tokens * P.splits;  // below 2^31: there is more than one split only with few tokens
   const int q_trips = (P.heads[0] + 3) >> 2, trips = q_trips + ((P.heads[1] + 3) >> 2);
   for (int u = blockIdx.x * kRotaryWarps + warp; u < units; u += gridDim.x * kRotaryWarps) {
@@ -236,7 +249,7 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kNorm ? 2 : 3) rotary_kerne
             F2 sq = f[0] * f[0], wt[8];
 #pragma unroll
             for (int i = 1; i < 8; ++i) sq = fma2(f[i], f[i], sq);
-            unpack16(t ? w[1][0] : w[0][0], t ? w[1][1] : w[0][1], wt);
+            unpack16(weights[t][sub], weights[t][8 + sub], wt);
             const F2 rstd = f2(rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps));
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * wt[i];
@@ -249,7 +262,7 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kNorm ? 2 : 3) rotary_kerne
             // Rows that do not exist hold zeros and add nothing.
             F2 x[8], g[8], sq = f2(0.f), dot = f2(0.f);
             unpack16(xraw[n][0], xraw[n][1], x);
-            unpack16(t ? w[1][0] : w[0][0], t ? w[1][1] : w[0][1], g);
+            unpack16(weights[t][sub], weights[t][8 + sub], g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               g[i] = g[i] * f[i];
@@ -776,7 +789,7 @@ int launch_rotary(const RotaryParams& P, int interleaved, bool backward, bool no
 
 int check_rotary(const FgaRotary* a, bool backward, RotaryParams& P) {
   FGA_REQUIRE(a != nullptr, "rotary: null arguments");
-  FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fffffff, "rotary: tokens must be in [1, 2^31)");
+  FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fff0000, "rotary: tokens must be in [1, 2^31 - 2^16]");
   FGA_REQUIRE(a->positions != nullptr && a->inv_freq != nullptr, "rotary: null pointer");
   FGA_REQUIRE(a->axes >= 1 && a->axes <= 4, "rotary: one to four axes");
   int at = 0;
