@@ -7,6 +7,7 @@
 // of per-sample vectors) go through FP32 partial sums in caller-provided scratch and are finished in a
 // fixed order, so results do not depend on scheduling.
 #include <cstdint>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include "../../include/fga.h"
 #include "common.cuh"
@@ -193,104 +194,119 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
     if (kNorm && P.w[t] != nullptr && threadIdx.x < kHeadDim / 8) weights[t][threadIdx.x] = load16(P.w[t] + threadIdx.x * 8);
   }
   if (kNorm) __syncthreads();
-  // A trip takes four head rows of q, or four of k, so the weight is the same for a whole warp. Four 16-byte
-  // loads of a lane are in flight before the first is used: two trips, or one that reads two tensors.
-  constexpr int kAhead = kNorm ? 1 : 2;
+  // A trip takes four head rows of q, or four of k. The loads of the first trip of both are in flight before
+  // the angles are worked out, and of two trips of a tensor before the first is used.
+  struct Trip {
+    uint4 raw[2], x[2];
+  };
   const int units = P.tokens * P.splits;  // below 2^31: there is more than one split only with few tokens
-  const int q_trips = (P.heads[0] + 3) >> 2, trips = q_trips + ((P.heads[1] + 3) >> 2);
   for (int u = blockIdx.x * kRotaryWarps + warp; u < units; u += gridDim.x * kRotaryWarps) {
     const int token = P.splits == 1 ? u : u / P.splits, split_at = u - token * P.splits;
-    bool fresh = true;
     F2 c[4], s[4];
-    for (int trip0 = split_at; trip0 < trips; trip0 += kAhead * P.splits) {
-      uint4 raw[kAhead][2], xraw[kAhead][2];
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 4 * (trip - (t ? q_trips : 0)) + quarter;
-        raw[n][0] = raw[n][1] = xraw[n][0] = xraw[n][1] = make_uint4(0, 0, 0, 0);
-        if (trip < trips && h < P.heads[t]) {
-          const uint16_t* xp = P.x[t] + token * P.x_tok[t] + static_cast<long long>(h) * P.x_head[t] + sub * 8;
-          if constexpr (kBackward) {
-            const uint16_t* gp = P.dy[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8;
-            raw[n][0] = load16(gp);
-            raw[n][1] = load16(gp + 64);
-            if (kNorm && P.w[t] != nullptr) {
-              xraw[n][0] = load16(xp);
-              xraw[n][1] = load16(xp + 64);
-            }
-          } else {
-            raw[n][0] = load16(xp);
-            raw[n][1] = load16(xp + 64);
+    // `tensor` is a compile-time 0 (q) or 1 (k), which keeps the parameters immediate
+    auto load = [&](auto tensor, int trip) {
+      constexpr int t = decltype(tensor)::value;
+      Trip v;
+      v.raw[0] = v.raw[1] = v.x[0] = v.x[1] = make_uint4(0, 0, 0, 0);
+      const int h = 4 * trip + quarter;
+      if (h < P.heads[t]) {
+        const uint16_t* xp = P.x[t] + token * P.x_tok[t] + static_cast<long long>(h) * P.x_head[t] + sub * 8;
+        if constexpr (kBackward) {
+          const uint16_t* gp = P.dy[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8;
+          v.raw[0] = load16(gp);
+          v.raw[1] = load16(gp + 64);
+          if (kNorm && P.w[t] != nullptr) {
+            v.x[0] = load16(xp);
+            v.x[1] = load16(xp + 64);
           }
-        }
-      }
-      if (fresh) {  // behind the first loads, which it hides
-        fresh = false;
-        float *ct = tables[warp][0], *st = tables[warp][1];
-        warp_rotation(P, angle, token, lane, ct, st);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // interleaved: pairs sub*4 .. +3 of the lower half, 32 + sub*4 .. +3 of the upper; else sub*8 .. +7
-          const int at = kInterleaved ? sub * 4 + (i & 1) * 2 + (i >> 1) * 32 : sub * 8 + 2 * i;
-          c[i] = f2(ct[at], ct[at + 1]);
-          s[i] = kBackward ? f2(-st[at], -st[at + 1]) : f2(st[at], st[at + 1]);
-        }
-        __syncwarp();  // the table is rewritten for the next token
-      }
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int trip = trip0 + n * P.splits, t = trip >= q_trips, h = 4 * (trip - (t ? q_trips : 0)) + quarter;
-        if (trip >= trips) break;  // the whole warp
-        const bool active = h < P.heads[t], normed = kNorm && P.w[t] != nullptr;
-        F2 f[8];
-        unpack16(raw[n][0], raw[n][1], f);
-        if constexpr (!kBackward) {
-          if (normed) {
-            F2 sq = f[0] * f[0], wt[8];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) sq = fma2(f[i], f[i], sq);
-            unpack16(weights[t][sub], weights[t][8 + sub], wt);
-            const F2 rstd = f2(rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * wt[i];
-          }
-          rotate16<kInterleaved>(f, c, s);
         } else {
-          rotate16<kInterleaved>(f, c, s);
-          if (normed) {
-            // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n)).
-            // Rows that do not exist hold zeros and add nothing.
-            F2 x[8], g[8], sq = f2(0.f), dot = f2(0.f);
-            unpack16(xraw[n][0], xraw[n][1], x);
-            unpack16(weights[t][sub], weights[t][8 + sub], g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              g[i] = g[i] * f[i];
-              sq = fma2(x[i], x[i], sq);
-              dot = fma2(g[i], x[i], dot);
-            }
-            const float rstd = rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps);
-            const F2 r = f2(rstd), mean = f2(-eight_lane_sum(sum(dot)) * rstd * (1.f / kHeadDim));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * r;
-            if (t == 0) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) dw[0][i] = fma2(f[i], x[i], dw[0][i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) dw[1][i] = fma2(f[i], x[i], dw[1][i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = r * fma2(x[i], mean, g[i]);
-          }
-        }
-        if (active) {
-          uint16_t* op = P.out[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8;
-          store16(op, make_uint4(bf16_of_f2(f[0]), bf16_of_f2(f[1]), bf16_of_f2(f[2]), bf16_of_f2(f[3])));
-          store16(op + 64, make_uint4(bf16_of_f2(f[4]), bf16_of_f2(f[5]), bf16_of_f2(f[6]), bf16_of_f2(f[7])));
+          v.raw[0] = load16(xp);
+          v.raw[1] = load16(xp + 64);
         }
       }
+      return v;
+    };
+    auto turn = [&](auto tensor, int trip, const Trip& v) {
+      constexpr int t = decltype(tensor)::value;
+      const int h = 4 * trip + quarter;
+      const bool normed = kNorm && P.w[t] != nullptr;
+      F2 f[8];
+      unpack16(v.raw[0], v.raw[1], f);
+      if constexpr (!kBackward) {
+        if (normed) {
+          F2 sq = f[0] * f[0], wt[8];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) sq = fma2(f[i], f[i], sq);
+          unpack16(weights[t][sub], weights[t][8 + sub], wt);
+          const F2 rstd = f2(rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * rstd * wt[i];
+        }
+        rotate16<kInterleaved>(f, c, s);
+      } else {
+        rotate16<kInterleaved>(f, c, s);
+        if (normed) {
+          // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n)).
+          // Rows that do not exist hold zeros and add nothing.
+          F2 x[8], g[8], sq = f2(0.f), dot = f2(0.f);
+          unpack16(v.x[0], v.x[1], x);
+          unpack16(weights[t][sub], weights[t][8 + sub], g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            g[i] = g[i] * f[i];
+            sq = fma2(x[i], x[i], sq);
+            dot = fma2(g[i], x[i], dot);
+          }
+          const float rstd = rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps);
+          const F2 r = f2(rstd), mean = f2(-eight_lane_sum(sum(dot)) * rstd * (1.f / kHeadDim));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] = x[i] * r;
+            dw[t][i] = fma2(f[i], x[i], dw[t][i]);
+            f[i] = r * fma2(x[i], mean, g[i]);
+          }
+        }
+      }
+      if (h < P.heads[t]) {
+        uint16_t* op = P.out[t] + (static_cast<long long>(token) * P.heads[t] + h) * kHeadDim + sub * 8;
+        store16(op, make_uint4(bf16_of_f2(f[0]), bf16_of_f2(f[1]), bf16_of_f2(f[2]), bf16_of_f2(f[3])));
+        store16(op + 64, make_uint4(bf16_of_f2(f[4]), bf16_of_f2(f[5]), bf16_of_f2(f[6]), bf16_of_f2(f[7])));
+      }
+    };
+    auto rest = [&](auto tensor, Trip v) {
+      constexpr int t = decltype(tensor)::value;
+      const int trips = (P.heads[t] + 3) >> 2;
+      int trip = split_at;
+      if constexpr (kBackward && kNorm) {  // no registers for a second trip: it reads two tensors
+        if (trip < trips) turn(tensor, trip, v);
+        for (trip += P.splits; trip < trips; trip += P.splits) turn(tensor, trip, load(tensor, trip));
+        return;
+      }
+      for (; trip + P.splits < trips; trip += 2 * P.splits) {
+        const Trip next = load(tensor, trip + P.splits);
+        turn(tensor, trip, v);
+        v = load(tensor, trip + 2 * P.splits);
+        turn(tensor, trip + P.splits, next);
+      }
+      if (trip < trips) turn(tensor, trip, v);
+    };
+    const std::integral_constant<int, 0> q{};
+    const std::integral_constant<int, 1> k{};
+    const Trip q0 = load(q, split_at);
+    Trip k0;
+    if constexpr (!(kBackward && kNorm)) k0 = load(k, split_at);
+    float *ct = tables[warp][0], *st = tables[warp][1];
+    warp_rotation(P, angle, token, lane, ct, st);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // interleaved: pairs sub*4 .. +3 of the lower half, 32 + sub*4 .. +3 of the upper; else sub*8 .. +7
+      const int at = kInterleaved ? sub * 4 + (i & 1) * 2 + (i >> 1) * 32 : sub * 8 + 2 * i;
+      c[i] = f2(ct[at], ct[at + 1]);
+      s[i] = kBackward ? f2(-st[at], -st[at + 1]) : f2(st[at], st[at + 1]);
     }
+    __syncwarp();  // the table is rewritten for the next token
+    rest(q, q0);
+    rest(k, kBackward && kNorm ? load(k, split_at) : k0);
   }
   if constexpr (kBackward && kNorm) {
 #pragma unroll
