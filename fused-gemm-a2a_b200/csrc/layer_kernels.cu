@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
 
 // =============================================================================================
 // Column sums of FP32 partials: out[s][col] (=|+=) sum over slots first(s) .. last(s) of part[slot][col].
-// 32 columns a block, 16 threads a column that each take every 16th slot, joined in order.
+// 128 columns a block (four a lane), 16 warps that each take every 16th slot, joined in order. Widths are
+// multiples of four.
 // =============================================================================================
 struct FinishParams {
   const float* part;       // slot pitch `pitch`
@@ -342,14 +343,14 @@ struct FinishParams {
   int slots;               // samples == 0: slots 0 .. slots-1 go into one row
   const int* cu;           // samples > 0: the slots of sample s are c + s for its row chunks c
   int samples, tokens, chunk_rows;
-  void* out[4];            // up to four results whose partials lie `width` floats apart in a slot
-  int out_f32[4], accumulate[4];
+  void* out[3];            // up to three results whose partials lie `width` floats apart in a slot
+  int out_f32[3], accumulate[3];
 };
 
-__global__ void __launch_bounds__(512) finish_sums_kernel(const FinishParams P) {
-  __shared__ float sums[16][33];
+__global__ void __launch_bounds__(512) finish_sums_kernel(const __grid_constant__ FinishParams P) {
+  __shared__ float4 sums[16][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane, which = blockIdx.y, sample = blockIdx.z;
+  const int col = blockIdx.x * 128 + lane * 4, which = blockIdx.y, sample = blockIdx.z;
   if (P.out[which] == nullptr) return;
   int first = 0, last = P.slots;
   if (P.samples > 0) {
@@ -357,23 +358,34 @@ __global__ void __launch_bounds__(512) finish_sums_kernel(const FinishParams P) 
     first = a / P.chunk_rows + sample;
     last = b > a ? (b - 1) / P.chunk_rows + sample + 1 : first;
   }
-  float v = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (col < P.width) {
     const float* p = P.part + static_cast<long long>(which) * P.width + col;
-#pragma unroll 4
-    for (int i = first + slice; i < last; i += 16) v += p[i * P.pitch];
+#pragma unroll 8
+    for (int i = first + slice; i < last; i += 16) {
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(p + i * P.pitch));
+      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+    }
   }
   sums[slice][lane] = v;
   __syncthreads();
   if (slice == 0 && col < P.width) {
 #pragma unroll
-    for (int k = 1; k < 16; ++k) v += sums[k][lane];
+    for (int k = 1; k < 16; ++k) {
+      const float4 x = sums[k][lane];
+      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+    }
     const long long at = static_cast<long long>(sample) * P.width + col;
     if (P.out_f32[which]) {
       float* o = static_cast<float*>(P.out[which]) + at;
-      *o = P.accumulate[which] ? *o + v : v;
+      const bool add = P.accumulate[which];
+      o[0] = add ? o[0] + v.x : v.x;
+      o[1] = add ? o[1] + v.y : v.y;
+      o[2] = add ? o[2] + v.z : v.z;
+      o[3] = add ? o[3] + v.w : v.w;
     } else {
-      static_cast<__nv_bfloat16*>(P.out[which])[at] = __float2bfloat16(v);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out[which]) + at) =
+          make_uint2(bf16_of_f2(f2(v.x, v.y)), bf16_of_f2(f2(v.z, v.w)));
     }
   }
 }
@@ -647,6 +659,8 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
     clear();
   };
   for (int i = 0; i < kBackwardAhead; ++i) fetch(row0 + i);
+  float next_rstd = row0 < row1 ? __ldg(P.rstd + row0) : 0.f;
+  float next_mean = row0 < row1 && P.mean != nullptr ? __ldg(P.mean + row0) : 0.f;
   RowRange s{P.samples, 0};
   int parity = 0;
   bool fresh = true;
@@ -668,7 +682,11 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
       }
     }
     const bool padding = s.sample >= P.samples;
-    const float rstd = __ldg(P.rstd + row), mean = P.mean != nullptr ? __ldg(P.mean + row) : 0.f;
+    const float rstd = next_rstd, mean = next_mean;
+    if (row + 1 < row1) {  // a trip to memory ahead
+      next_rstd = __ldg(P.rstd + row + 1);
+      if (P.mean != nullptr) next_mean = __ldg(P.mean + row + 1);
+    }
     F2 n[kVec][4], dn[kVec][4], dot2 = f2(0.f), sum2 = f2(0.f);
     copy_wait<kBackwardAhead - 1>();
     const uint32_t slot = mine + (row % kBackwardAhead) * kParts * kVec * piece;
@@ -822,6 +840,7 @@ int check_rotary(const FgaRotary* a, bool backward, RotaryParams& P) {
                 "rotary: null pointer");
     FGA_REQUIRE(aligned16(a->x[t]) && aligned16(a->dy[t]) && aligned16(a->out[t]) && aligned16(a->weight[t]),
                 "rotary: pointers must be 16-byte aligned");
+    FGA_REQUIRE(a->dweight_f32[t] || aligned16(a->dweight[t]), "rotary: pointers must be 16-byte aligned");
     FGA_REQUIRE(a->x_token_stride[t] % 8 == 0 && a->x_head_stride[t] % 8 == 0,
                 "rotary: strides must be multiples of 8 elements");
     P.x[t] = static_cast<const uint16_t*>(a->x[t]);
@@ -851,8 +870,9 @@ int check_norm(const FgaNorm* a, NormParams& P) {
   FGA_REQUIRE(a->samples >= 1 && a->samples <= 65535, "norm: 1 to 65535 samples");
   FGA_REQUIRE(a->cu_seqlens != nullptr || a->samples == 1, "norm: several samples need cu_seqlens");
   FGA_REQUIRE(a->gate == nullptr || a->branch != nullptr, "norm: a gate needs a branch");
-  const void* all[] = {a->x, a->branch, a->weight, a->gate, a->scale, a->shift, a->y, a->r, a->dy, a->dr, a->dx,
-                       a->dbranch, a->scratch};
+  const void* all[] = {a->x,  a->branch, a->weight,  a->gate,  a->scale, a->shift,  a->y,       a->r,
+                       a->dy, a->dr,     a->dx,      a->dbranch, a->dgate, a->dscale, a->dshift, a->scratch,
+                       a->dweight_f32 ? nullptr : a->dweight};
   for (const void* p : all) FGA_REQUIRE(aligned16(p), "norm: pointers must be 16-byte aligned");
   P.x = static_cast<const uint16_t*>(a->x);
   P.branch = static_cast<const uint16_t*>(a->branch);
@@ -905,7 +925,7 @@ int fga_rotary_backward(const FgaRotary* args, void* stream) {
   int rc = check_rotary(args, true, P);
   if (rc != kSuccess) return rc;
   const bool norm = P.w[0] || P.w[1];
-  FGA_REQUIRE(!norm || args->scratch != nullptr, "rotary: weight gradients need scratch");
+  FGA_REQUIRE(!norm || (args->scratch != nullptr && aligned16(args->scratch)), "rotary: weight gradients need scratch");
   P.partial = args->scratch;
   const int grid = rotary_grid(static_cast<long long>(P.tokens) * P.splits, norm, sm_count());
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -921,7 +941,7 @@ int fga_rotary_backward(const FgaRotary* args, void* stream) {
     F.out_f32[t] = args->dweight_f32[t];
     F.accumulate[t] = args->dweight_accumulate[t];
   }
-  finish_sums_kernel<<<dim3(kHeadDim / 32, 2, 1), 512, 0, st>>>(F);
+  finish_sums_kernel<<<dim3(1, 2, 1), 512, 0, st>>>(F);
   FGA_LAUNCHED();
   return kSuccess;
 }
@@ -976,7 +996,7 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
              : run_norm(norm_backward_kernel<2, false>, grid, shape, smem, P, st);
   if (rc != kSuccess) return rc;
   FGA_LAUNCHED();
-  const int blocks = static_cast<int>(ceil_div(P.hidden, 32));
+  const int blocks = static_cast<int>(ceil_div(P.hidden, 128));
   if (args->dweight != nullptr) {
     FinishParams F = {};
     F.part = P.part_weight;
