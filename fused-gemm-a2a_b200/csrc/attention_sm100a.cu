@@ -220,30 +220,6 @@ __device__ __forceinline__ void shared_pairs(uint32_t at, F2 (&v)[2]) {
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[0].v), "=l"(v[1].v) : "r"(at) : "memory");
 }
 __device__ __forceinline__ F2 f2_of_bits(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
-// 2^x of both halves without the special function unit, whose 16 results per cycle bound a softmax that
-// feeds tensor cores of this rate. x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
-// bits of the sum) and |f| <= 1/2; 2^f by the polynomial 1 + c1 f + .. + c4 f^4 of least relative error on that
-// interval (2.8e-6, fitted by iteratively reweighted least squares, constant term fixed), n added to the
-// exponent field. x below -127 gives 0; a NaN stays one.
-__device__ __forceinline__ F2 exp2_poly(F2 x) {
-  float lo, hi;
-  split(x, lo, hi);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
-  x = f2(lo, hi);
-  const F2 magic = f2(12582912.f), minus = f2(-12582912.f);
-  const F2 t = x + magic, n = t + minus, f = fma2(n, f2(-1.f), x);
-  F2 y = fma2(f, f2(0.009582854876057492f), f2(0.05590643239793828f));
-  y = fma2(y, f, f2(0.24024098625996076f));
-  y = fma2(y, f, f2(0.6931241925312817f));
-  y = fma2(y, f, f2(1.f));
-  float tl, th, yl, yh;
-  split(t, tl, th);
-  split(y, yl, yh);
-  const F2 r = f2(__uint_as_float(__float_as_uint(yl) + (__float_as_uint(tl) << 23)),
-                  __uint_as_float(__float_as_uint(yh) + (__float_as_uint(th) << 23)));
-  return fma2(x, f2(0.f), r);
-}
 // 2^x of both halves.
 __device__ __forceinline__ F2 exp2_pair(F2 x) {
   float lo, hi;
@@ -318,8 +294,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (wt.padding) {
     const int row = wt.first + wt.row0, end = min(row + 2 * kTile, wt.first + wt.len);
     zero_rows(P.o, P.heads, head, row, end);
-    for (int r = row + threadIdx.x; r < end; r += blockDim.x)
-      P.lse[static_cast<long long>(head) * P.tokens + r] = -INFINITY;
+    if (P.lse != nullptr)
+      for (int r = row + threadIdx.x; r < end; r += blockDim.x)
+        P.lse[static_cast<long long>(head) * P.tokens + r] = -INFINITY;
     return;
   }
   // key tiles of the two query tiles; a second tile that starts behind the sequence has none
@@ -474,13 +451,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       };
       const F2 c2 = f2(c);
       uint32_t p[2][16];
-      // 32 probabilities; one pair in four by polynomial. One rounding to BF16, the type the products take;
-      // their sum stays FP32 and unrounded.
+      // 32 probabilities, all from the special function unit: a quarter of them by a polynomial of degree four
+      // instead, to relieve it, made the kernel 5 % slower (8192 tokens of packed prompts: 258 against 246 us).
+      // One rounding to BF16, the type the products take; their sum stays FP32 and unrounded.
       auto probabilities = [&](int q, F2 shift, F2& total, uint32_t (&out)[16]) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const F2 x = fma2(f2_of_bits(s[q][2 * e], s[q][2 * e + 1]), c2, shift);
-          const F2 y = (e & 3) == 3 ? exp2_poly(x) : exp2_pair(x);
+          const F2 y = exp2_pair(x);
           total = total + y;
           out[e] = bf16_of_f2(y);
         }
@@ -491,17 +469,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_local(p_full + 16 * i + 8 * part);
       };
-      if (j == 0) {
-        const float top = row_max();
-        m = top == -INFINITY ? 0.f : top;
-      }
-      // The first half goes ahead with the maximum of the tiles before, while this tile's is still being
-      // found; only a row that outgrows it by 2^8 has to start again.
-      F2 shift = f2(-m * c), sum2[2] = {f2(0.f), f2(0.f)};
-      probabilities(0, shift, sum2[0], p[0]);
-      probabilities(1, shift, sum2[1], p[1]);
       const float top = row_max();
-      if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {  // never in the first tile
+      if (j == 0) {
+        m = top == -INFINITY ? 0.f : top;
+      } else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
         // S(j) was issued behind the product that last wrote the output: its arrival covers both
         const float up = fmaxf(m, top), f = exp2_approx((m - up) * c);
         m = up;
@@ -515,11 +486,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
           tmem_st_32x32(o_tmem + q * 32, o);
         }
-        shift = f2(-m * c);
-        sum2[0] = sum2[1] = f2(0.f);
-        probabilities(0, shift, sum2[0], p[0]);
-        probabilities(1, shift, sum2[1], p[1]);
       }
+      const F2 shift = f2(-m * c);
+      F2 sum2[2] = {f2(0.f), f2(0.f)};
+      probabilities(0, shift, sum2[0], p[0]);
+      probabilities(1, shift, sum2[1], p[1]);
       tmem_st_32x16(s_tmem, p[0]);
       tmem_st_32x16(s_tmem + 16, p[1]);
       probabilities(2, shift, sum2[0], p[0]);
@@ -537,7 +508,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       // The query tile has been read by its last product: its shared memory stages the output.
       store_row(o_tmem, q_smem + i * kTileBytes + row_in_tile * kSlotPitch, P.o + (at * P.heads + head) * kDim,
                 l > 0.f || l != l ? 1.f / l : 0.f, valid);
-      if (valid) P.lse[static_cast<long long>(head) * P.tokens + at] = (m * c + log2f(l)) * kLn2;
+      if (valid && P.lse != nullptr) P.lse[static_cast<long long>(head) * P.tokens + at] = (m * c + log2f(l)) * kLn2;
       bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
     }
   }
@@ -551,44 +522,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // =============================================================================================
 // Backward. With P = exp(scale S - lse) and delta = rowsum(dO * O):
 //   dV = P^T dO,   dS = P * (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q.
-// Two kernels recompute S and dP: one owns key/value rows and walks over the queries (of all query heads
-// that share them, so a shared head's gradient is one sum in one accumulator), one owns query rows and
-// walks over the keys. That is 7 tile products where a single kernel would need 5, but dQ is then not
-// summed by atomics across blocks: every run gives the same bits, and no FP32 copy of dQ is kept.
+// Two kernels recompute S and dP: the first owns query rows and walks over the keys for dQ, and finds delta of
+// its rows on the way; the second owns key/value rows and walks over the queries (of all query heads that
+// share them, so a shared head's gradient is one sum in one accumulator). That is 7 tile products where a
+// single kernel would need 5, but dQ is then not summed by atomics across blocks: every run gives the same
+// bits, and no FP32 copy of dQ is kept.
 //
 // In both kernels two warpgroups share a 128 x 128 tile of scores, thread = row, 64 columns each. They
 // write their halves of P or dS as BF16 over their own halves of the scores, 64 columns apart.
 // =============================================================================================
 constexpr int kBwdThreads = 384;
-
-// delta[h, row]: half a warp per row, 8 elements a lane.
-__global__ void __launch_bounds__(256) attention_delta_kernel(const uint16_t* o, const uint16_t* d_o, float* delta,
-                                                              int tokens, int heads) {
-  const long long rows = static_cast<long long>(tokens) * heads;
-  const int sub = threadIdx.x & 15;
-  for (long long first = static_cast<long long>(blockIdx.x) * 16; first < rows;
-       first += static_cast<long long>(gridDim.x) * 16) {  // the whole block goes round together
-    const long long row = first + (threadIdx.x >> 4);
-    const bool on = row < rows;
-    float sum = 0.f;
-    if (on) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(o + row * kDim) + sub);
-      const uint4 b = __ldg(reinterpret_cast<const uint4*>(d_o + row * kDim) + sub);
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sum = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), sum);
-        sum = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), sum);
-      }
-    }
-#pragma unroll
-    for (int m = 8; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    if (on && sub == 0) {
-      const int token = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<long long>(token) * heads);
-      delta[static_cast<long long>(head) * tokens + token] = sum;
-    }
-  }
-}
 
 // ---- dK, dV: S^T and dP^T tiles, rows = keys, columns = queries. TMEM: S^T (then P^T) 0, dP^T (then
 // dS^T) 128, dV 256, dK 384. The tensor cores run dV(i) and S(i+1) while the warps compute dS(i), and
@@ -857,8 +800,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t* x = &s[v >> 3][(v & 7) * 4 + 2 * e];
-            const F2 y = fma2(f2_of_bits(x[0], x[1]), c2, n[e]);
-            p[v * 2 + e] = (v & 1) && e ? exp2_poly(y) : exp2_pair(y);
+            p[v * 2 + e] = exp2_pair(fma2(f2_of_bits(x[0], x[1]), c2, n[e]));
           }
           if (v == 7) hand_over(0);
         }
@@ -1008,7 +950,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // 256, dQ 384. The tensor cores run S(j+1) and dP(j+1) while the warps compute dS(j).
 // K has three slots and V two for the same reason as above.
 constexpr int kKSlots = 3, kVSlots = 2;
-constexpr uint32_t kDqSmem = (2 + kKSlots + kVSlots) * kTileBytes + 256 + 1024;
+constexpr uint32_t kDqSmem = (2 + kKSlots + kVSlots) * kTileBytes + 1024 + 256 + 1024;
 
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1018,7 +960,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_smem = base, do_smem = base + kTileBytes, k_ring = base + 2 * kTileBytes,
                  v_ring = k_ring + kKSlots * kTileBytes;
-  const uint32_t bars = v_ring + kVSlots * kTileBytes;
+  const uint32_t sums_smem = v_ring + kVSlots * kTileBytes;  // halves of the rows' delta
+  const uint32_t bars = sums_smem + 1024;
   const uint32_t q_full = bars, k_full = bars + 8, k_empty = k_full + 8 * kKSlots, v_full = k_empty + 8 * kKSlots,
                  v_empty = v_full + 8 * kVSlots, s_full = v_empty + 8 * kVSlots, dp_full = s_full + 16,
                  dp_read = dp_full + 8, ds_full = dp_read + 8, acc_done = ds_full + 8, own_bar = acc_done + 8,
@@ -1159,7 +1102,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const long long at = wt.first + (valid ? row : 0);
     const F2 c2 = f2(P.scale_log2);
     const F2 neg = f2(-kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at));
-    const F2 delta = f2(-__ldg(P.delta + static_cast<long long>(head) * P.tokens + at));
+    // delta of the row: each of its two threads sums over its 64 columns; kept for the dK/dV kernel
+    F2 partial = f2(0.f);
+    {
+      const long long from = (at * P.heads + head) * kDim + g * 64;
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(P.o + from) + v);
+        const uint4 b = __ldg(reinterpret_cast<const uint4*>(P.d_o + from) + v);
+        partial = fma2(f2_of_bf16(a.x), f2_of_bf16(b.x), partial);
+        partial = fma2(f2_of_bf16(a.y), f2_of_bf16(b.y), partial);
+        partial = fma2(f2_of_bf16(a.z), f2_of_bf16(b.z), partial);
+        partial = fma2(f2_of_bf16(a.w), f2_of_bf16(b.w), partial);
+      }
+    }
+    float own = sum(partial), other;
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (g * 128 + row_in_tile) * 4), "f"(own) : "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(sums_smem + ((1 - g) * 128 + row_in_tile) * 4) : "memory");
+    const float row_delta = g ? other + own : own + other;
+    if (g == 0 && valid) P.delta[static_cast<long long>(head) * P.tokens + at] = row_delta;
+    const F2 delta = f2(-row_delta);
     bool alive = true;
     for (int j = 0; j < n; ++j) {
       const uint32_t s_tmem = tmem + lanes + (j & 1) * 128 + g * 64, dp_tmem = tmem + lanes + 256 + g * 64;
@@ -1176,10 +1139,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; ++e)
-        {
-          const F2 x = fma2(f2_of_bits(s[e >> 4][2 * (e & 15)], s[e >> 4][2 * (e & 15) + 1]), c2, neg);
-          p[e] = (e & 3) == 3 ? exp2_poly(x) : exp2_pair(x);
-        }
+          p[e] = exp2_pair(fma2(f2_of_bits(s[e >> 4][2 * (e & 15)], s[e >> 4][2 * (e & 15) + 1]), c2, neg));
       }
       if (!warp_wait(dp_full, j & 1, w, 97)) {
         alive = false;
@@ -1248,7 +1208,7 @@ static int check_attention(const FgaAttention* a, AttentionParams& P) {
   FGA_REQUIRE(a->samples >= 1 && a->samples <= 65535, "attention: 1 to 65535 sequences");
   FGA_REQUIRE(a->cu_seqlens != nullptr || a->samples == 1, "attention: several sequences need cu_seqlens");
   FGA_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "attention: scale must be positive and finite");
-  FGA_REQUIRE(a->q && a->k && a->v && a->o && a->lse && a->status, "attention: null pointer");
+  FGA_REQUIRE(a->q && a->k && a->v && a->o && a->status, "attention: null pointer");
   for (const void* p : {a->q, a->k, a->v, const_cast<const void*>(a->o)})
     FGA_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "attention: pointers must be 16-byte aligned");
   for (int t = 0; t < 3; ++t)
@@ -1329,7 +1289,7 @@ int fga_attention_backward(const FgaAttention* args, void* stream) {
   AttentionParams P = {};
   int rc = check_attention(args, P);
   if (rc != kSuccess) return rc;
-  FGA_REQUIRE(args->d_o && args->dq && args->dk && args->dv && args->delta, "attention: null pointer");
+  FGA_REQUIRE(args->lse && args->d_o && args->dq && args->dk && args->dv && args->delta, "attention: null pointer");
   for (const void* p : {args->d_o, const_cast<const void*>(args->dq), const_cast<const void*>(args->dk),
                         const_cast<const void*>(args->dv)})
     FGA_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "attention: pointers must be 16-byte aligned");
@@ -1347,9 +1307,8 @@ int fga_attention_backward(const FgaAttention* args, void* stream) {
   FGA_REQUIRE(blocks <= 0x7fffffff, "attention: too many heads and sequences for one launch");
   P.tiles = static_cast<int>(tiles);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const long long row_blocks = (static_cast<long long>(P.tokens) * P.heads + 15) / 16, most = 16ll * sm_count();
-  attention_delta_kernel<<<static_cast<unsigned>(row_blocks < most ? row_blocks : most), 256, 0, st>>>(P.o, P.d_o, P.delta,
-                                                                                                      P.tokens, P.heads);
+  if ((rc = allow_smem(attention_dq_kernel, kDqSmem, g_smem_dq)) != kSuccess) return rc;
+  attention_dq_kernel<<<static_cast<unsigned>(blocks), kBwdThreads, kDqSmem, st>>>(q, k, v, d, P);
   FGA_LAUNCHED();
   if ((rc = allow_smem(attention_dkv_kernel, kDkvSmem, g_smem_dkv)) != kSuccess) return rc;
   const long long units = tiles * P.kv_heads;
@@ -1367,9 +1326,6 @@ int fga_attention_backward(const FgaAttention* args, void* stream) {
   config.attrs = &cluster;
   config.numAttrs = 1;
   FGA_CUDA(cudaLaunchKernelEx(&config, attention_dkv_kernel, q, k, v, d, P));
-  FGA_LAUNCHED();
-  if ((rc = allow_smem(attention_dq_kernel, kDqSmem, g_smem_dq)) != kSuccess) return rc;
-  attention_dq_kernel<<<static_cast<unsigned>(blocks), kBwdThreads, kDqSmem, st>>>(q, k, v, d, P);
   FGA_LAUNCHED();
   return kSuccess;
 }

@@ -280,15 +280,15 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
       if constexpr (kBackward && kNorm) {  // no registers for a second trip: it reads two tensors
         if (trip < trips) turn(tensor, trip, v);
         for (trip += P.splits; trip < trips; trip += P.splits) turn(tensor, trip, load(tensor, trip));
-        return;
+      } else {
+        for (; trip + P.splits < trips; trip += 2 * P.splits) {
+          const Trip next = load(tensor, trip + P.splits);
+          turn(tensor, trip, v);
+          v = load(tensor, trip + 2 * P.splits);
+          turn(tensor, trip + P.splits, next);
+        }
+        if (trip < trips) turn(tensor, trip, v);
       }
-      for (; trip + P.splits < trips; trip += 2 * P.splits) {
-        const Trip next = load(tensor, trip + P.splits);
-        turn(tensor, trip, v);
-        v = load(tensor, trip + 2 * P.splits);
-        turn(tensor, trip + P.splits, next);
-      }
-      if (trip < trips) turn(tensor, trip, v);
     };
     const std::integral_constant<int, 0> q{};
     const std::integral_constant<int, 1> k{};
@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
     }
     __syncwarp();  // the table is rewritten for the next token
     rest(q, q0);
-    rest(k, kBackward && kNorm ? load(k, split_at) : k0);
+    if constexpr (kBackward && kNorm) k0 = load(k, split_at);
+    rest(k, k0);
   }
   if constexpr (kBackward && kNorm) {
 #pragma unroll

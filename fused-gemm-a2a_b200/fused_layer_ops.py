@@ -147,7 +147,7 @@ def _status(device):
 
 
 def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale):
-    args = _native.FgaAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr())
+    args = _native.FgaAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _address(lse))
     args.cu_seqlens, args.status = _address(cu_seqlens), _status(q.device).data_ptr()
     args.timeout_ns = _k.DEVICE_TIMEOUT_NS
     for i, t in enumerate((q, k, v)):
@@ -158,10 +158,10 @@ def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale):
     return args
 
 
-def _attend(q, k, v, cu_seqlens, causal, scale):
+def _attend(q, k, v, cu_seqlens, causal, scale, keep_lse):
     tokens, heads, _ = q.shape
     o = _fresh(q)
-    lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32)
+    lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32) if keep_lse else None
     if tokens:
         _launch(_native.lib().fga_attention_forward, _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale), q.device)
     return o, lse
@@ -169,18 +169,20 @@ def _attend(q, k, v, cu_seqlens, causal, scale):
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, causal, scale):
-        o, lse = _attend(q, k, v, cu_seqlens, causal, scale)
+    def forward(ctx, q, k, v, cu_seqlens, causal, scale, return_lse):
+        o, lse = _attend(q, k, v, cu_seqlens, causal, scale, True)
         ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
         ctx.rule = (causal, scale)
-        ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
+        if not return_lse:
+            return o
+        ctx.mark_non_differentiable(lse)
         return o, lse
 
     @staticmethod
-    def backward(ctx, d_o, _):
+    def backward(ctx, d_o, *_):
         if d_o is None:
-            return (None,) * 6
+            return (None,) * 7
         q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
         d_o = _grad_rows(d_o, o.shape)
         grads = [_fresh(t) for t in (q, k, v)]
@@ -190,7 +192,7 @@ class _Attention(torch.autograd.Function):
             args.d_o, args.delta = d_o.data_ptr(), delta.data_ptr()
             args.dq, args.dk, args.dv = (t.data_ptr() for t in grads)
             _launch(_native.lib().fga_attention_backward, args, q.device)
-        return (*grads, None, None, None)
+        return (*grads, None, None, None, None)
 
 
 def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, return_lse=False):
@@ -224,8 +226,9 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
         if cu_seqlens.shape[0] > 65536:
             raise ValueError('at most 65535 packed sequences')
     _same_device(q, k, v, cu_seqlens)
-    attend = _Attention.apply if _differentiable(q, k, v) else _attend
-    o, lse = attend(q, k, v, cu_seqlens, bool(causal), scale)
+    if _differentiable(q, k, v):
+        return _Attention.apply(q, k, v, cu_seqlens, bool(causal), scale, bool(return_lse))
+    o, lse = _attend(q, k, v, cu_seqlens, bool(causal), scale, return_lse)
     return (o, lse) if return_lse else o
 
 
