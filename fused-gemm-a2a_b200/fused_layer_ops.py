@@ -16,8 +16,6 @@ is no CPU or PyTorch fallback. Calls may be captured into CUDA graphs, backward 
 autograd code, no graph recorded outside the capture may then still hold the same leaves (autograd ties a
 leaf to the stream of the first graph that uses it and would wait on that stream from inside the capture).
 """
-from ctypes import byref
-
 import torch
 
 import _fga_native as _native
@@ -28,7 +26,7 @@ MAX_HIDDEN = 8192
 
 
 def _address(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _same_device(first, *others):
@@ -40,15 +38,16 @@ def _same_device(first, *others):
 
 
 def _launch(entry, args, device):
-    """Call a libfga entry point on the current stream of `device`, whichever device is current."""
+    """Call a libfga entry point with packed arguments on the current stream of `device`, whichever device is
+    current."""
     index = device.index
     if torch.cuda.current_device() == index:
-        rc = entry(byref(args), torch._C._cuda_getCurrentRawStream(index))
+        rc = entry(args, torch._C._cuda_getCurrentRawStream(index))
         if rc:
             _native.check(rc)
         return
     with torch.cuda.device(device):
-        _native.check(entry(byref(args), torch._C._cuda_getCurrentRawStream(index)))
+        _native.check(entry(args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _floats(entry, device, *sizes):
@@ -61,7 +60,7 @@ def _floats(entry, device, *sizes):
 
 def _fresh(t):
     """Contiguous, uninitialised storage for a tensor like `t`."""
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _differentiable(*tensors):
@@ -71,6 +70,10 @@ def _differentiable(*tensors):
 def _head_tensor(t, label):
     """[tokens, heads, 128] BF16 whose heads are contiguous 16-byte aligned rows, with any token and head
     stride that keeps them so."""
+    shape = t.shape
+    if (len(shape) == 3 and shape[2] == HEAD_DIM and shape[1] and t.dtype is torch.bfloat16 and t.is_contiguous()
+            and not t.data_ptr() & 15):
+        return
     if t.ndim != 3 or t.shape[2] != HEAD_DIM or t.dtype != torch.bfloat16:
         raise ValueError(f'{label} must be a BF16 tensor [tokens, heads, {HEAD_DIM}], got {t.dtype} {tuple(t.shape)}')
     if t.shape[1] < 1:
@@ -146,16 +149,14 @@ def _status(device):
     return word
 
 
-def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale):
-    args = _native.FgaAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _address(lse))
-    args.cu_seqlens, args.status = _address(cu_seqlens), _status(q.device).data_ptr()
-    args.timeout_ns = _k.DEVICE_TIMEOUT_NS
-    for i, t in enumerate((q, k, v)):
-        args.token_stride[i], args.head_stride[i] = _strides(t)
-    args.tokens, args.heads, args.kv_heads = q.shape[0], q.shape[1], k.shape[1]
-    args.samples = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    args.causal, args.scale = causal, scale
-    return args
+def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale, d_o=None, dq=None, dk=None, dv=None, delta=None):
+    (q_token, q_head), (k_token, k_head), (v_token, v_head) = _strides(q), _strides(k), _strides(v)
+    tokens, heads, _ = q.shape
+    return _native.ATTENTION_BYTES.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _address(lse), _address(d_o), _address(dq), _address(dk),
+        _address(dv), _address(delta), _address(cu_seqlens), _status(q.device).data_ptr(), _k.DEVICE_TIMEOUT_NS, q_token,
+        k_token, v_token, q_head, k_head, v_head, tokens, heads, k.shape[1],
+        1 if cu_seqlens is None else cu_seqlens.shape[0] - 1, causal, scale)
 
 
 def _attend(q, k, v, cu_seqlens, causal, scale, keep_lse):
@@ -187,11 +188,8 @@ class _Attention(torch.autograd.Function):
         d_o = _grad_rows(d_o, o.shape)
         grads = [_fresh(t) for t in (q, k, v)]
         if q.shape[0]:
-            delta = torch.empty_like(lse)
-            args = _attention_args(q, k, v, o, lse, cu_seqlens, *ctx.rule)
-            args.d_o, args.delta = d_o.data_ptr(), delta.data_ptr()
-            args.dq, args.dk, args.dv = (t.data_ptr() for t in grads)
-            _launch(_native.lib().fga_attention_backward, args, q.device)
+            _launch(_native.lib().fga_attention_backward,
+                    _attention_args(q, k, v, o, lse, cu_seqlens, *ctx.rule, d_o, *grads, torch.empty_like(lse)), q.device)
         return (*grads, None, None, None, None)
 
 
@@ -235,21 +233,17 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
 # ----------------------------------------------------------------------------------------------
 # Rotary positions
 # ----------------------------------------------------------------------------------------------
-def _rotary_args(xs, outs, weights, positions, inv_freq, sections, interleaved, eps):
-    args = _native.FgaRotary()
-    for t in range(2):
-        args.out[t] = outs[t].data_ptr()
-        args.heads[t] = outs[t].shape[1]
-        args.weight[t] = _address(weights[t])
-        if xs[t] is not None:
-            args.x[t] = xs[t].data_ptr()
-            args.x_token_stride[t], args.x_head_stride[t] = _strides(xs[t])
-    args.positions, args.positions_int64 = positions.data_ptr(), positions.dtype == torch.int64
-    args.inv_freq, args.inv_freq_f64 = inv_freq.data_ptr(), inv_freq.dtype == torch.float64
-    args.tokens, args.axes, args.interleaved, args.eps = outs[0].shape[0], len(sections), interleaved, eps
-    for i, pairs in enumerate(sections):
-        args.sections[i] = pairs
-    return args
+def _rotary_args(xs, outs, weights, positions, inv_freq, sections, interleaved, eps, dys=(None, None),
+                 targets=((None, False), (None, False)), scratch=None):
+    (q_token, q_head), (k_token, k_head) = ((0, 0) if x is None else _strides(x) for x in xs)
+    pairs = sections + (0,) * (4 - len(sections))
+    (dwq, add_q), (dwk, add_k) = targets
+    return _native.ROTARY_BYTES.pack(
+        _address(xs[0]), _address(xs[1]), q_token, k_token, q_head, k_head, _address(dys[0]), _address(dys[1]),
+        outs[0].data_ptr(), outs[1].data_ptr(), _address(weights[0]), _address(weights[1]), _address(dwq), _address(dwk),
+        positions.data_ptr(), inv_freq.data_ptr(), _address(scratch), outs[0].shape[0], outs[0].shape[1], outs[1].shape[1],
+        positions.dtype is torch.int64, inv_freq.dtype is torch.float64, len(sections), *pairs, interleaved,
+        dwq is not None and dwq.dtype is torch.float32, dwk is not None and dwk.dtype is torch.float32, add_q, add_k, eps)
 
 
 def _rotate(q, k, q_weight, k_weight, positions, inv_freq, sections, interleaved, eps):
@@ -280,17 +274,12 @@ class _Rotary(torch.autograd.Function):
         targets = [_weight_target(w, needed) for w, needed in zip(ctx.owners, ctx.needs_input_grad[2:4])]
         tokens = outs[0].shape[0]
         if tokens:
-            lib = _native.lib()
-            args = _rotary_args((q, k), outs, (q_weight, k_weight), positions, inv_freq, sections, interleaved, eps)
-            for t, (target, accumulate) in enumerate(targets):
-                args.dy[t] = grads[t].data_ptr()
-                args.dweight[t] = _address(target)
-                args.dweight_f32[t] = target is not None and target.dtype == torch.float32
-                args.dweight_accumulate[t] = accumulate
+            lib, scratch = _native.lib(), None
             if q_weight is not None or k_weight is not None:
-                scratch = _floats(lib.fga_rotary_scratch_floats, positions.device, tokens, args.heads[0], args.heads[1])
-                args.scratch = scratch.data_ptr()
-            _launch(lib.fga_rotary_backward, args, positions.device)
+                scratch = _floats(lib.fga_rotary_scratch_floats, positions.device, tokens, outs[0].shape[1], outs[1].shape[1])
+            _launch(lib.fga_rotary_backward,
+                    _rotary_args((q, k), outs, (q_weight, k_weight), positions, inv_freq, sections, interleaved, eps,
+                                 grads, targets, scratch), positions.device)
         else:
             for target, accumulate in targets:
                 if target is not None and not accumulate:
@@ -343,10 +332,10 @@ def _normalise(x, branch, weight, gate, scale, shift, cu_seqlens, samples, eps, 
     y = torch.empty_like(x)
     r = None if branch is None else torch.empty_like(x)
     if tokens:
-        args = _native.FgaNorm(_address(x), _address(branch), _address(weight), _address(gate), _address(scale),
-                               _address(shift), _address(cu_seqlens), _address(y), _address(r), _address(rstd),
-                               _address(mean))
-        args.tokens, args.hidden, args.samples, args.center, args.eps = tokens, hidden, samples, center, eps
+        args = _native.NORM_BYTES.pack(
+            x.data_ptr(), _address(branch), _address(weight), _address(gate), _address(scale), _address(shift),
+            _address(cu_seqlens), y.data_ptr(), _address(r), _address(rstd), _address(mean), 0, 0, 0, 0, 0, 0, 0, 0, 0,
+            tokens, hidden, samples, center, 0, 0, eps)
         _launch(_native.lib().fga_norm_forward, args, x.device)
     return y, x if r is None else r
 
@@ -383,13 +372,11 @@ class _ResidualNorm(torch.autograd.Function):
             if target is not None or modulated:
                 scratch = _floats(lib.fga_norm_scratch_floats, r.device, tokens, hidden, samples, target is not None,
                                   modulated)
-            args = _native.FgaNorm(None, _address(branch), _address(weight), _address(gate), _address(scale), None,
-                                   _address(cu_seqlens), None, _address(r), _address(rstd), _address(mean),
-                                   _address(dy), _address(dr), _address(dx), _address(dbranch), _address(target),
-                                   *(_address(t) for t in rows), _address(scratch))
-            args.tokens, args.hidden, args.samples, args.center, args.eps = tokens, hidden, samples, center, eps
-            args.dweight_f32 = target is not None and target.dtype == torch.float32
-            args.dweight_accumulate = accumulate
+            args = _native.NORM_BYTES.pack(
+                0, _address(branch), _address(weight), _address(gate), _address(scale), 0, _address(cu_seqlens), 0,
+                r.data_ptr(), rstd.data_ptr(), _address(mean), _address(dy), _address(dr), dx.data_ptr(), _address(dbranch),
+                _address(target), *(_address(t) for t in rows), _address(scratch), tokens, hidden, samples, center,
+                target is not None and target.dtype is torch.float32, accumulate, eps)
             _launch(lib.fga_norm_backward, args, r.device)
         else:
             for t in (*rows, None if accumulate else target):
