@@ -1299,4 +1299,4 @@ class FusedOutputProjection(_CallerOwnedProjection):
 
 
 # Operators around the projections (their own module; part of this module's public surface)
-from fused_layer_ops import packed_attention, residual_norm, rotary_embedding  # noqa: E402,F401
+from fused_layer_ops import check_status, packed_attention, residual_norm, rotary_embedding  # noqa: E402,F401

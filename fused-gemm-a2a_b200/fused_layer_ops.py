@@ -17,6 +17,7 @@ autograd code, no graph recorded outside the capture may then still hold the sam
 leaf to the stream of the first graph that uses it and would wait on that stream from inside the capture).
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 import _fga_native as _native
 import fused_gemm_a2a_kernels as _k
@@ -97,6 +98,11 @@ def _vector(t, length, label):
         raise ValueError(f'{label} must be a contiguous, 16-byte aligned BF16 vector of {length} entries')
 
 
+def _epsilon(eps):
+    if not 0.0 <= eps < float('inf'):
+        raise ValueError('eps must be finite and not negative')
+
+
 def _offsets(cu_seqlens, label='cu_seqlens'):
     if (cu_seqlens.ndim != 1 or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous()
             or cu_seqlens.shape[0] < 2):
@@ -149,6 +155,23 @@ def _status(device):
     return word
 
 
+def check_status(device=None, *, clear=False):
+    """Synchronize and raise if an attention kernel on `device` (default: the current one) gave up on a bounded
+    wait. Such an error is sticky: later attention calls on the device return without computing until it has
+    been cleared, here with clear=True or by a group's clear_status()."""
+    device = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
+    word = _k._local_status.get(device)
+    if word is None:
+        return
+    code, where, detail, _ = word.tolist()
+    if clear:
+        word.zero_()
+    if code:
+        reason = _native.DEVICE_ERRORS.get(code, 'unknown device error')
+        raise RuntimeError(f'Attention device error {code}: {reason} (where={where}, detail={detail}). Outputs and '
+                           'gradients produced since then are not valid')
+
+
 def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale, d_o=None, dq=None, dk=None, dv=None, delta=None):
     (q_token, q_head), (k_token, k_head), (v_token, v_head) = _strides(q), _strides(k), _strides(v)
     tokens, heads, _ = q.shape
@@ -181,6 +204,7 @@ class _Attention(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o, *_):
         if d_o is None:
             return (None,) * 7
@@ -208,8 +232,8 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
 
     Scores, softmax statistics and all sums are FP32; the probabilities (and in the backward pass the
     gradients of the scores) are rounded to BF16 for the second product. Results, gradients included, are
-    the same bits in every run. Kernel waits are bounded as in the projections and report through the
-    status word that comm.check_status() reads."""
+    the same bits in every run. Kernel waits are bounded as in the projections and report through the device's
+    status word, which check_status() and a group's comm.check_status() read."""
     for t, label in ((q, 'q'), (k, 'k'), (v, 'v')):
         _head_tensor(t, label)
     if k.shape != v.shape or k.shape[0] != q.shape[0]:
@@ -266,6 +290,7 @@ class _Rotary(torch.autograd.Function):
         return outs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
         sections, interleaved, eps = ctx.rule
@@ -293,12 +318,11 @@ def rotary_embedding(q, k, positions, inv_freq, sections=None, *, interleaved=Tr
     """Rotary positions of the query and key heads, with several axes: q [tokens, heads, 128], k [tokens,
     kv_heads, 128] BF16 -> new contiguous tensors of the same shapes. One launch for both.
 
-    positions: int32 or int64 [tokens, axes] (or [tokens] for one axis), any integer below 2^31 in size
-    (int64 positions wrap beyond that as int64 products do not: all 64 bits count). inv_freq: FP32 or FP64
-    [64], radians per position of each pair of elements; the first sections[0] pairs turn with axis 0
-    (time), the next sections[1] with axis 1 (height), and so on (default: all with one axis). Pairs are
-    elements (2i, 2i+1) when `interleaved`, (i, i+64) otherwise. Angles are exact modulo a turn whatever
-    the position (64-bit fixed point), so far positions lose nothing.
+    positions: int32 or int64 [tokens, axes] (or [tokens] for one axis), negative ones included. inv_freq:
+    FP32 or FP64 [64], radians per position of each pair of elements; the first sections[0] pairs turn with
+    axis 0 (time), the next sections[1] with axis 1 (height), and so on (default: all with one axis). Pairs
+    are elements (2i, 2i+1) when `interleaved`, (i, i+64) otherwise. Angles are kept modulo a turn in 64-bit
+    fixed point: far positions lose nothing.
 
     q_weight / k_weight (BF16 [128], each optional): the head is first divided by its root mean square
     (mean of squares + eps) and multiplied by the weight, in FP32 with the rotation. Gradients flow to q,
@@ -317,6 +341,7 @@ def rotary_embedding(q, k, positions, inv_freq, sections=None, *, interleaved=Tr
     if (tuple(inv_freq.shape) != (HEAD_DIM // 2,) or inv_freq.dtype not in (torch.float32, torch.float64)
             or not inv_freq.is_contiguous()):
         raise ValueError(f'inv_freq must be a contiguous FP32 or FP64 vector of {HEAD_DIM // 2} frequencies')
+    _epsilon(eps)
     _vector(q_weight, HEAD_DIM, 'q_weight')
     _vector(k_weight, HEAD_DIM, 'k_weight')
     _same_device(q, k, positions, inv_freq, q_weight, k_weight)
@@ -353,6 +378,7 @@ class _ResidualNorm(torch.autograd.Function):
         return y, r
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dr):
         r, branch, weight, gate, scale, cu_seqlens, rstd, mean = ctx.saved_tensors
         samples, eps, center = ctx.rule
@@ -408,6 +434,7 @@ def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=N
         raise ValueError('branch must be a contiguous, 16-byte aligned BF16 tensor of the shape of x')
     if gate is not None and branch is None:
         raise ValueError('gate scales the branch: pass one')
+    _epsilon(eps)
     _vector(weight, hidden, 'weight')
     samples = 1
     if cu_seqlens is not None:

@@ -49,7 +49,7 @@ def test_refusals_of_the_rotary_call():
         ('sections', dict(sections=(65, -1))), ('sections', dict(sections=(16, 16, 16, 8, 8))),
         ('inv_freq', dict(inv_freq=freq[:32])), ('inv_freq', dict(inv_freq=freq.half())),
         ('q_weight', dict(q_weight=torch.ones(64, dtype=bf))), ('k_weight', dict(k_weight=torch.ones(128))),
-        ('CUDA', {}),
+        ('eps', dict(eps=-1e-6)), ('CUDA', {}),
     ]
     for message, change in bad:
         args = dict(q=q, k=k, positions=pos, inv_freq=freq) | change
@@ -71,7 +71,7 @@ def test_refusals_of_the_norm_call():
         ('gate', dict(branch=x, gate=rows.float(), cu_seqlens=cu)),
         ('cu_seqlens', dict(cu_seqlens=cu.long())), ('cu_seqlens', dict(cu_seqlens=cu[:1])),
         ('65535', dict(cu_seqlens=torch.zeros(65537, dtype=torch.int32))),
-        ('CUDA', dict(weight=w)),
+        ('eps', dict(eps=float('nan'))), ('CUDA', dict(weight=w)),
     ]
     for message, change in bad:
         with pytest.raises(ValueError, match=message):
@@ -336,3 +336,37 @@ def test_norm_is_the_same_twice_and_in_a_graph_and_on_a_side_stream(native):
     torch.cuda.synchronize()
     for a, c, d in zip(first, second, captured):
         assert torch.equal(a, c) and torch.equal(a, d)
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_31_elements(native):
+    """Offsets that do not fit 32 bits: the last rows come out like the same rows alone."""
+    rotary, norm = ops()
+    gen = torch.Generator(device='cuda').manual_seed(6)
+    tokens, heads = 540_000, 32                      # 2.2e9 elements
+    q = torch.empty(tokens, heads, 128, dtype=torch.bfloat16, device='cuda')
+    q[:8], q[-8:] = normal(gen, 8, heads, 128), normal(gen, 8, heads, 128)
+    q[8:-8] = 1.0
+    k, w = normal(gen, tokens, 1, 128), normal(gen, 128, mean=1.0)
+    pos, freq = torch.arange(tokens, device='cuda'), frequencies((64,)).cuda()
+    whole = rotary(q, k, pos, freq, q_weight=w)
+    alone = rotary(q[-8:], k[-8:], pos[-8:], freq, q_weight=w)
+    assert torch.equal(whole[0][-8:], alone[0]) and torch.equal(whole[1][-8:], alone[1])
+    dq = torch.autograd.grad(rotary(q.requires_grad_(), k, pos, freq, q_weight=w)[0], q, whole[0])[0]
+    part = q[-8:].detach().requires_grad_()
+    assert torch.equal(dq[-8:], torch.autograd.grad(rotary(part, k[-8:], pos[-8:], freq, q_weight=w)[0], part, whole[0][-8:])[0])
+    del whole, dq
+    x = q.detach().view(-1, 8192)
+    y, r = norm(x, x, weight=normal(gen, 8192, mean=1.0).fill_(0.5))
+    assert torch.equal(r[-2:], (x[-2:].float() * 2).bfloat16())
+    want = plain.residual_norm(x[-2:].double(), x[-2:].double(), torch.full((8192,), 0.5, device='cuda').double())[0]
+    within(y[-2:], want, HALF * want.abs() + FINE * want.abs().max(), 'y')
+
+
+@pytest.mark.gpu
+def test_gradients_are_not_differentiable_twice(native):
+    _, norm = ops()
+    x = torch.ones(4, 64, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+    dx, = torch.autograd.grad(norm(x)[0].float().square().sum(), x, create_graph=True)   # depends on y, so on x
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        dx.float().sum().backward()

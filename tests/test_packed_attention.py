@@ -256,3 +256,63 @@ def test_no_tokens(native):
     o = attention(q, q, q)
     assert o.shape == q.shape
     assert torch.autograd.grad(o.sum(), q)[0].shape == q.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('causal', [False, True])
+def test_thousands_of_short_sequences(native, causal):
+    gen = torch.Generator(device='cuda').manual_seed(10)
+    count, n, heads = 5000, 3, 2
+    q, k, v, do = (normal(gen, count * n, h, 128) for h in (heads, 1, 1, heads))
+    cu = torch.arange(0, count * n + 1, n, dtype=torch.int32, device='cuda')
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = attention(*leaves, cu, causal=causal)
+    flat = [t.detach().double().requires_grad_() for t in leaves]
+    qq, kk, vv = (t.view(count, n, -1, 128).transpose(1, 2) for t in flat)
+    s = qq @ kk.transpose(2, 3) * 128 ** -0.5
+    if causal:
+        s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device='cuda').triu(1), -math.inf)
+    p = s.softmax(-1)
+    o = (p @ vv).transpose(1, 2).reshape(count * n, heads, 128)
+    # rounding of P (2^-8 of sum p|v|) and of the output, and the gradients' chain of four such roundings
+    reach = (p @ vv.abs()).transpose(1, 2).reshape(o.shape)
+    within(got.detach(), o.detach(), (2 * HALF * reach + HALF * o.abs() + 1e-6).detach(), 'o')
+    for a, b in zip(torch.autograd.grad(got, leaves, do), torch.autograd.grad(o, flat, do.double())):
+        error = (a.double() - b).norm() / b.norm()
+        assert error <= 4 * HALF, error
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_31_elements(native):
+    """Offsets that do not fit 32 bits: the last sequence comes out like the same sequence alone."""
+    tokens, heads, n = 540_000, 32, 1000             # 2.2e9 query elements
+    gen = torch.Generator(device='cuda').manual_seed(12)
+    q = torch.ones(tokens, heads, 128, dtype=torch.bfloat16, device='cuda')
+    q[-n:] = normal(gen, n, heads, 128)
+    k, v = normal(gen, tokens, 1, 128), normal(gen, tokens, 1, 128)
+    cu = torch.arange(0, tokens + 1, n, dtype=torch.int32, device='cuda')
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    whole = attention(*leaves, cu, causal=True)
+    grads = torch.autograd.grad(whole, leaves, q.detach())
+    part = [t[-n:].detach().clone().requires_grad_() for t in leaves]
+    alone = attention(*part, causal=True)
+    assert torch.equal(whole[-n:], alone)
+    for a, b in zip(grads, torch.autograd.grad(alone, part, q.detach()[-n:])):
+        # one block or two share a key/value tile, so its sums may be taken in another order
+        assert (a[-n:].double() - b.double()).norm() <= 2 * HALF * b.double().norm()
+
+
+@pytest.mark.gpu
+def test_a_recorded_device_error_is_sticky_and_raises(native):
+    import fused_gemm_a2a
+    import fused_gemm_a2a_kernels as kernels
+    q = torch.ones(4, 1, 128, dtype=torch.bfloat16, device='cuda')
+    attention(q, q, q)
+    fused_gemm_a2a.check_status()
+    word = kernels._local_status[q.device]
+    word[0] = 3
+    attention(q, q, q)                   # returns at once and computes nothing
+    with pytest.raises(RuntimeError, match='pipeline barrier'):
+        fused_gemm_a2a.check_status(clear=True)
+    fused_gemm_a2a.check_status()
+    assert torch.equal(attention(q, q, q), q)
