@@ -446,7 +446,7 @@ __device__ __forceinline__ RowRange range_of(const NormParams& P, int row) {
   return s;
 }
 
-constexpr int kForwardAhead = 4, kBackwardAhead = 3;  // rows in flight, see norm_smem()
+constexpr int kRowsAhead = 2;  // rows in flight: more (3 or 4) cost up to a fifth, see norm_smem()
 
 template <int kVec>
 __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormParams P) {
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
   const uint32_t mine = smem_u32(ring) + threadIdx.x * 16, piece = blockDim.x * 16;
   auto fetch = [&](int row) {  // a group per row, also when there is none left
     if (row < row1) {
-      const uint32_t at = mine + (row % kForwardAhead) * 2 * kVec * piece;
+      const uint32_t at = mine + (row % kRowsAhead) * 2 * kVec * piece;
 #pragma unroll
       for (int k = 0; k < kVec; ++k)
         if (on[k]) {
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
     }
     copy_commit();
   };
-  for (int i = 0; i < kForwardAhead; ++i) fetch(row0 + i);
+  for (int i = 0; i < kRowsAhead; ++i) fetch(row0 + i);
   RowRange s{0, 0};
   int parity = 0;
   for (int row = row0; row < row1; ++row) {
@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
     }
     const bool padding = s.sample >= P.samples;
     F2 r[kVec][4];
-    copy_wait<kForwardAhead - 1>();
-    const uint32_t slot = mine + (row % kForwardAhead) * 2 * kVec * piece;
+    copy_wait<kRowsAhead - 1>();
+    const uint32_t slot = mine + (row % kRowsAhead) * 2 * kVec * piece;
     F2 total = f2(0.f);
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
     float t[1] = {sum(total)};
     block_sum(t, buf[parity], warps);
     parity ^= 1;
-    fetch(row + kForwardAhead);  // this row's pieces are in registers
+    fetch(row + kRowsAhead);  // this row's pieces are in registers
     const float rstd = rsqrtf(t[0] * inv_h + P.eps);
     if (threadIdx.x == 0 && P.rstd != nullptr) {
       P.rstd[row] = rstd;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
   const uint32_t mine = smem_u32(ring) + threadIdx.x * 16, piece = blockDim.x * 16;
   auto fetch = [&](int row) {  // a group per row, also when there is none left
     if (row < row1) {
-      const uint32_t at = mine + (row % kBackwardAhead) * kParts * kVec * piece;
+      const uint32_t at = mine + (row % kRowsAhead) * kParts * kVec * piece;
 #pragma unroll
       for (int k = 0; k < kVec; ++k)
         if (on[k]) {
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
       }
     clear();
   };
-  for (int i = 0; i < kBackwardAhead; ++i) fetch(row0 + i);
+  for (int i = 0; i < kRowsAhead; ++i) fetch(row0 + i);
   float next_rstd = row0 < row1 ? __ldg(P.rstd + row0) : 0.f;
   float next_mean = row0 < row1 && P.mean != nullptr ? __ldg(P.mean + row0) : 0.f;
   RowRange s{P.samples, 0};
@@ -689,8 +689,8 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
       if (P.mean != nullptr) next_mean = __ldg(P.mean + row + 1);
     }
     F2 n[kVec][4], dn[kVec][4], dot2 = f2(0.f), sum2 = f2(0.f);
-    copy_wait<kBackwardAhead - 1>();
-    const uint32_t slot = mine + (row % kBackwardAhead) * kParts * kVec * piece;
+    copy_wait<kRowsAhead - 1>();
+    const uint32_t slot = mine + (row % kRowsAhead) * kParts * kVec * piece;
     const F2 scaled = f2(rstd), offset = f2(-mean * rstd);
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
           store16(P.dbranch + at, padding ? make_uint4(0, 0, 0, 0) : pack8(g));
         }
       }
-    fetch(row + kBackwardAhead);  // what it overwrites this thread has read and used
+    fetch(row + kRowsAhead);  // what it overwrites this thread has read and used
   }
   if (row0 < row1) {
     if (s.sample < P.samples) {
@@ -762,7 +762,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // Rows a norm block walks: the blocks that are resident at once (four on an SM up to 1024 columns, else
-// two) share the rows evenly; at least one row.
+// two) share the rows evenly; at least one row. A forward pass that has no per-sample rows to load takes a
+// fourth of that, so that SMs which are ahead take more (8191 x 5120: 62.5 -> 55.2 us; with gate, scale and
+// shift loaded four times as often 16384 x 4096 went from 90 to 94 us). In the backward pass every block
+// leaves its sums behind.
 int norm_chunk_rows(long long tokens, int hidden, int sms) {
   return static_cast<int>(ceil_div(tokens, (hidden <= 1024 ? 4ll : 2ll) * sms));
 }
@@ -864,7 +867,7 @@ int check_rotary(const FgaRotary* a, bool backward, RotaryParams& P) {
   return kSuccess;
 }
 
-int check_norm(const FgaNorm* a, NormParams& P) {
+int check_norm(const FgaNorm* a, bool backward, NormParams& P) {
   FGA_REQUIRE(a != nullptr, "norm: null arguments");
   FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fffffff, "norm: tokens must be in [1, 2^31)");
   FGA_REQUIRE(a->hidden >= 8 && a->hidden % 8 == 0 && a->hidden <= 8192, "norm: hidden must be a multiple of 8 up to 8192");
@@ -895,7 +898,8 @@ int check_norm(const FgaNorm* a, NormParams& P) {
   P.tokens = static_cast<int>(a->tokens);
   P.hidden = a->hidden;
   P.samples = a->samples;
-  P.chunk_rows = norm_chunk_rows(a->tokens, a->hidden, sm_count());
+  const int rows = norm_chunk_rows(a->tokens, a->hidden, sm_count());
+  P.chunk_rows = backward || a->gate || a->scale || a->shift ? rows : (rows + 3) / 4;
   return kSuccess;
 }
 
@@ -949,7 +953,7 @@ int fga_rotary_backward(const FgaRotary* args, void* stream) {
 
 int fga_norm_forward(const FgaNorm* args, void* stream) {
   NormParams P = {};
-  const int rc = check_norm(args, P);
+  const int rc = check_norm(args, false, P);
   if (rc != kSuccess) return rc;
   FGA_REQUIRE(P.x != nullptr && P.y != nullptr && (P.branch == nullptr) == (P.r == nullptr),
               "norm: x, y, and r exactly where there is a branch");
@@ -957,7 +961,7 @@ int fga_norm_forward(const FgaNorm* args, void* stream) {
   const NormShape shape = norm_shape(P.hidden);
   const int grid = static_cast<int>(ceil_div(P.tokens, P.chunk_rows));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const uint32_t smem = norm_smem(shape, kForwardAhead, 2);
+  const uint32_t smem = norm_smem(shape, kRowsAhead, 2);
   const int rc2 = shape.vec == 1 ? run_norm(norm_forward_kernel<1>, grid, shape, smem, P, st)
                                  : run_norm(norm_forward_kernel<2>, grid, shape, smem, P, st);
   if (rc2 != kSuccess) return rc2;
@@ -973,7 +977,7 @@ int64_t fga_norm_scratch_floats(int64_t tokens, int hidden, int samples, int has
 
 int fga_norm_backward(const FgaNorm* args, void* stream) {
   NormParams P = {};
-  int rc = check_norm(args, P);
+  int rc = check_norm(args, true, P);
   if (rc != kSuccess) return rc;
   P.x = P.r;  // what the forward normalised: the residual sum, or x itself where there is no branch
   const bool modulated = args->dgate || args->dscale || args->dshift;
@@ -988,7 +992,7 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = static_cast<int>(chunks);
   const bool mod = P.gate || P.scale || modulated;
-  const uint32_t smem = norm_smem(shape, kBackwardAhead, mod ? 4 : 3);
+  const uint32_t smem = norm_smem(shape, kRowsAhead, mod ? 4 : 3);
   if (shape.vec == 1)
     rc = mod ? run_norm(norm_backward_kernel<1, true>, grid, shape, smem, P, st)
              : run_norm(norm_backward_kernel<1, false>, grid, shape, smem, P, st);
