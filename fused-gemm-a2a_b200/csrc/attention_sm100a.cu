@@ -1102,9 +1102,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const long long at = wt.first + (valid ? row : 0);
     const F2 c2 = f2(P.scale_log2);
     const F2 neg = f2(-kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at));
-    // delta of the row: each of its two threads sums over its 64 columns; kept for the dK/dV kernel
-    F2 partial = f2(0.f);
-    {
+    // delta of the row, kept for the dK/dV kernel: each of its two threads sums over its 64 columns. Where all
+    // keys lie in one tile it is the sum of P * dP, which needs no rounded output: a row that sees a single key
+    // then gets dS = 0, not the rounding error of its output. (That error is 2^-9 |o| |dO|; beside the spread
+    // of dP it vanishes with the root of the number of keys.)
+    const bool one_tile = n == 1;
+    auto row_sum = [&](float own) {
+      float other;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (g * 128 + row_in_tile) * 4), "f"(own) : "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(sums_smem + ((1 - g) * 128 + row_in_tile) * 4) : "memory");
+      const float all = g ? other + own : own + other;
+      if (g == 0 && valid) P.delta[static_cast<long long>(head) * P.tokens + at] = all;
+      return f2(-all);
+    };
+    F2 delta = f2(0.f);
+    if (!one_tile) {
+      F2 partial = f2(0.f);
       const long long from = (at * P.heads + head) * kDim + g * 64;
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
@@ -1115,14 +1129,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         partial = fma2(f2_of_bf16(a.z), f2_of_bf16(b.z), partial);
         partial = fma2(f2_of_bf16(a.w), f2_of_bf16(b.w), partial);
       }
+      delta = row_sum(sum(partial));
     }
-    float own = sum(partial), other;
-    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (g * 128 + row_in_tile) * 4), "f"(own) : "memory");
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(sums_smem + ((1 - g) * 128 + row_in_tile) * 4) : "memory");
-    const float row_delta = g ? other + own : own + other;
-    if (g == 0 && valid) P.delta[static_cast<long long>(head) * P.tokens + at] = row_delta;
-    const F2 delta = f2(-row_delta);
     bool alive = true;
     for (int j = 0; j < n; ++j) {
       const uint32_t s_tmem = tmem + lanes + (j & 1) * 128 + g * 64, dp_tmem = tmem + lanes + 256 + g * 64;
@@ -1153,18 +1161,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_local(dp_read);
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        p[e] = p[e] * (f2_of_bits(d[e >> 4][2 * (e & 15)], d[e >> 4][2 * (e & 15) + 1]) + delta);
-      if (j == n - 1) {
+      if (j == n - 1) {  // keys behind the sequence, and behind the row under a causal mask
         const int limit = min(wt.len, P.causal ? row + 1 : wt.len) - j * kTile - g * 64;
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           float lo, hi;
           split(p[e], lo, hi);
           p[e] = f2(2 * e >= limit ? 0.f : lo, 2 * e + 1 >= limit ? 0.f : hi);
+          if (2 * e >= limit) d[e >> 4][2 * (e & 15)] = 0;  // may be anything, NaN included
+          if (2 * e + 1 >= limit) d[e >> 4][2 * (e & 15) + 1] = 0;
         }
       }
+      if (one_tile) {
+        F2 partial = f2(0.f);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          partial = fma2(p[e], f2_of_bits(d[e >> 4][2 * (e & 15)], d[e >> 4][2 * (e & 15) + 1]), partial);
+        delta = row_sum(sum(partial));
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        p[e] = p[e] * (f2_of_bits(d[e >> 4][2 * (e & 15)], d[e >> 4][2 * (e & 15) + 1]) + delta);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t b[16];

@@ -316,3 +316,23 @@ def test_a_recorded_device_error_is_sticky_and_raises(native):
         fused_gemm_a2a.check_status(clear=True)
     fused_gemm_a2a.check_status()
     assert torch.equal(attention(q, q, q), q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lengths,causal', [([1] * 40, False), ([1, 2, 3] * 20, True), ([1] + [128] * 3, True)])
+def test_rows_that_see_one_key_have_no_score_gradient(native, lengths, causal):
+    """A row with a single key has P = 1 and dS = 0 whatever its output rounds to: dq = 0, dk only from others."""
+    gen = torch.Generator(device='cuda').manual_seed(13)
+    cu = offsets(lengths)
+    q, k, v, do = (normal(gen, cu[-1], h, 128) for h in (4, 2, 2, 4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = attention(*leaves, torch.tensor(cu, dtype=torch.int32, device='cuda'), causal=causal)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    for a, b in plain.segments(cu, cu[-1]):
+        alone = slice(a, b if b - a == 1 else a + 1 if causal else a)
+        # FP32: the product of 128 terms and the exponential of a score minus its own logarithm
+        assert (dq[alone].abs() <= 128 * 2.0 ** -20 * 40).all()
+        if b - a == 1:
+            assert (dk[a:b].abs() <= 2 * 128 * 2.0 ** -20 * 40).all()
+            want = do[a:b].double().view(1, 2, 2, 128).sum(2)
+            within(dv[a:b], want, HALF * want.abs() + 1e-5, 'dv')
