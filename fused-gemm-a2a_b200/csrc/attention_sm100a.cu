@@ -558,15 +558,15 @@ constexpr int kBwdThreads = 384;
 // their ranks, so the result does not depend on who is first.
 constexpr int kQSlots = 3, kDoSlots = 2, kRowSlots = 2;
 constexpr uint32_t kPiecePitch = 272;  // bytes of 64 FP32 values and a skew against bank conflicts
-constexpr uint32_t kDkvSmem = (2 + kQSlots + kDoSlots) * kTileBytes + 3072;
-static_assert(kDkvSmem <= 227 * 1024 && kRowSlots * 1024 + 256 <= 3072, "shared memory");
+constexpr uint32_t kDkvSmem = (2 + kQSlots + kDoSlots) * kTileBytes + 3 * 1024;
+static_assert(kDkvSmem <= 227 * 1024 && kRowSlots * 1024 + 256 <= 3 * 1024, "shared memory");
 
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                          const __grid_constant__ AttentionParams P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const uint32_t front = smem_u32(smem_raw), base = front + 3072;
+  const uint32_t front = smem_u32(smem_raw), base = front + 3 * 1024;
   const uint32_t k_smem = base, v_smem = base + kTileBytes, q_ring = base + 2 * kTileBytes,
                  do_ring = q_ring + kQSlots * kTileBytes;
   const uint32_t rows_smem = front;  // per slot: -lse * log2(e) [128], delta [128]
