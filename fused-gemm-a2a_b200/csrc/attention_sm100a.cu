@@ -1235,7 +1235,8 @@ static int check_attention(const FgaAttention* a, AttentionParams& P) {
               "attention: query heads must be a multiple of key/value heads");
   FGA_REQUIRE(a->samples >= 1 && a->samples <= 65535, "attention: 1 to 65535 sequences");
   FGA_REQUIRE(a->cu_seqlens != nullptr || a->samples == 1, "attention: several sequences need cu_seqlens");
-  FGA_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "attention: scale must be positive and finite");
+  // far from where scale * log2(e) would overflow, or flush to 0 and make 0 * -inf of a masked score
+  FGA_REQUIRE(a->scale >= 1e-30f && a->scale <= 1e30f, "attention: scale must be from 1e-30 to 1e30");
   FGA_REQUIRE(a->q && a->k && a->v && a->o && a->status, "attention: null pointer");
   for (const void* p : {a->q, a->k, a->v, const_cast<const void*>(a->o)})
     FGA_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "attention: pointers must be 16-byte aligned");

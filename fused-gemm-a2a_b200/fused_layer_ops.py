@@ -226,7 +226,8 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
     cu_seqlens: sequence offsets (default: all tokens are one sequence); a token sees the tokens of its own
     sequence, with `causal` those up to itself. Lengths may be anything, zero and one included. Rows behind
     the last sequence give o = 0 and gradients of 0, and what they hold in q, k, v and in the incoming
-    gradient is not looked at. scale: positive, default 128 ** -0.5. return_lse: also return the FP32
+    gradient is not looked at. A NaN or infinity inside a sequence may reach every row of that sequence, of
+    others none. scale: positive, default 128 ** -0.5. return_lse: also return the FP32
     [heads, tokens] logarithms of the rows' sums of exponentials (-inf behind the last sequence; no gradient
     flows through them).
 
@@ -241,8 +242,8 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
     if q.shape[1] % k.shape[1]:
         raise ValueError('Query heads must be a multiple of key/value heads')
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float('inf'):
-        raise ValueError('scale must be positive and finite')
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError('scale must be positive, from 1e-30 to 1e30')
     if cu_seqlens is not None:
         _offsets(cu_seqlens)
         if cu_seqlens.shape[0] > 65536:

@@ -300,9 +300,9 @@ int fga_norm_backward(const FgaNorm* args, void* stream);
 /* Attention over packed sequences: o = softmax(scale * q k^T) v for each sequence and query head, with
  * causal only over keys at or before the query's position; query head h reads key/value head
  * h / (heads / kv_heads). lse[h, row] is the natural logarithm of the row's sum of exponentials. Rows
- * behind the last sequence: o = 0, lse = -inf, all gradients 0. lse may be NULL in the forward. scale > 0.
- * status and timeout_ns as for
- * the GEMMs; the calls of a device share its status word, whatever their streams.
+ * behind the last sequence: o = 0, lse = -inf, all gradients 0. lse may be NULL in the forward. scale:
+ * from 1e-30 to 1e30. status and timeout_ns as for the GEMMs; the calls of a device share its status word,
+ * whatever their streams.
  * backward reads q, k, v, o, lse and the contiguous gradient d_o, and writes contiguous dq, dk, dv;
  * delta: scratch of heads * tokens floats. The results do not depend on scheduling: no atomics. */
 typedef struct FgaAttention {

@@ -370,3 +370,24 @@ def test_gradients_are_not_differentiable_twice(native):
     dx, = torch.autograd.grad(norm(x)[0].float().square().sum(), x, create_graph=True)   # depends on y, so on x
     with pytest.raises(RuntimeError, match='once_differentiable'):
         dx.float().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('used', ['y', 'r'])
+@pytest.mark.parametrize('modulated', [False, True])
+def test_norm_gradients_where_one_output_is_not_used(native, used, modulated):
+    _, norm = ops()
+    gen = torch.Generator(device='cuda').manual_seed(15)
+    t = dict(x=normal(gen, 70, 256), branch=normal(gen, 70, 256), weight=normal(gen, 256, mean=1.0), gate=None, scale=None,
+             shift=None)
+    if modulated:
+        t.update({n: normal(gen, 2, 256, std=0.5) for n in ('gate', 'scale', 'shift')})
+    cu, g, none = [0, 33, 70], normal(gen, 70, 256), torch.zeros(70, 256, dtype=torch.bfloat16, device='cuda')
+    leaves = {n: None if v is None else v.detach().requires_grad_() for n, v in t.items()}
+    outs = norm(leaves['x'], leaves['branch'], **{n: leaves[n] for n in ('weight', 'gate', 'scale', 'shift')},
+                cu_seqlens=torch.tensor(cu, dtype=torch.int32, device='cuda'))
+    present = [n for n in leaves if leaves[n] is not None]
+    got = torch.autograd.grad(outs[used == 'r'], [leaves[n] for n in present], g)
+    _, _, grads, bounds = norm_bounds(t, cu, False, g if used == 'y' else none, g if used == 'r' else none, True)
+    for name, value in zip(present, got):
+        within(value, grads[name], bounds[name], name)

@@ -39,7 +39,7 @@ def test_refusals():
             ('BF16', dict(q=q.float())), ('BF16', dict(q=q.half())), ('BF16', dict(k=k[..., :64])), ('BF16', dict(v=k[0])),
             ('head', dict(k=k[:, :0], v=k[:, :0])), ('one shape', dict(v=q)), ('tokens', dict(k=k[:5], v=k[:5])),
             ('multiple', dict(k=q[:, :3], v=q[:, :3])), ('scale', dict(scale=0.0)), ('scale', dict(scale=-1.0)),
-            ('scale', dict(scale=math.inf)), ('scale', dict(scale=math.nan)),
+            ('scale', dict(scale=math.inf)), ('scale', dict(scale=math.nan)), ('scale', dict(scale=1e-40)),
             ('strides', dict(q=torch.zeros(6, 4, 256, dtype=bf)[..., ::2])),
             ('strides', dict(v=torch.zeros(6, 1, 128, dtype=bf).expand(6, 2, 128))),
             ('strides', dict(q=torch.zeros(6 * 4 * 128 + 4, dtype=bf)[4:].view(6, 4, 128))),
@@ -336,3 +336,17 @@ def test_rows_that_see_one_key_have_no_score_gradient(native, lengths, causal):
             assert (dk[a:b].abs() <= 2 * 128 * 2.0 ** -20 * 40).all()
             want = do[a:b].double().view(1, 2, 2, 128).sum(2)
             within(dv[a:b], want, HALF * want.abs() + 1e-5, 'dv')
+
+
+@pytest.mark.gpu
+def test_gradients_of_some_inputs_only(native):
+    gen = torch.Generator(device='cuda').manual_seed(14)
+    q, k, v, do = (normal(gen, 200, h, 128) for h in (4, 2, 2, 4))
+    full = [t.detach().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(attention(*full), full, do)
+    for i in range(3):
+        some = [t.detach().requires_grad_(n == i) for n, t in enumerate((q, k, v))]
+        assert torch.equal(torch.autograd.grad(attention(*some), some[i], do)[0], want[i])
+    o, lse = attention(*full, return_lse=True)
+    assert not lse.requires_grad
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(o, full, do), want))
