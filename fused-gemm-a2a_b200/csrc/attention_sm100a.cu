@@ -1113,34 +1113,45 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const long long at = wt.first + (valid ? row : 0);
     const F2 c2 = f2(P.scale_log2);
     const F2 neg = f2(-kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at));
-    // delta of the row, kept for the dK/dV kernel: each of its two threads sums over its 64 columns. Where all
-    // keys lie in one tile it is the sum of P * dP, which needs no rounded output: a row that sees a single key
-    // then gets dS = 0, not the rounding error of its output. (That error is 2^-9 |o| |dO|; beside the spread
-    // of dP it vanishes with the root of the number of keys.)
+    // delta of the rows, kept for the dK/dV kernel. Where all keys lie in one tile it is the sum of P * dP, which
+    // needs no rounded output: a row that sees a single key then gets dS = 0, not the rounding error of its
+    // output. (That error is 2^-9 |o| |dO|; beside the spread of dP it vanishes with the root of the number of
+    // keys.)
     const bool one_tile = n == 1;
-    auto row_sum = [&](float own) {
-      float other;
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (g * 128 + row_in_tile) * 4), "f"(own) : "memory");
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(sums_smem + ((1 - g) * 128 + row_in_tile) * 4) : "memory");
-      const float all = g ? other + own : own + other;
+    auto keep_delta = [&](float all) {
       if (g == 0 && valid) P.delta[static_cast<long long>(head) * P.tokens + at] = all;
       return f2(-all);
     };
+    auto shared_float = [&](int i) {
+      float v;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(sums_smem + i * 4) : "memory");
+      return v;
+    };
     F2 delta = f2(0.f);
-    if (!one_tile) {
-      F2 partial = f2(0.f);
-      const long long from = (at * P.heads + head) * kDim + g * 64;
+    if (!one_tile) {  // o * dO, half a warp per row
+      uint4 o[8], d[8];
+      const int half = lane >> 4, sub = lane & 15;
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(P.o + from) + v);
-        const uint4 b = __ldg(reinterpret_cast<const uint4*>(P.d_o + from) + v);
-        partial = fma2(f2_of_bf16(a.x), f2_of_bf16(b.x), partial);
-        partial = fma2(f2_of_bf16(a.y), f2_of_bf16(b.y), partial);
-        partial = fma2(f2_of_bf16(a.z), f2_of_bf16(b.z), partial);
-        partial = fma2(f2_of_bf16(a.w), f2_of_bf16(b.w), partial);
+        const int r = wt.row0 + warp * 16 + 2 * v + half;
+        const long long from = (static_cast<long long>(wt.first + min(r, wt.len - 1)) * P.heads + head) * kDim + sub * 8;
+        o[v] = __ldg(reinterpret_cast<const uint4*>(P.o + from));
+        d[v] = __ldg(reinterpret_cast<const uint4*>(P.d_o + from));
       }
-      delta = row_sum(sum(partial));
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        F2 partial = f2_of_bf16(o[v].x) * f2_of_bf16(d[v].x);
+        partial = fma2(f2_of_bf16(o[v].y), f2_of_bf16(d[v].y), partial);
+        partial = fma2(f2_of_bf16(o[v].z), f2_of_bf16(d[v].z), partial);
+        partial = fma2(f2_of_bf16(o[v].w), f2_of_bf16(d[v].w), partial);
+        float all = sum(partial);
+#pragma unroll
+        for (int m = 8; m; m >>= 1) all += __shfl_xor_sync(0xffffffffu, all, m);
+        if (sub == 0)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (warp * 16 + 2 * v + half) * 4), "f"(all) : "memory");
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      delta = keep_delta(shared_float(row_in_tile));
     }
     bool alive = true;
     for (int j = 0; j < n; ++j) {
@@ -1188,7 +1199,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int e = 0; e < 32; ++e)
           partial = fma2(p[e], f2_of_bits(d[e >> 4][2 * (e & 15)], d[e >> 4][2 * (e & 15) + 1]), partial);
-        delta = row_sum(sum(partial));
+        const float own = sum(partial);  // the other 64 columns are the other warpgroup's
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (g * 128 + row_in_tile) * 4), "f"(own) : "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        delta = keep_delta(shared_float(row_in_tile) + shared_float(128 + row_in_tile));
       }
 #pragma unroll
       for (int e = 0; e < 32; ++e)
