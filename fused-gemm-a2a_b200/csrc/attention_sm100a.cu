@@ -273,8 +273,9 @@ __device__ __forceinline__ bool begin(const AttentionParams& P, const CUtensorMa
 // What bounds it: an iteration (256 queries x 128 keys) takes 3150 cycles where its products take 2048. A
 // tile's softmax is 1690 of them (1024 for 16384 exponentials at 16 per cycle), then come the rest of P V and
 // the next S (640) and the latencies of two hand-overs; both tiles run that chain half a period apart. An
-// issuing warp for each tile, one hand-over instead of two, or a polynomial in place of a quarter of the
-// exponentials were no faster or slower. 16383 tokens x 8 heads: 1.0 ms, 1.1 PFLOP/s at the 1.6 GHz that the
+// issuing warp for each tile (263 against 247 us for the packed prompts below), key tiles of 64 with two score
+// buffers per query tile (271 us), one hand-over instead of two (the same) and a polynomial in place of a
+// quarter of the exponentials (258 us) do not shorten it. 16383 tokens x 8 heads: 1.0 ms, 1.1 PFLOP/s at the 1.6 GHz that the
 // power limit leaves; 8192 tokens of packed causal prompts, 32 heads on 8: 240 us, 0.84 PFLOP/s.
 // =============================================================================================
 constexpr int kFwdThreads = 384;
