@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(512) finish_sums_kernel(const __grid_constant_
 // what it will read itself, so a row costs one barrier (two when centred) for its sums.
 //
 // Bound by memory: 8191 x 5120 with a residual sum 53 us (6.3 TB/s), 16384 x 4096 centred with gate, scale
-// and shift 90 us forward (6.0 TB/s) and 158 us backward (5.1 TB/s: six streams, 48 FP32 column sums a
+// and shift 90 us forward (6.0 TB/s) and 134 us backward (6.0 TB/s: six streams, 48 FP32 column sums a
 // thread).
 // =============================================================================================
 struct NormParams {
@@ -593,7 +593,6 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
   const int row0 = blockIdx.x * P.chunk_rows, row1 = min(row0 + P.chunk_rows, P.tokens);
   const int vecs = P.hidden >> 3;
   const float inv_h = 1.f / P.hidden;
-  uint4 wt[kVec], gt[kVec], sc[kVec];
   F2 sa[kVec][4], dg[kVec][4], dh[kVec][4];
   bool on[kVec];
   int col[kVec];
@@ -608,11 +607,22 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
     const int v = threadIdx.x + k * blockDim.x;
     on[k] = v < vecs;
     col[k] = v * 8;
-    wt[k] = gt[k] = sc[k] = make_uint4(0, 0, 0, 0);
-    if (on[k] && P.weight != nullptr) wt[k] = load16(P.weight + col[k]);
   }
   clear();
   const uint32_t mine = smem_u32(ring) + threadIdx.x * 16, piece = blockDim.x * 16;
+  // weight, gate and scale of this thread's columns, behind the rows in flight: registers are short
+  const uint32_t kept = mine + kRowsAhead * kParts * kVec * piece;
+  auto keep = [&](int which, int k, const uint16_t* from) {
+    const uint4 v = load16(from);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(kept + (which * kVec + k) * piece), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+  };
+  auto kept_row = [&](int which, int k) { return shared16(kept + (which * kVec + k) * piece); };
+  if (P.weight != nullptr)
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (on[k]) keep(0, k, P.weight + col[k]);
   auto fetch = [&](int row) {  // a group per row, also when there is none left
     if (row < row1) {
       const uint32_t at = mine + (row % kRowsAhead) * kParts * kVec * piece;
@@ -633,9 +643,10 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
       if (on[k]) {
+        const uint4 none = make_uint4(0, 0, 0, 0);
         F2 w[4], a[4];
-        unpack8(wt[k], w);
-        unpack8(sc[k], a);
+        unpack8(P.weight != nullptr ? kept_row(0, k) : none, w);
+        unpack8(kMod && P.scale != nullptr ? kept_row(2, k) : none, a);
         auto put = [&](float* at, const F2(&v)[4], bool add) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -684,8 +695,8 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
         for (int k = 0; k < kVec; ++k)
           if (on[k]) {
             const long long at = static_cast<long long>(s.sample) * P.hidden + col[k];
-            if (P.gate != nullptr) gt[k] = load16(P.gate + at);
-            if (P.scale != nullptr) sc[k] = load16(P.scale + at);
+            if (P.gate != nullptr) keep(1, k, P.gate + at);
+            if (P.scale != nullptr) keep(2, k, P.scale + at);
           }
       }
     }
@@ -712,12 +723,12 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
           if (kMod) dh[k][i] = dh[k][i] + dn[k][i];
         }
         if (kMod && P.scale != nullptr) {
-          unpack8(sc[k], e);
+          unpack8(kept_row(2, k), e);
 #pragma unroll
           for (int i = 0; i < 4; ++i) dn[k][i] = fma2(dn[k][i], e[i], dn[k][i]);
         }
         if (P.weight != nullptr) {
-          unpack8(wt[k], e);
+          unpack8(kept_row(0, k), e);
 #pragma unroll
           for (int i = 0; i < 4; ++i) dn[k][i] = dn[k][i] * e[i];
         }
@@ -744,7 +755,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
         if (kMod && P.dbranch != nullptr) {
           F2 b[4], g[4];
           unpack8(shared16(slot + (3 * kVec + k) * piece), b);
-          unpack8(gt[k], g);
+          unpack8(kept_row(1, k), g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (!padding) dg[k][i] = fma2(d[i], b[i], dg[k][i]);
@@ -787,8 +798,8 @@ NormShape norm_shape(int hidden) {
   return {vec, static_cast<int>(ceil_div(ceil_div(vecs, vec), 32) * 32)};
 }
 
-// Bytes of the rows in flight: `ahead` rows of `parts` tensors, 16 bytes a thread and vector.
-uint32_t norm_smem(NormShape s, int ahead, int parts) { return 16u * s.vec * s.threads * ahead * parts; }
+// Bytes of the rows in flight, `parts` tensors each, and of `kept` rows beside them: 16 bytes a thread and vector.
+uint32_t norm_smem(NormShape s, int parts, int kept) { return 16u * s.vec * s.threads * (kRowsAhead * parts + kept); }
 
 int run_norm(void (*kernel)(NormParams), int grid, NormShape shape, uint32_t smem, const NormParams& P, cudaStream_t st) {
   if (smem > 40 * 1024)  // beside the static arrays, 48 KiB need no leave
@@ -968,7 +979,7 @@ int fga_norm_forward(const FgaNorm* args, void* stream) {
   const NormShape shape = norm_shape(P.hidden);
   const int grid = static_cast<int>(ceil_div(P.tokens, P.chunk_rows));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const uint32_t smem = norm_smem(shape, kRowsAhead, 2);
+  const uint32_t smem = norm_smem(shape, 2, 0);
   const int rc2 = shape.vec == 1 ? run_norm(norm_forward_kernel<1>, grid, shape, smem, P, st)
                                  : run_norm(norm_forward_kernel<2>, grid, shape, smem, P, st);
   if (rc2 != kSuccess) return rc2;
@@ -999,7 +1010,7 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = static_cast<int>(chunks);
   const bool mod = P.gate || P.scale || modulated;
-  const uint32_t smem = norm_smem(shape, kRowsAhead, mod ? 4 : 3);
+  const uint32_t smem = norm_smem(shape, mod ? 4 : 3, mod ? 3 : 1);
   if (shape.vec == 1)
     rc = mod ? run_norm(norm_backward_kernel<1, true>, grid, shape, smem, P, st)
              : run_norm(norm_backward_kernel<1, false>, grid, shape, smem, P, st);
