@@ -205,6 +205,16 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
   for (int u = blockIdx.x * kRotaryWarps + warp; u < units; u += gridDim.x * kRotaryWarps) {
     const int token = P.splits == 1 ? u : u / P.splits, split_at = u - token * P.splits;
     F2 c[4], s[4];
+    const float *ct = tables[warp][0], *st = tables[warp][1];
+    auto angles = [&]() {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // interleaved: pairs sub*4 .. +3 of the lower half, 32 + sub*4 .. +3 of the upper; else sub*8 .. +7
+        const int at = kInterleaved ? sub * 4 + (i & 1) * 2 + (i >> 1) * 32 : sub * 8 + 2 * i;
+        c[i] = f2(ct[at], ct[at + 1]);
+        s[i] = kBackward ? f2(-st[at], -st[at + 1]) : f2(st[at], st[at + 1]);
+      }
+    };
     // `tensor` is a compile-time 0 (q) or 1 (k), which keeps the parameters immediate
     auto load = [&](auto tensor, int trip) {
       constexpr int t = decltype(tensor)::value;
@@ -246,6 +256,7 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
         }
         rotate16<kInterleaved>(f, c, s);
       } else {
+        if constexpr (kNorm) angles();  // from shared memory every time: registers are short
         rotate16<kInterleaved>(f, c, s);
         if (normed) {
           // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n)).
@@ -297,16 +308,9 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
     const Trip q0 = load(q, split_at);
     Trip k0;
     if constexpr (!(kBackward && kNorm)) k0 = load(k, split_at);
-    float *ct = tables[warp][0], *st = tables[warp][1];
-    warp_rotation(P, angle, token, lane, ct, st);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // interleaved: pairs sub*4 .. +3 of the lower half, 32 + sub*4 .. +3 of the upper; else sub*8 .. +7
-      const int at = kInterleaved ? sub * 4 + (i & 1) * 2 + (i >> 1) * 32 : sub * 8 + 2 * i;
-      c[i] = f2(ct[at], ct[at + 1]);
-      s[i] = kBackward ? f2(-st[at], -st[at + 1]) : f2(st[at], st[at + 1]);
-    }
-    __syncwarp();  // the table is rewritten for the next token
+    __syncwarp();  // the table of the last token has been read
+    warp_rotation(P, angle, token, lane, tables[warp][0], tables[warp][1]);
+    if constexpr (!(kBackward && kNorm)) angles();
     rest(q, q0);
     if constexpr (kBackward && kNorm) k0 = load(k, split_at);
     rest(k, k0);
