@@ -61,8 +61,8 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
 // cosines once for all heads. Eight lanes hold a head row, each 8 elements of its lower and 8 of its upper
 // half, so both kinds of pairs turn inside a lane; a warp takes four head rows at a time. The first version
 // (16 lanes a row, scalar arithmetic) issued 870 instructions per token of 8 heads and was bound by that, at
-// 3.7 TB/s. Now 131072 tokens x (4 + 4) heads with head norms take 99 us forward (5.4 TB/s) and 163 us
-// backward (4.9 TB/s; its registers hold it to 16 warps an SM), 16384 x (32 + 8) without norms 54 us
+// 3.7 TB/s. Now 131072 tokens x (4 + 4) heads with head norms take 99 us forward (5.4 TB/s) and 158 us
+// backward (5.1 TB/s; its registers hold it to 16 warps an SM), 16384 x (32 + 8) without norms 54 us
 // (6.2 TB/s, where a plain copy measures 6.55).
 // =============================================================================================
 constexpr int kRotaryWarps = 8;
