@@ -891,7 +891,8 @@ int check_rotary(const FgaRotary* a, bool backward, RotaryParams& P) {
 
 int check_norm(const FgaNorm* a, bool backward, NormParams& P) {
   FGA_REQUIRE(a != nullptr, "norm: null arguments");
-  FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fffffff, "norm: tokens must be in [1, 2^31)");
+  // 2^16 rows of room: a chunk's end and the rows fetched ahead of it are 32-bit sums
+  FGA_REQUIRE(a->tokens >= 1 && a->tokens <= 0x7fff0000, "norm: tokens must be in [1, 2^31 - 2^16]");
   FGA_REQUIRE(a->hidden >= 8 && a->hidden % 8 == 0 && a->hidden <= 8192, "norm: hidden must be a multiple of 8 up to 8192");
   FGA_REQUIRE(a->samples >= 1 && a->samples <= 65535, "norm: 1 to 65535 samples");
   FGA_REQUIRE(a->cu_seqlens != nullptr || a->samples == 1, "norm: several samples need cu_seqlens");

@@ -420,11 +420,12 @@ def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=N
     one pass. Returns (y, r); without a branch r is x. All BF16; sums and statistics in FP32, y computed
     from the unrounded r.
 
-    x, branch: contiguous [tokens, hidden], hidden a multiple of 8 up to 8192. The norm divides by the root
-    mean square of the row, after subtracting its mean with `center` (a layer norm). weight: [hidden].
-    gate, scale, shift: [samples, hidden], one row for each packed sequence of cu_seqlens (one sample, or
-    [hidden], without it). With cu_seqlens, rows behind the last sequence have a gate of 0
-    and y = 0, and pass dr through to x in the backward pass. Gradients flow to everything but cu_seqlens."""
+    x, branch: contiguous [tokens, hidden], hidden a multiple of 8 up to 8192, at most 2^31 - 2^16 tokens.
+    The norm divides by the root mean square of the row, after subtracting its mean with `center` (a layer
+    norm). weight: [hidden]. gate, scale, shift: [samples, hidden], one row for each packed sequence of
+    cu_seqlens (one sample, or [hidden], without it). With cu_seqlens, rows behind the last sequence have a
+    gate of 0 and y = 0, and pass dr through to x in the backward pass. Gradients flow to everything but
+    cu_seqlens."""
     if x.ndim != 2 or x.dtype != torch.bfloat16 or not x.is_contiguous() or x.data_ptr() % 16:
         raise ValueError('x must be a contiguous, 16-byte aligned BF16 tensor [tokens, hidden]')
     tokens, hidden = x.shape

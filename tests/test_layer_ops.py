@@ -106,6 +106,16 @@ def test_the_c_entries_refuse_what_the_kernels_cannot_do(native):
         assert native.fga_rotary_forward(ctypes.byref(broken), None) == -1 and message in native.fga_last_error()
 
 
+@pytest.mark.parametrize('tokens', [(1 << 31) - 1, (1 << 31) - (1 << 16) + 1])
+def test_norm_rows_leave_room_for_32_bit_sums(native, tokens):
+    import ctypes
+
+    import _fga_native as api
+    norm = api.FgaNorm(16, tokens=tokens, hidden=8, samples=1)
+    for entry in (native.fga_norm_forward, native.fga_norm_backward):
+        assert entry(ctypes.byref(norm), None) == -1 and b'tokens' in native.fga_last_error()
+
+
 def test_gradients_of_the_plain_forms_against_differences():
     g = torch.Generator().manual_seed(3)
 
