@@ -159,7 +159,9 @@ def check_status(device=None, *, clear=False):
     """Synchronize and raise if an attention kernel on `device` (default: the current one) gave up on a bounded
     wait. Such an error is sticky: later attention calls on the device return without computing until it has
     been cleared, here with clear=True or by a group's clear_status()."""
-    device = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
+    device = torch.device('cuda' if device is None else device)
+    if device.index is None:
+        device = torch.device('cuda', torch.cuda.current_device())
     word = _k._local_status.get(device)
     if word is None:
         return

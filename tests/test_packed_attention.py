@@ -31,6 +31,16 @@ def offsets(lengths):
 
 
 # ----------------------------------------------------------------------------------------- CPU
+@pytest.mark.parametrize('device', [None, 'cuda', 'cuda:1', torch.device('cuda'), 1])
+def test_check_status_reads_the_current_device_for_every_way_to_name_it(monkeypatch, device):
+    import fused_gemm_a2a_kernels as kernels
+    import fused_layer_ops
+    monkeypatch.setattr(kernels, '_local_status', {torch.device('cuda', 1): torch.tensor([3, 70, 5, 0])})
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 1)
+    with pytest.raises(RuntimeError, match='device error 3'):
+        fused_layer_ops.check_status(device)
+
+
 def test_refusals():
     bf = torch.bfloat16
     q, k = torch.zeros(6, 4, 128, dtype=bf), torch.zeros(6, 2, 128, dtype=bf)
