@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(512) finish_sums_kernel(const __grid_constant_
 // y = n * weight * (1 + scale) + shift.  gate, scale and shift are one row per packed sample.
 //
 // A block takes a chunk of consecutive rows, a thread the same 8 * kVec columns of each, so weight,
-// scale, shift and gate stay in registers from row to row and the column sums of the backward pass are
+// scale, shift and gate stay on the SM from row to row (forward in registers, backward in shared memory: see
+// norm_smem()) and the column sums of the backward pass are
 // register sums over the chunk. Slot chunk + sample of the partial sums is unique: walking down the rows
 // either of the two grows. The next rows are on their way to shared memory meanwhile, each thread fetching
 // what it will read itself, so a row costs one barrier (two when centred) for its sums.
@@ -588,6 +589,10 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
 // dx = dr + dc;  dbranch = gate * dx;  sums over the rows of a sample: dgate = sum dx * branch,
 // dshift = sum dy, a = sum dy * n, from which dscale = a * weight and dweight gets (1 + scale) * a. The
 // mean over a centred row of dc is rstd * mean(dn), because the mean of n is zero up to rounding.
+//
+// n comes from r as the forward pass stored it: one rounding to BF16 (at most 2^-9 of r) that y does not have.
+// Gradients are then 2.4e-3 from 64 bits in the 2-norm, where rounding them alone gives 1.7e-3; computing
+// r again would read x and the branch in place of r, five streams instead of four in a pass bound by memory.
 template <int kVec, bool kMod>
 __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormParams P) {
   __shared__ float buf[2][64];
