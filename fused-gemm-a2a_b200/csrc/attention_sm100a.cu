@@ -248,7 +248,8 @@ __device__ __forceinline__ void settle(WaitCtx& w) {
   __syncthreads();
 }
 
-// First thing in a kernel: what takes a trip to global memory and is needed a little later.
+// First thing in a kernel: what takes a trip to global memory and is needed a little later. The answer is the
+// same for the lanes of a warp, which go on to wait together.
 __device__ __forceinline__ bool begin(const AttentionParams& P, const CUtensorMap* a, const CUtensorMap* b,
                                       const CUtensorMap* c, const CUtensorMap* d) {
   if (threadIdx.x == 0) {
@@ -257,7 +258,7 @@ __device__ __forceinline__ bool begin(const AttentionParams& P, const CUtensorMa
     tma_prefetch_desc(c);
     if (d != nullptr) tma_prefetch_desc(d);
   }
-  return ld_relaxed_sys_s32(P.status) != 0;  // an error of an earlier kernel is sticky
+  return __any_sync(0xffffffffu, ld_relaxed_sys_s32(P.status) != 0);  // an error of an earlier kernel is sticky
 }
 
 // =============================================================================================
@@ -977,8 +978,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t q_full = bars, k_full = bars + 8, k_empty = k_full + 8 * kKSlots, v_full = k_empty + 8 * kKSlots,
                  v_empty = v_full + 8 * kVSlots, s_full = v_empty + 8 * kVSlots, dp_full = s_full + 16,
                  dp_read = dp_full + 8, ds_full = dp_read + 8, acc_done = ds_full + 8, own_bar = acc_done + 8,
-                 tmem_slot = own_bar + 8, abort_word = tmem_slot + 8;
-  static_assert(8 + 16 * (kKSlots + kVSlots) + 56 + 16 <= 256, "barrier area");
+                 sums_full = own_bar + 8, tmem_slot = sums_full + 8, abort_word = tmem_slot + 8;
+  static_assert(8 + 16 * (kKSlots + kVSlots) + 64 + 16 <= 256, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const bool sticky = begin(P, &map_q, &map_k, &map_v, &map_do);
@@ -1011,6 +1012,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(ds_full, 8);
     mbar_init(acc_done, 1);
     mbar_init(own_bar, 1);
+    mbar_init(sums_full, 8);
     asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_word), "r"(0u) : "memory");
     fence_mbar_init();
     if (!w.dead) {  // on their way while the block sets up
@@ -1151,7 +1153,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (sub == 0)
           asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (warp * 16 + 2 * v + half) * 4), "f"(all) : "memory");
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // all eight warps: none has waited for anything yet
       delta = keep_delta(shared_float(row_in_tile));
     }
     bool alive = true;
@@ -1202,7 +1204,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           partial = fma2(p[e], f2_of_bits(d[e >> 4][2 * (e & 15)], d[e >> 4][2 * (e & 15) + 1]), partial);
         const float own = sum(partial);  // the other 64 columns are the other warpgroup's
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(sums_smem + (g * 128 + row_in_tile) * 4), "f"(own) : "memory");
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        // a barrier with a limit: a warp that gave up on a wait above never comes here
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(sums_full);
+        if (!warp_wait(sums_full, 0, w, 99)) {
+          alive = false;
+          break;
+        }
         delta = keep_delta(shared_float(row_in_tile) + shared_float(128 + row_in_tile));
       }
 #pragma unroll

@@ -81,6 +81,22 @@ def test_the_c_entry_refuses_what_the_kernels_cannot_do(native):
     assert native.fga_attention_forward(ctypes.byref(broken), None) == -1 and b'strides' in native.fga_last_error()
 
 
+def test_barriers_without_a_limit_stand_in_front_of_every_wait_that_may_give_up():
+    """A warp that gives up on a bounded wait leaves for the end of its block. Another warp of its role that
+    then met it at a named barrier, which has no limit, would wait for good."""
+    import os
+    import re
+    import build_native
+    source = open(os.path.join(build_native.CSRC, 'attention_sm100a.cu')).read()
+    found = 0
+    for kernel in source.split('__global__')[1:]:
+        for role in re.split(r'// -{20,}', kernel):
+            for barrier in re.finditer(r'\bbar(rier)?\.(cta\.)?(sync|red)\b', role):
+                found += 1
+                assert 'wait' not in re.sub(r'(tmem_ld|tmem_st|bulk)_wait', '', role[:barrier.start()]), role[:80].strip()
+    assert found
+
+
 def test_gradient_of_the_plain_form_against_differences():
     g = torch.Generator().manual_seed(3)
     q, k, v = (torch.randn(5, h, 8, generator=g, dtype=torch.float64).requires_grad_() for h in (4, 2, 2))
