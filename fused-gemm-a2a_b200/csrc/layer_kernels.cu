@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
         rotate16<kInterleaved>(f, c, s);
         if (normed) {
           // n = x * rstd, g the gradient behind the norm: dw += g * n, dx = rstd * (g*w - n * mean(g*w*n)).
-          // Rows that do not exist hold zeros and add nothing.
+          // Rows that do not exist hold zeros and add nothing: their rstd, which eps = 0 would make infinite, is 0.
           F2 x[8], g[8], sq = f2(0.f), dot = f2(0.f);
           unpack16(v.x[0], v.x[1], x);
           unpack16(weights[t][sub], weights[t][8 + sub], g);
@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(32 * kRotaryWarps, kBackward && kNorm ? 2 : 3)
             sq = fma2(x[i], x[i], sq);
             dot = fma2(g[i], x[i], dot);
           }
-          const float rstd = rsqrtf(eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps);
+          const float square = eight_lane_sum(sum(sq)) * (1.f / kHeadDim) + P.eps;
+          const float rstd = h < P.heads[t] ? rsqrtf(square) : 0.f;
           const F2 r = f2(rstd), mean = f2(-eight_lane_sum(sum(dot)) * rstd * (1.f / kHeadDim));
 #pragma unroll
           for (int i = 0; i < 8; ++i) {

@@ -179,6 +179,27 @@ def test_rotary_matches_the_plain_form(native, tokens, heads, kv_heads, sections
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('heads,kv_heads', [(1, 1), (6, 2), (3, 3), (5, 1), (4, 4)])
+def test_rotary_weight_gradients_without_an_epsilon(native, heads, kv_heads):
+    """eps = 0 and head counts that do not fill a group of four head rows."""
+    rotary, _ = ops()
+    gen = torch.Generator(device='cuda').manual_seed(heads)
+    tokens, pos, freq = 70, torch.arange(70, device='cuda'), frequencies((64,)).cuda()
+    q, k = normal(gen, tokens, heads, 128, std=2.0), normal(gen, tokens, kv_heads, 128)
+    gq, gk = normal(gen, tokens, heads, 128), normal(gen, tokens, kv_heads, 128)
+    wq, wk = (normal(gen, 128, std=0.2, mean=1.0).requires_grad_() for _ in range(2))
+    outs = rotary(q, k, pos, freq, q_weight=wq, k_weight=wk, eps=0.0)
+    for x, w, dy, y, dw in zip((q, k), (wq, wk), (gq, gk), outs, torch.autograd.grad(outs, (wq, wk), (gq, gk))):
+        w64 = w.detach().double().requires_grad_()
+        want = plain.rotary(x.double(), pos[:, None], freq, (64,), True, w64, eps=0.0)
+        dwant = torch.autograd.grad(want, w64, dy.double())[0]
+        within(y.detach(), want.detach(), HALF * want.detach().abs() + FINE * want.detach().abs().amax(-1, keepdim=True), 'output')
+        n = x.double() / x.double().square().mean(-1, keepdim=True).sqrt()
+        terms = (dy.double().abs().amax(-1, keepdim=True) * n.abs()).sum((0, 1)) * 2 ** 0.5
+        within(dw, dwant, HALF * dwant.abs() + FINE * terms, 'weight gradient')
+
+
+@pytest.mark.gpu
 def test_rotary_reads_strided_heads_and_leaves_its_inputs(native):
     rotary, _ = ops()
     gen = torch.Generator(device='cuda').manual_seed(1)
