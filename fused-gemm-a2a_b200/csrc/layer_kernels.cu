@@ -959,6 +959,9 @@ int fga_rotary_backward(const FgaRotary* args, void* stream) {
   int rc = check_rotary(args, true, P);
   if (rc != kSuccess) return rc;
   const bool norm = P.w[0] || P.w[1];
+  FGA_REQUIRE(args->dweight[0] == nullptr || args->dweight[0] != args->dweight[1] ||
+                  (args->dweight_f32[0] && args->dweight_f32[1] && args->dweight_accumulate[1]),
+              "rotary: one weight gradient for both tensors must be FP32 and accumulate");
   FGA_REQUIRE(!norm || (args->scratch != nullptr && aligned16(args->scratch)), "rotary: weight gradients need scratch");
   P.partial = args->scratch;
   const int grid = rotary_grid(static_cast<long long>(P.tokens) * P.splits, norm, sm_count());
@@ -975,8 +978,16 @@ int fga_rotary_backward(const FgaRotary* args, void* stream) {
     F.out_f32[t] = args->dweight_f32[t];
     F.accumulate[t] = args->dweight_accumulate[t];
   }
+  const bool shared = F.out[0] != nullptr && F.out[0] == F.out[1];
+  if (shared) F.out[1] = nullptr;
   finish_sums_kernel<<<dim3(1, 2, 1), 512, 0, st>>>(F);
   FGA_LAUNCHED();
+  if (shared) {  // one gradient for both weights: k's sums are added when q's are there
+    F.out[1] = F.out[0];
+    F.out[0] = nullptr;
+    finish_sums_kernel<<<dim3(1, 2, 1), 512, 0, st>>>(F);
+    FGA_LAUNCHED();
+  }
   return kSuccess;
 }
 

@@ -253,7 +253,8 @@ int fga_mx_quantize(const void* a, int64_t rows, int k, int64_t stride_row, int6
  * 2i+1 when interleaved, i and i+64 otherwise) turns by positions[token, axis] * inv_freq[i], where the
  * first sections[0] pairs belong to axis 0, the next to axis 1, and so on; the sections add up to 64.
  * backward: dy (contiguous) in, out = gradient of x, dweight (=|+=) gradient of the weight through
- * `scratch` of fga_rotary_scratch_floats() floats; x is read only where weight is set. */
+ * `scratch` of fga_rotary_scratch_floats() floats; x is read only where weight is set. Both dweight may be one FP32
+ * vector that accumulates (dweight_accumulate[1] set): q's gradient is added first, then k's. */
 typedef struct FgaRotary {
   const void* x[2];          /* BF16, strides in elements, multiples of 8; the 128 elements of a head adjoin */
   int64_t x_token_stride[2], x_head_stride[2];

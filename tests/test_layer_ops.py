@@ -244,6 +244,42 @@ def test_rotary_accumulates_into_main_grad_and_takes_no_tokens(native):
     assert torch.autograd.grad(outs, bare, [torch.ones_like(t) for t in outs])[0].abs().max() == 0
 
 
+def test_one_weight_gradient_for_both_tensors_has_to_accumulate(native):
+    import ctypes
+
+    import _fga_native as api
+    rotary = api.FgaRotary(tokens=4, axes=1, positions=16, inv_freq=16, scratch=16)
+    rotary.sections[0] = 64
+    for t in range(2):
+        rotary.x[t], rotary.dy[t], rotary.out[t], rotary.weight[t], rotary.dweight[t] = 16, 16, 16, 16, 32
+        rotary.heads[t] = 1
+    for f32, accumulate in (((1, 1), (0, 0)), ((1, 1), (1, 0)), ((0, 0), (1, 1)), ((1, 0), (1, 1))):
+        for t in range(2):
+            rotary.dweight_f32[t], rotary.dweight_accumulate[t] = f32[t], accumulate[t]
+        assert native.fga_rotary_backward(ctypes.byref(rotary), None) == -1 and b'accumulate' in native.fga_last_error()
+
+
+@pytest.mark.gpu
+def test_one_head_norm_weight_for_queries_and_keys(native):
+    """A weight tied between q and k gets the sum of both gradients in its main_grad, in every run."""
+    rotary, _ = ops()
+    gen = torch.Generator(device='cuda').manual_seed(16)
+    q, k = normal(gen, 64, 8, 128), normal(gen, 64, 8, 128)
+    gq, gk = normal(gen, 64, 8, 128), normal(gen, 64, 8, 128)
+    pos, freq = torch.arange(64, device='cuda'), frequencies((64,)).cuda()
+    w = normal(gen, 128, mean=1.0)
+    apart = [torch.nn.Parameter(w.clone()) for _ in range(2)]
+    for p in apart:
+        p.main_grad = torch.zeros(128, device='cuda')
+    torch.autograd.backward(rotary(q, k, pos, freq, q_weight=apart[0], k_weight=apart[1]), (gq, gk))
+    want = apart[0].main_grad + apart[1].main_grad            # what adding q's, then k's to zero rounds to
+    for _ in range(200):
+        tied = torch.nn.Parameter(w.clone())
+        tied.main_grad = torch.zeros(128, device='cuda')
+        torch.autograd.backward(rotary(q, k, pos, freq, q_weight=tied, k_weight=tied), (gq, gk))
+        assert torch.equal(tied.main_grad, want)
+
+
 def norm_bounds(t, cu, center, dy, dr, has_branch):
     """Expected values and error bounds of y, r and every gradient, in 64 bits."""
     names = ('x', 'branch', 'weight', 'gate', 'scale', 'shift')
