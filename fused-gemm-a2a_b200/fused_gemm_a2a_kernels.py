@@ -9,6 +9,7 @@ counter; a CTA pair owns a 256-row MMA tile; a QKV push maps one 128-column tile
 """
 import math
 import os
+import threading
 
 import torch
 
@@ -237,13 +238,21 @@ def bf16_wgrad(dy, x, out, status, *, accumulate=False):
 
 
 _local_status = {}
+_local_status_lock = threading.Lock()
 
 
 def _status_word(device):
-    """A per-device status word for kernels launched outside a CP group (bounded-wait reports)."""
+    """A per-device status word for kernels launched outside a CP group (bounded-wait reports). It is zero
+    before any other thread can find it, whatever stream that thread launches on."""
     word = _local_status.get(device)
     if word is None:
-        word = _local_status[device] = torch.zeros(4, dtype=torch.int32, device=device)
+        with _local_status_lock:
+            word = _local_status.get(device)
+            if word is None:
+                word = torch.zeros(4, dtype=torch.int32, device=device)
+                if word.is_cuda and not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(device).synchronize()
+                _local_status[device] = word
     return word
 
 

@@ -144,14 +144,12 @@ def _weight_result(weight, target, accumulated):
 # ----------------------------------------------------------------------------------------------
 def _status(device):
     """The device's status word for kernels outside a CP group, which the check_status() of any group on
-    the device covers. Zeroed before any stream may read it, and never from inside a capture."""
+    the device covers. Never created from inside a capture."""
     word = _k._local_status.get(device)
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('Call packed_attention once on this device before capturing it into a CUDA graph')
-        with torch.cuda.device(device):
-            word = _k._status_word(device)
-            torch.cuda.current_stream().synchronize()
+        word = _k._status_word(device)
     return word
 
 

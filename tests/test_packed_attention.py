@@ -41,6 +41,34 @@ def test_check_status_reads_the_current_device_for_every_way_to_name_it(monkeypa
         fused_layer_ops.check_status(device)
 
 
+def test_the_status_word_is_zero_before_another_thread_can_find_it(monkeypatch):
+    """A second thread that found the word earlier could launch on its own stream, in front of the zeros."""
+    import fused_gemm_a2a_kernels as kernels
+    import fused_layer_ops
+    device, found = torch.device('cuda', 0), []
+
+    class Word:
+        is_cuda = True
+
+    class Stream:
+        def synchronize(self):
+            found.append(dict(kernels._local_status))
+
+    class Nothing:
+        def __init__(self, *_):
+            pass
+        __enter__ = __exit__ = lambda *_: None
+
+    monkeypatch.setattr(kernels, '_local_status', {})
+    monkeypatch.setattr(torch, 'zeros', lambda *a, **k: Word())
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda *_: Stream())
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    monkeypatch.setattr(torch.cuda, 'device', Nothing)
+    word = fused_layer_ops._status(device)
+    assert isinstance(word, Word) and found == [{}]        # waited for once, and not to be found meanwhile
+    assert kernels._local_status == {device: word} and fused_layer_ops._status(device) is word and len(found) == 1
+
+
 def test_refusals():
     bf = torch.bfloat16
     q, k = torch.zeros(6, 4, 128, dtype=bf), torch.zeros(6, 2, 128, dtype=bf)
