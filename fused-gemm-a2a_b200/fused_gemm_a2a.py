@@ -538,8 +538,9 @@ class _Comm:
                                'the CP group, then call clear_status()')
 
     def check_status(self):
-        """Synchronize and raise if any kernel of this group (or an MXFP8 weight gradient launched
-        outside a group on this device) gave up on a bounded wait."""
+        """Synchronize with all streams of the device and raise if any kernel of this group (or an attention
+        kernel or MXFP8 weight gradient launched outside a group on this device) gave up on a bounded wait."""
+        _k._synchronize(self.status)
         self._raise_for(self.status.tolist())
         local = _k._local_status.get(self.device)
         if local is not None:
@@ -568,6 +569,7 @@ class _Comm:
         local = _k._local_status.get(self.device)
         if local is not None:
             local.zero_()
+        _k._synchronize(self.status)     # before any other stream may launch on it
 
     def post_status(self):
         """Queue a copy of the status word into pinned host memory behind the work issued so far

@@ -256,6 +256,12 @@ def _status_word(device):
     return word
 
 
+def _synchronize(word):
+    """Wait for all streams of a status word's device: any of them may hold a kernel that still reports to it."""
+    if word.is_cuda:
+        torch.cuda.synchronize(word.device)
+
+
 def mxfp8_gemm(a, sa, b, sb, out, m, n, status, *, accumulate=False):
     """out[m, n] (=|+=) dequant(a) @ dequant(b)^T for operands produced by mxfp8_quantize (same
     padded K); block-scaled tcgen05 MMAs with FP32 accumulation."""

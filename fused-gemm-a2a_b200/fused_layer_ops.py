@@ -154,8 +154,8 @@ def _status(device):
 
 
 def check_status(device=None, *, clear=False):
-    """Synchronize and raise if an attention kernel on `device` (default: the current one) gave up on a bounded
-    wait. Such an error is sticky: later attention calls on the device return without computing until it has
+    """Synchronize with all streams of `device` (default: the current one) and raise if an attention kernel gave up
+    on a bounded wait. Such an error is sticky: later attention calls on the device return without computing until it has
     been cleared, here with clear=True or by a group's clear_status()."""
     device = torch.device('cuda' if device is None else device)
     if device.index is None:
@@ -163,9 +163,11 @@ def check_status(device=None, *, clear=False):
     word = _k._local_status.get(device)
     if word is None:
         return
+    _k._synchronize(word)
     code, where, detail, _ = word.tolist()
     if clear:
         word.zero_()
+        _k._synchronize(word)     # before any other stream may launch on it
     if code:
         reason = _native.DEVICE_ERRORS.get(code, 'unknown device error')
         raise RuntimeError(f'Attention device error {code}: {reason} (where={where}, detail={detail}). Outputs and '

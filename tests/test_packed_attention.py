@@ -41,6 +41,35 @@ def test_check_status_reads_the_current_device_for_every_way_to_name_it(monkeypa
         fused_layer_ops.check_status(device)
 
 
+@pytest.mark.parametrize('clear', [False, True])
+def test_check_status_waits_for_all_streams(monkeypatch, clear):
+    """An error that a kernel on any stream records before it ends is seen, and not erased unseen."""
+    import fused_gemm_a2a_kernels as kernels
+    import fused_layer_ops
+    events = []
+
+    class Word:
+        is_cuda, device, code = True, torch.device('cuda', 0), 0
+
+        def tolist(self):
+            events.append('read')
+            return [self.code, 70, 5, 0]
+
+        def zero_(self):
+            events.append('zero')
+
+    def synchronize(device):
+        events.append('synchronize')
+        word.code = 3                    # what was running has given up meanwhile
+
+    word = Word()
+    monkeypatch.setattr(kernels, '_local_status', {word.device: word})
+    monkeypatch.setattr(torch.cuda, 'synchronize', synchronize)
+    with pytest.raises(RuntimeError, match='device error 3'):
+        fused_layer_ops.check_status(word.device, clear=clear)
+    assert events == ['synchronize', 'read'] + ['zero', 'synchronize'] * clear
+
+
 def test_the_status_word_is_zero_before_another_thread_can_find_it(monkeypatch):
     """A second thread that found the word earlier could launch on its own stream, in front of the zeros."""
     import fused_gemm_a2a_kernels as kernels
@@ -370,6 +399,30 @@ def test_a_recorded_device_error_is_sticky_and_raises(native):
         fused_gemm_a2a.check_status(clear=True)
     fused_gemm_a2a.check_status()
     assert torch.equal(attention(q, q, q), q)
+
+
+@pytest.mark.gpu
+def test_check_status_sees_an_error_behind_work_of_another_stream(native):
+    import fused_gemm_a2a
+    import fused_gemm_a2a_kernels as kernels
+    q = torch.ones(4, 1, 128, dtype=torch.bfloat16, device='cuda')
+    attention(q, q, q)
+    word, code = kernels._local_status[q.device], torch.tensor([3, 0, 0, 0], dtype=torch.int32, device='cuda')
+    a, b = (torch.zeros(1 << 28, dtype=torch.uint8, device='cuda') for _ in range(2))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(300):             # tens of milliseconds
+            a.copy_(b, non_blocking=True)
+        word.copy_(code, non_blocking=True)
+    try:
+        with pytest.raises(RuntimeError, match='pipeline barrier'):
+            fused_gemm_a2a.check_status(clear=True)
+    finally:
+        side.synchronize()
+        word.zero_()
+        torch.cuda.synchronize()
+    fused_gemm_a2a.check_status()
 
 
 @pytest.mark.gpu
