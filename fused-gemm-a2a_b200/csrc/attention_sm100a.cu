@@ -1282,17 +1282,6 @@ static int check_attention(const FgaAttention* a, AttentionParams& P) {
   return kSuccess;
 }
 
-// Lets `kernel` use `bytes` of dynamic shared memory on the current device, once per device and kernel.
-template <typename Kernel>
-static int allow_smem(Kernel kernel, uint32_t bytes, uint64_t& done) {
-  int dev = 0;
-  FGA_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit) return kSuccess;
-  FGA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
-  return kSuccess;
-}
 static uint64_t g_smem_forward, g_smem_dkv, g_smem_dq;
 
 // Upper bound of the work tiles of `rows` rows: each sequence, and the rows behind the last, ends in one

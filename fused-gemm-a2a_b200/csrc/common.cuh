@@ -61,4 +61,18 @@ int encode_tmap_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t p
 
 int sm_count();
 
+// Lets `kernel` use up to `bytes` of dynamic shared memory on the current device, once per device and kernel
+// (`done` belongs to the kernel). The limit is the kernel's, whoever launches it: `bytes` is the most that any
+// call needs, so that calls of several host threads never lower it for one another.
+template <typename Kernel>
+inline int allow_smem(Kernel kernel, uint32_t bytes, uint64_t& done) {
+  int dev = 0;
+  FGA_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit) return kSuccess;
+  FGA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+  return kSuccess;
+}
+
 }  // namespace fga

@@ -811,12 +811,16 @@ NormShape norm_shape(int hidden) {
 // Bytes of the rows in flight, `parts` tensors each, and of `kept` rows beside them: 16 bytes a thread and vector.
 uint32_t norm_smem(NormShape s, int parts, int kept) { return 16u * s.vec * s.threads * (kRowsAhead * parts + kept); }
 
-int run_norm(void (*kernel)(NormParams), int grid, NormShape shape, uint32_t smem, const NormParams& P, cudaStream_t st) {
-  if (smem > 40 * 1024)  // beside the static arrays, 48 KiB need no leave
-    FGA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<grid, shape.threads, smem, st>>>(P);
+// `done`: the kernel's own, for allow_smem().
+int run_norm(void (*kernel)(NormParams), uint64_t& done, int grid, NormShape shape, int parts, int kept,
+             const NormParams& P, cudaStream_t st) {
+  const NormShape widest = norm_shape(shape.vec == 1 ? 2048 : 8192);
+  const int rc = allow_smem(kernel, norm_smem(widest, parts, kept), done);
+  if (rc != kSuccess) return rc;
+  kernel<<<grid, shape.threads, norm_smem(shape, parts, kept), st>>>(P);
   return kSuccess;
 }
+uint64_t g_norm_smem[6];  // forward, backward, modulated backward; each with 8 and 16 columns a thread
 
 int rotary_grid(long long units, bool sums, int sms) {
   // With sums every block leaves a row of partials behind, so the grid is what is resident at once.
@@ -1001,9 +1005,8 @@ int fga_norm_forward(const FgaNorm* args, void* stream) {
   const NormShape shape = norm_shape(P.hidden);
   const int grid = static_cast<int>(ceil_div(P.tokens, P.chunk_rows));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const uint32_t smem = norm_smem(shape, 2, 0);
-  const int rc2 = shape.vec == 1 ? run_norm(norm_forward_kernel<1>, grid, shape, smem, P, st)
-                                 : run_norm(norm_forward_kernel<2>, grid, shape, smem, P, st);
+  const int rc2 = shape.vec == 1 ? run_norm(norm_forward_kernel<1>, g_norm_smem[0], grid, shape, 2, 0, P, st)
+                                 : run_norm(norm_forward_kernel<2>, g_norm_smem[1], grid, shape, 2, 0, P, st);
   if (rc2 != kSuccess) return rc2;
   FGA_LAUNCHED();
   return kSuccess;
@@ -1032,13 +1035,12 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = static_cast<int>(chunks);
   const bool mod = P.gate || P.scale || modulated;
-  const uint32_t smem = norm_smem(shape, mod ? 4 : 3, mod ? 3 : 1);
   if (shape.vec == 1)
-    rc = mod ? run_norm(norm_backward_kernel<1, true>, grid, shape, smem, P, st)
-             : run_norm(norm_backward_kernel<1, false>, grid, shape, smem, P, st);
+    rc = mod ? run_norm(norm_backward_kernel<1, true>, g_norm_smem[4], grid, shape, 4, 3, P, st)
+             : run_norm(norm_backward_kernel<1, false>, g_norm_smem[2], grid, shape, 3, 1, P, st);
   else
-    rc = mod ? run_norm(norm_backward_kernel<2, true>, grid, shape, smem, P, st)
-             : run_norm(norm_backward_kernel<2, false>, grid, shape, smem, P, st);
+    rc = mod ? run_norm(norm_backward_kernel<2, true>, g_norm_smem[5], grid, shape, 4, 3, P, st)
+             : run_norm(norm_backward_kernel<2, false>, g_norm_smem[3], grid, shape, 3, 1, P, st);
   if (rc != kSuccess) return rc;
   FGA_LAUNCHED();
   const int blocks = static_cast<int>(ceil_div(P.hidden, 128));

@@ -431,6 +431,39 @@ def test_more_than_2_to_31_elements(native):
 
 
 @pytest.mark.gpu
+def test_norms_of_several_widths_from_several_threads(native):
+    """The limits a launch needs are the kernel's: threads with other widths must not lower them in between."""
+    import threading
+
+    import _fga_native as api
+    widths, calls, failures = (8192, 4608, 6144, 5120), 20000, []
+    start = threading.Barrier(len(widths))
+
+    def work(hidden):
+        try:
+            stream = torch.cuda.Stream()
+            x, b, y, r = (torch.ones(2, hidden, dtype=torch.bfloat16, device='cuda') for _ in range(4))
+            torch.cuda.synchronize()
+            args = api.NORM_BYTES.pack(x.data_ptr(), b.data_ptr(), 0, 0, 0, 0, 0, y.data_ptr(), r.data_ptr(), *(0,) * 11,
+                                       2, hidden, 1, 0, 0, 0, 1e-6)
+            start.wait()
+            refused = sum(native.fga_norm_forward(args, stream.cuda_stream) != 0 for _ in range(calls))
+            stream.synchronize()
+            assert (r == 2).all() and (y == 1).all()
+            if refused:
+                failures.append(f'{hidden}: {refused} of {calls} launches refused')
+        except Exception as error:                                                  # noqa: BLE001
+            failures.append(f'{hidden}: {error!r}')
+
+    threads = [threading.Thread(target=work, args=(hidden,)) for hidden in widths]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
+
+
+@pytest.mark.gpu
 def test_gradients_are_not_differentiable_twice(native):
     _, norm = ops()
     x = torch.ones(4, 64, dtype=torch.bfloat16, device='cuda', requires_grad=True)
