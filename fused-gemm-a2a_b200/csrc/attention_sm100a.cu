@@ -32,6 +32,16 @@ constexpr uint32_t kHalfBytes = 16384;    // 128 rows x 128 bytes
 constexpr uint32_t kTileBytes = 2 * kHalfBytes;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Range of the scores. The exponent of a probability is fma(s, scale * log2(e), -top) with `top`, the row's largest
+// product, rounded to FP32. All of a row's probabilities are off by the same factor then, which their sum
+// undoes, as long as it stays inside FP32: half a step is 16 at 2^29. The backward pass starts from the
+// logarithm of the sum, rounded twice, and nothing undoes that: probabilities are off by about 2^-23 of the score,
+// half a BF16 step at 2^15 and an eighth at 2^20. Rows beyond come out as NaN, not as plausible values.
+constexpr float kMaxTop = 536870912.f;  // 2^29, in units of log2
+constexpr float kMaxLse = 1048576.f;    // 2^20
+__device__ __forceinline__ float exponent_of_lse(float lse) {
+  return fabsf(lse) <= kMaxLse ? -kLog2e * lse : __int_as_float(0x7fffffff);
+}
 
 struct AttentionParams {
   const int* cu;
@@ -514,10 +524,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       tc_fence_after();
       const bool valid = row < wt.len;
       const long long at = wt.first + row;
+      const float invalid = fabsf(m * c) <= kMaxTop ? 0.f : __int_as_float(0x7fffffff);  // see the range of the scores
       // The query tile has been read by its last product: its shared memory stages the output.
       store_row(o_tmem, q_smem + i * kTileBytes + row_in_tile * kSlotPitch, P.o + (at * P.heads + head) * kDim,
-                l > 0.f || l != l ? 1.f / l : 0.f, valid);
-      if (valid && P.lse != nullptr) P.lse[static_cast<long long>(head) * P.tokens + at] = (m * c + log2f(l)) * kLn2;
+                (l > 0.f || l != l ? 1.f / l : 0.f) + invalid, valid);
+      if (valid && P.lse != nullptr)
+        P.lse[static_cast<long long>(head) * P.tokens + at] = (m * c + log2f(l)) * kLn2 + invalid;
       bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
     }
   }
@@ -685,7 +697,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           neg[c] = -INFINITY;  // a probability of 0 behind the sequence
           delta[c] = 0.f;
           if (row + q < wt.len) {
-            neg[c] = -kLog2e * __ldg(P.lse + at + q);
+            neg[c] = exponent_of_lse(__ldg(P.lse + at + q));
             delta[c] = __ldg(P.delta + at + q);
           }
         }
@@ -1115,7 +1127,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const bool valid = row < wt.len;
     const long long at = wt.first + (valid ? row : 0);
     const F2 c2 = f2(P.scale_log2);
-    const F2 neg = f2(-kLog2e * __ldg(P.lse + static_cast<long long>(head) * P.tokens + at));
+    const F2 neg = f2(exponent_of_lse(__ldg(P.lse + static_cast<long long>(head) * P.tokens + at)));
     // delta of the rows, kept for the dK/dV kernel. Where all keys lie in one tile it is the sum of P * dP, which
     // needs no rounded output: a row that sees a single key then gets dS = 0, not the rounding error of its
     // output. (That error is 2^-9 |o| |dO|; beside the spread of dP it vanishes with the root of the number of

@@ -233,6 +233,10 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
     [heads, tokens] logarithms of the rows' sums of exponentials (-inf behind the last sequence; no gradient
     flows through them).
 
+    Range of the scores: the output holds its precision while a row's largest |scale * q k| is below 2^28, and
+    the row is NaN from 2^29 on. In the backward pass probabilities are off by about 2^-23 of the score: less than their
+    rounding to BF16 up to scores of 2^14, an eighth at 2^20; gradients of and through rows beyond that are NaN.
+
     Scores, softmax statistics and all sums are FP32; the probabilities (and in the backward pass the
     gradients of the scores) are rounded to BF16 for the second product. Results, gradients included, are
     the same bits in every run. Kernel waits are bounded as in the projections and report through the device's

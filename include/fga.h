@@ -302,7 +302,8 @@ int fga_norm_backward(const FgaNorm* args, void* stream);
  * causal only over keys at or before the query's position; query head h reads key/value head
  * h / (heads / kv_heads). lse[h, row] is the natural logarithm of the row's sum of exponentials. Rows
  * behind the last sequence: o = 0, lse = -inf, all gradients 0. lse may be NULL in the forward. scale:
- * from 1e-30 to 1e30. status and timeout_ns as for the GEMMs; the calls of a device share its status word,
+ * from 1e-30 to 1e30. A row whose largest |scale * q k| is beyond 2^28 gives NaN, in the backward pass beyond
+ * 2^20; gradients are as exact as BF16 up to 2^14. status and timeout_ns as for the GEMMs; the calls of a device share its status word,
  * whatever their streams.
  * backward reads q, k, v, o, lse and the contiguous gradient d_o, and writes contiguous dq, dk, dv;
  * delta: scratch of heads * tokens floats. The results do not depend on scheduling: no atomics. */

@@ -286,6 +286,44 @@ def test_other_scales_and_peaked_rows(native, scale, std):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('causal', [False, True])
+def test_scores_at_and_beyond_the_end_of_their_range(native, causal):
+    """Where scores are so far apart that a row is its largest key's value, and where FP32 cannot hold them."""
+    gen = torch.Generator(device='cuda').manual_seed(17)
+    q, k, v, do = (normal(gen, 400, 1, 128) for _ in range(4))
+    products = q[:, 0].double() @ k[:, 0].double().T
+    if causal:
+        products = products.masked_fill(torch.ones(400, 400, dtype=torch.bool, device='cuda').triu(1), -math.inf)
+    top, best = products.max(-1)
+    # FP32 sums of 128 products are off by 128 * 2^-24 of their absolute sum: rows whose second key is closer are left out
+    second = products.scatter(1, best[:, None], -math.inf).max(-1).values
+    clear = top - second > 128 * 2.0 ** -24 * (q.double().abs() @ k.double().abs().transpose(1, 2)).max() + 1e-3
+    assert clear.sum() > 300
+    # The one probability p is a power of two that the rounded shift leaves, rounded to BF16, and the sum it is divided
+    # by is p unrounded: o = v (1 + 2^-8)(1 + 2^-8) at most, output rounding included; FP32 steps take 2^-20.
+    want = v[best].double()
+    bound = (2 * HALF + HALF ** 2 + 2.0 ** -20) * want.abs()
+    for scale in (1e5, 5e6):                                   # up to 2^28
+        scores = top.abs() * scale
+        assert scores.max() < 2 ** 28 * 1.5
+        o, lse = attention(q, k, v, causal=causal, scale=scale, return_lse=True)
+        within(o[clear], want[clear], bound[clear], f'o at scale {scale}')
+        within(lse[0], top * scale, (128 * 2.0 ** -24 + 2.0 ** -20) * scale * 128 * 8 + 10, 'lse')
+    scale = 1e8
+    beyond = (top.abs() * scale > 2 ** 29.1) & clear           # in units of log2 well above 2^29
+    within_range = (top.abs() * scale < 2 ** 28) & clear
+    assert beyond.sum() > 300
+    o, lse = attention(q, k, v, causal=causal, scale=scale, return_lse=True)
+    assert o[beyond].isnan().all() and lse[0, beyond].isnan().all()
+    within(o[within_range], want[within_range], bound[within_range], 'o beside rows out of range')
+    # gradients: NaN from a largest score of 2^20 on, in every row that such a query reaches
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(attention(*leaves, causal=causal, scale=1e6), leaves, do)
+    far = top.abs() * 1e6 > 2 ** 20.1
+    assert far.sum() > 300 and dq[far].isnan().all() and dv[0].isnan().all() and dk[0].isnan().all()
+
+
+@pytest.mark.gpu
 def test_strided_heads_and_expanded_gradients(native):
     gen = torch.Generator(device='cuda').manual_seed(8)
     packed = normal(gen, 300, 8, 128)
