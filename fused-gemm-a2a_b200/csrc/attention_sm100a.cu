@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const float top = row_max();
       if (j == 0) {
         m = top == -INFINITY ? 0.f : top;
-      } else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
+      } else if (__any_sync(0xffffffffu, row < wt.len && (top - m) * c > 8.f)) {  // rows behind the sequence have no say
         // S(j) was issued behind the product that last wrote the output: its arrival covers both
         const float up = fmaxf(m, top), f = exp2_approx((m - up) * c);
         m = up;

@@ -324,6 +324,25 @@ def test_scores_at_and_beyond_the_end_of_their_range(native, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('pad_is_a_sequence', [False, True])
+def test_rows_behind_a_sequence_do_not_change_a_bit_of_it(native, pad_is_a_sequence):
+    """The last tile of queries holds rows of padding, or of the next sequence, whose maxima rise from key tile to
+    key tile or do not."""
+    gen = torch.Generator(device='cuda').manual_seed(18)
+    n, pad = 300, 200
+    q, k, v, do = (normal(gen, n + pad, 2, 128) for _ in range(4))
+    cu = torch.tensor([0, n, n + pad] if pad_is_a_sequence else [0, n], dtype=torch.int32, device='cuda')
+    results = []
+    for behind in (0.0, k[200:201].float() * 30):
+        q[n:] = behind
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        o, lse = attention(*leaves, cu, return_lse=True)
+        results.append([o.detach()[:n], lse[:, :n], *(g[:n] for g in torch.autograd.grad(o, leaves, do))])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_strided_heads_and_expanded_gradients(native):
     gen = torch.Generator(device='cuda').manual_seed(8)
     packed = normal(gen, 300, 8, 128)
