@@ -38,13 +38,14 @@ class FgaAttention(ctypes.Structure):
     _fields_ = ([(name, c_void_p) for name in (
         'q', 'k', 'v', 'o', 'lse', 'd_o', 'dq', 'dk', 'dv', 'delta', 'cu_seqlens', 'status')]
         + [('timeout_ns', c_uint64), ('token_stride', c_int64 * 3), ('head_stride', c_int64 * 3), ('tokens', c_int64),
-           ('heads', c_int32), ('kv_heads', c_int32), ('samples', c_int32), ('causal', c_int32), ('scale', c_float)])
+           ('heads', c_int32), ('kv_heads', c_int32), ('samples', c_int32), ('causal', c_int32), ('scale', c_float),
+           ('host_status', c_void_p)])
 
 
 # The same layouts as packed bytes, which a launch builds in a fraction of the time of a ctypes structure.
 ROTARY_BYTES = struct.Struct('@2P2q2q2P2P2P2P3Pq2i3i4ii2i2if0q')
 NORM_BYTES = struct.Struct('@20Pq5if0q')
-ATTENTION_BYTES = struct.Struct('@12PQ6qq4if0q')
+ATTENTION_BYTES = struct.Struct('@12PQ6qq4ifP0q')
 for _layout, _fields in ((ROTARY_BYTES, FgaRotary), (NORM_BYTES, FgaNorm), (ATTENTION_BYTES, FgaAttention)):
     assert _layout.size == ctypes.sizeof(_fields), _fields.__name__
 

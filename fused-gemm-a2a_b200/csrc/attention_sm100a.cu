@@ -57,6 +57,7 @@ struct AttentionParams {
   int tiles;                                    // work tiles per head in the grid (an upper bound)
   int parts;                                    // dK/dV: blocks (one cluster) that share the queries of a tile
   int* status;
+  int* host_status;                             // a copy of the status word in pinned host memory, or null
   unsigned long long timeout_ns;
 };
 
@@ -244,14 +245,26 @@ __device__ __forceinline__ void zero_rows(uint16_t* base, int heads, int head, i
         make_uint4(0, 0, 0, 0);
 }
 
+// An error that this block met, its own or an earlier kernel's: to where the host sees it without asking the
+// device. The code goes last.
+__device__ __forceinline__ void tell_host(const AttentionParams& P) {
+  if (P.host_status == nullptr) return;
+  volatile int* to = P.host_status;
+  to[1] = ld_relaxed_sys_s32(P.status + 1);
+  to[2] = ld_relaxed_sys_s32(P.status + 2);
+  __threadfence_system();
+  to[0] = ld_relaxed_sys_s32(P.status);
+}
+
 // Teardown shared by the kernels: copies that were issued but never consumed after an abort may still be
 // landing in this block's shared memory.
-__device__ __forceinline__ void settle(WaitCtx& w) {
+__device__ __forceinline__ void settle(WaitCtx& w, const AttentionParams& P) {
   uint32_t aborted;
   asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(aborted) : "r"(w.abort_flag) : "memory");
   if (aborted != 0 || w.dead) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) nanosleep(1000);
+    if (w.dead && (threadIdx.x & 31) == 0) tell_host(P);
   }
   __syncwarp();
   tc_fence_before();
@@ -533,7 +546,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
     }
   }
-  settle(w);
+  settle(w, P);
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -613,7 +626,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   WaitCtx w{P.status, P.timeout_ns, abort_word, sticky};
   if ((front & 1023u) != 0) {  // the tiles would not be where their swizzle needs them
-    if (threadIdx.x == 0 && atomicCAS(P.status, 0, kErrPipelineTimeout) == 0) P.status[1] = 78;
+    if (threadIdx.x == 0) {
+      if (atomicCAS(P.status, 0, kErrPipelineTimeout) == 0) P.status[1] = 78;
+      tell_host(P);
+    }
     return;
   }
   if (warp == 8 && lane == 0) {
@@ -964,7 +980,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   }
-  settle(w);
+  settle(w, P);
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1248,7 +1264,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       bulk_wait_read_all();  // shared memory may go; the writes complete with the kernel
     }
   }
-  settle(w);
+  settle(w, P);
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1290,6 +1306,7 @@ static int check_attention(const FgaAttention* a, AttentionParams& P) {
   P.o = static_cast<uint16_t*>(a->o);
   P.lse = a->lse;
   P.status = a->status;
+  P.host_status = a->host_status;
   P.timeout_ns = a->timeout_ns;
   return kSuccess;
 }

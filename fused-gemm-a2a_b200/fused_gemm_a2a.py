@@ -570,6 +570,7 @@ class _Comm:
         if local is not None:
             local.zero_()
         _k._synchronize(self.status)     # before any other stream may launch on it
+        _k._forget_host_status(self.device)
 
     def post_status(self):
         """Queue a copy of the status word into pinned host memory behind the work issued so far

@@ -7,6 +7,7 @@ through ctypes on the current CUDA stream. There is no CPU or PyTorch fallback.
 Geometry (reference fused_gemm_a2a_kernels.py:34-123): a CTA owns 128 output rows and one arrival
 counter; a CTA pair owns a 256-row MMA tile; a QKV push maps one 128-column tile to one head.
 """
+import ctypes
 import math
 import os
 import threading
@@ -254,6 +255,38 @@ def _status_word(device):
                     torch.cuda.current_stream(device).synchronize()
                 _local_status[device] = word
     return word
+
+
+class _HostStatus:
+    """Four words of pinned host memory to which kernels copy a device's status word once it holds an error.
+    Reading them takes no call of the CUDA runtime."""
+
+    def __init__(self):
+        self._memory = torch.zeros(4, dtype=torch.int32, pin_memory=True)
+        self.address = self._memory.data_ptr()
+        self.words = (ctypes.c_int32 * 4).from_address(self.address)
+
+
+_local_host_status = {}
+
+
+def _host_status(device):
+    """The host's copy of the device's status word, or None inside a capture that is the first to ask for it (pinned
+    memory cannot be allocated there)."""
+    copy = _local_host_status.get(device)
+    if copy is None and not torch.cuda.is_current_stream_capturing():
+        with _local_status_lock:
+            copy = _local_host_status.get(device)
+            if copy is None:
+                copy = _local_host_status[device] = _HostStatus()
+    return copy
+
+
+def _forget_host_status(device):
+    """Zero the host's copy; the device's word is zero and no kernel is running that could still write here."""
+    copy = _local_host_status.get(device)
+    if copy is not None:
+        copy.words[:] = (0, 0, 0, 0)
 
 
 def _synchronize(word):

@@ -155,8 +155,9 @@ def _status(device):
 
 def check_status(device=None, *, clear=False):
     """Synchronize with all streams of `device` (default: the current one) and raise if an attention kernel gave up
-    on a bounded wait. Such an error is sticky: later attention calls on the device return without computing until it has
-    been cleared, here with clear=True or by a group's clear_status()."""
+    on a bounded wait. Such an error is sticky: the kernels of later attention calls on the device return without
+    computing, and every attention call raises as soon as the host has got the error, without waiting for it, until it
+    has been cleared, here with clear=True or by a group's clear_status()."""
     device = torch.device('cuda' if device is None else device)
     if device.index is None:
         device = torch.device('cuda', torch.cuda.current_device())
@@ -168,10 +169,27 @@ def check_status(device=None, *, clear=False):
     if clear:
         word.zero_()
         _k._synchronize(word)     # before any other stream may launch on it
+    if clear or not code:
+        _k._forget_host_status(device)
+    _raise_for(code, where, detail)
+
+
+def _raise_for(code, where, detail):
     if code:
         reason = _native.DEVICE_ERRORS.get(code, 'unknown device error')
         raise RuntimeError(f'Attention device error {code}: {reason} (where={where}, detail={detail}). Outputs and '
-                           'gradients produced since then are not valid')
+                           'gradients produced since then are not valid; check_status(clear=True) clears it')
+
+
+def _host_status_address(device):
+    """Where kernels leave an error for the host. Raises what an earlier one has left there."""
+    copy = _k._host_status(device)
+    if copy is None:
+        return 0
+    words = copy.words
+    if words[0]:
+        _raise_for(*words[:3])
+    return copy.address
 
 
 def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale, d_o=None, dq=None, dk=None, dv=None, delta=None):
@@ -181,7 +199,7 @@ def _attention_args(q, k, v, o, lse, cu_seqlens, causal, scale, d_o=None, dq=Non
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _address(lse), _address(d_o), _address(dq), _address(dk),
         _address(dv), _address(delta), _address(cu_seqlens), _status(q.device).data_ptr(), _k.DEVICE_TIMEOUT_NS, q_token,
         k_token, v_token, q_head, k_head, v_head, tokens, heads, k.shape[1],
-        1 if cu_seqlens is None else cu_seqlens.shape[0] - 1, causal, scale)
+        1 if cu_seqlens is None else cu_seqlens.shape[0] - 1, causal, scale, _host_status_address(q.device))
 
 
 def _attend(q, k, v, cu_seqlens, causal, scale, keep_lse):
@@ -239,8 +257,9 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
 
     Scores, softmax statistics and all sums are FP32; the probabilities (and in the backward pass the
     gradients of the scores) are rounded to BF16 for the second product. Results, gradients included, are
-    the same bits in every run. Kernel waits are bounded as in the projections and report through the device's
-    status word, which check_status() and a group's comm.check_status() read."""
+    the same bits in every run. Kernel waits are bounded as in the projections. One that expires is recorded in the
+    device's status word, which check_status() and a group's comm.check_status() read, and raised by the first
+    later call, forward or backward, that finds it in host memory."""
     for t, label in ((q, 'q'), (k, 'k'), (v, 'v')):
         _head_tensor(t, label)
     if k.shape != v.shape or k.shape[0] != q.shape[0]:

@@ -304,7 +304,9 @@ int fga_norm_backward(const FgaNorm* args, void* stream);
  * behind the last sequence: o = 0, lse = -inf, all gradients 0. lse may be NULL in the forward. scale:
  * from 1e-30 to 1e30. A row whose largest |scale * q k| is beyond 2^28 gives NaN, in the backward pass beyond
  * 2^20; gradients are as exact as BF16 up to 2^14. status and timeout_ns as for the GEMMs; the calls of a device share its status word,
- * whatever their streams.
+ * whatever their streams. A kernel that gives up, or returns at entry because the word holds an error, also
+ * copies the word to host_status, so that the host finds it there without a synchronizing call; whoever clears
+ * the word clears both.
  * backward reads q, k, v, o, lse and the contiguous gradient d_o, and writes contiguous dq, dk, dv;
  * delta: scratch of heads * tokens floats. The results do not depend on scheduling: no atomics. */
 typedef struct FgaAttention {
@@ -321,6 +323,7 @@ typedef struct FgaAttention {
   int64_t tokens;
   int32_t heads, kv_heads, samples, causal;
   float scale;
+  int32_t* host_status;      /* int32[4] in pinned host memory that the device can write, or NULL */
 } FgaAttention;
 int fga_attention_forward(const FgaAttention* args, void* stream);
 int fga_attention_backward(const FgaAttention* args, void* stream);

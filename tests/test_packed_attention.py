@@ -70,6 +70,22 @@ def test_check_status_waits_for_all_streams(monkeypatch, clear):
     assert events == ['synchronize', 'read'] + ['zero', 'synchronize'] * clear
 
 
+def test_a_call_raises_an_error_that_the_host_has_got(monkeypatch):
+    import fused_gemm_a2a_kernels as kernels
+    import fused_layer_ops
+    device = torch.device('cuda', 0)
+
+    class Copy:
+        address, words = 64, [3, 70, 5, 0]
+
+    monkeypatch.setattr(kernels, '_local_host_status', {device: Copy()})
+    monkeypatch.setattr(kernels, '_local_status', {device: torch.zeros(4, dtype=torch.int32)})
+    with pytest.raises(RuntimeError, match='device error 3.*where=70, detail=5'):
+        fused_layer_ops._host_status_address(device)
+    fused_layer_ops.check_status(device)          # the device's word has been cleared: nothing to raise any more
+    assert fused_layer_ops._host_status_address(device) == 64
+
+
 def test_the_status_word_is_zero_before_another_thread_can_find_it(monkeypatch):
     """A second thread that found the word earlier could launch on its own stream, in front of the zeros."""
     import fused_gemm_a2a_kernels as kernels
@@ -456,6 +472,39 @@ def test_a_recorded_device_error_is_sticky_and_raises(native):
         fused_gemm_a2a.check_status(clear=True)
     fused_gemm_a2a.check_status()
     assert torch.equal(attention(q, q, q), q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('call', ['forward', 'backward', 'graph'])
+def test_an_error_reaches_the_next_call_without_a_synchronizing_one(native, call):
+    import fused_gemm_a2a
+    import fused_gemm_a2a_kernels as kernels
+    q = torch.ones(4, 1, 128, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+    o = attention(q, q, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        attention(q, q, q)
+    fused_gemm_a2a.check_status()
+    word = kernels._local_status[q.device]
+    word.copy_(torch.tensor([3, 70, 5, 0], dtype=torch.int32))
+    try:
+        if call == 'graph':
+            graph.replay()
+        elif call == 'backward':
+            torch.autograd.grad(o, q, o.detach(), retain_graph=True)
+        else:
+            attention(q.detach(), q.detach(), q.detach())
+        torch.cuda.current_stream().synchronize()      # the kernel has run; nobody has read the word
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match='pipeline barrier.*where=70, detail=5'):
+                attention(q, q, q)
+        with pytest.raises(RuntimeError, match='pipeline barrier.*where=70, detail=5'):
+            torch.autograd.grad(o, q, o.detach(), retain_graph=True)
+    finally:
+        with pytest.raises(RuntimeError, match='pipeline barrier'):
+            fused_gemm_a2a.check_status(clear=True)
+    assert torch.equal(attention(q, q, q), q)
+    fused_gemm_a2a.check_status()
 
 
 @pytest.mark.gpu
