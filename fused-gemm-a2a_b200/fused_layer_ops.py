@@ -12,11 +12,13 @@ tensors; a weight with a Megatron `main_grad` gets its gradient accumulated ther
 described by `cu_seqlens`, an int32 device tensor [samples + 1] of ascending offsets into the token axis
 that starts at 0 and is never read by the host; rows from its last offset on belong to no sequence.
 All device work is one or a few launches of libfga.so on the current stream of the tensors' device; there
-is no CPU or PyTorch fallback. Calls may be captured into CUDA graphs, backward passes included; as with any
+is no CPU or PyTorch fallback. Gradients are of first order and in reverse; forward-mode derivatives and function
+transforms (torch.func) raise. Calls may be captured into CUDA graphs, backward passes included; as with any
 autograd code, no graph recorded outside the capture may then still hold the same leaves (autograd ties a
 leaf to the stream of the first graph that uses it and would wait on that stream from inside the capture).
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 import _fga_native as _native
@@ -64,8 +66,11 @@ def _fresh(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _differentiable(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _through_autograd(*tensors):
+    """Whether autograd has to see a call: for gradients; for forward-mode derivatives and function transforms, which
+    it refuses there, where a plain call would drop them; and for a trace, which would record no kernel."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+            or forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active() or torch._C._is_tracing())
 
 
 def _head_tensor(t, label):
@@ -274,7 +279,7 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
         if cu_seqlens.shape[0] > 65536:
             raise ValueError('at most 65535 packed sequences')
     _same_device(q, k, v, cu_seqlens)
-    if _differentiable(q, k, v):
+    if _through_autograd(q, k, v):
         return _Attention.apply(q, k, v, cu_seqlens, bool(causal), scale, bool(return_lse))
     o, lse = _attend(q, k, v, cu_seqlens, bool(causal), scale, return_lse)
     return (o, lse) if return_lse else o
@@ -371,7 +376,7 @@ def rotary_embedding(q, k, positions, inv_freq, sections=None, *, interleaved=Tr
     _vector(q_weight, HEAD_DIM, 'q_weight')
     _vector(k_weight, HEAD_DIM, 'k_weight')
     _same_device(q, k, positions, inv_freq, q_weight, k_weight)
-    rotate = _Rotary.apply if _differentiable(q, k, q_weight, k_weight) else _rotate
+    rotate = _Rotary.apply if _through_autograd(q, k, q_weight, k_weight) else _rotate
     return rotate(q, k, q_weight, k_weight, positions, inv_freq, sections, bool(interleaved), float(eps))
 
 
@@ -478,5 +483,5 @@ def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=N
             raise ValueError(f'{label} must be a contiguous, 16-byte aligned BF16 tensor [{samples}, {hidden}]')
         rows.append(t)
     _same_device(x, branch, weight, cu_seqlens, *rows)
-    normalise = _ResidualNorm.apply if _differentiable(x, branch, weight, *rows) else _normalise
+    normalise = _ResidualNorm.apply if _through_autograd(x, branch, weight, *rows) else _normalise
     return normalise(x, branch, weight, *rows, cu_seqlens, samples, float(eps), bool(center))

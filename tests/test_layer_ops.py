@@ -78,6 +78,43 @@ def test_refusals_of_the_norm_call():
             norm(**(dict(x=x) | change))
 
 
+@pytest.fixture
+def calls_without_kernels(monkeypatch):
+    """The three public calls on CPU tensors, with what launches the kernels replaced by something of the right shape."""
+    import fused_layer_ops as module
+    monkeypatch.setattr(module, '_same_device', lambda *_: None)
+    monkeypatch.setattr(module, '_attend', lambda q, k, v, cu, causal, scale, keep: (q.clone(), q[:, :, 0].T.float()))
+    monkeypatch.setattr(module, '_rotate', lambda q, k, *_: (q.clone(), k.clone()))
+    monkeypatch.setattr(module, '_normalise', lambda x, branch, *_: (x.clone(), x.clone()))
+    heads, rows = torch.ones(4, 2, 128, dtype=torch.bfloat16), torch.ones(4, 256, dtype=torch.bfloat16)
+    pos, freq = torch.arange(4), frequencies((64,))
+    return [(lambda t: module.packed_attention(t, heads, heads), heads),
+            (lambda t: module.rotary_embedding(t, heads, pos, freq)[0], heads),
+            (lambda t: module.residual_norm(rows, t)[0], rows)]
+
+
+@pytest.mark.parametrize('which', [0, 1, 2])
+def test_derivatives_that_do_not_exist_are_refused_not_dropped(calls_without_kernels, which):
+    call, t = calls_without_kernels[which]
+    with torch.autograd.forward_ad.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match='jvp'):
+                call(torch.autograd.forward_ad.make_dual(t, t))
+    for transform in (lambda: torch.func.jvp(call, (t,), (t,)), lambda: torch.func.vmap(call)(torch.stack((t, t))),
+                      lambda: torch.func.grad(lambda u: call(u).float().sum())(t)):
+        with pytest.raises(RuntimeError, match='functorch transforms|data pointer'):
+            transform()
+    assert call(t).shape == t.shape                     # and nothing of it stays behind
+
+
+@pytest.mark.parametrize('which', [0, 1, 2])
+@pytest.mark.filterwarnings('ignore')
+def test_a_trace_records_the_operator(calls_without_kernels, which):
+    call, t = calls_without_kernels[which]
+    graph = str(torch.jit.trace(call, t, check_trace=False).graph)
+    assert ('^_Attention', '^_Rotary', '^_ResidualNorm')[which] in graph
+
+
 def test_the_c_entries_refuse_what_the_kernels_cannot_do(native):
     import ctypes
 
