@@ -54,8 +54,9 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
 //
 // Angles: a position of 10^6 times a frequency of 1 leaves an FP32 product with errors of 0.06 rad. The
 // angle is only needed modulo one turn, so the frequency is held as a 64-bit fixed-point number of turns
-// (2^-64 each), the product with the integer position wraps modulo 2^64 exactly, and only the top 32 bits
-// become a float: the error is below 2^-25 turns at every position below 2^31.
+// (2^-64 each, rounded once from twice FP64's precision), the product with the integer position wraps modulo
+// 2^64 exactly, and only the top 32 bits become a float. The frequency's rounding is off by |position| * 2^-64
+// turns, the float by 2^-28: together below 2^-27 turns at every position below 2^36, whatever the frequency.
 //
 // Mapping: one warp per token (several when tokens are few), which computes the token's 64 sines and
 // cosines once for all heads. Eight lanes hold a head row, each 8 elements of its lower and 8 of its upper
@@ -99,8 +100,11 @@ __device__ __forceinline__ LaneAngle lane_angle(const RotaryParams& P, int lane)
     const int pair = lane + 32 * i;
     const double f = P.freq64 ? __ldg(static_cast<const double*>(P.freq) + pair)
                               : static_cast<double>(__ldg(static_cast<const float*>(P.freq) + pair));
-    const double t = f * 0.15915494309189533577;  // turns per position
-    a.turns[i] = static_cast<unsigned long long>((t - floor(t)) * 18446744073709551616.0);
+    // turns per position: f / (2 pi) as the sum of two FP64 numbers, 1 / (2 pi) being one as well; whole turns go
+    const double per_turn = 0.15915494309189535, per_turn_rest = -9.839338337591243e-18;
+    const double t = f * per_turn, rest = fma(f, per_turn, -t) + f * per_turn_rest;
+    a.turns[i] = static_cast<unsigned long long>(__double2ll_rn((t - rint(t)) * 18446744073709551616.0)) +
+                 static_cast<unsigned long long>(__double2ll_rn(rest * 18446744073709551616.0));
     a.axis[i] = (P.axes > 1 && pair >= P.ends[0]) + (P.axes > 2 && pair >= P.ends[1]) + (P.axes > 3 && pair >= P.ends[2]);
   }
   return a;

@@ -353,7 +353,8 @@ def rotary_embedding(q, k, positions, inv_freq, sections=None, *, interleaved=Tr
     FP32 or FP64 [64], radians per position of each pair of elements; the first sections[0] pairs turn with
     axis 0 (time), the next sections[1] with axis 1 (height), and so on (default: all with one axis). Pairs
     are elements (2i, 2i+1) when `interleaved`, (i, i+64) otherwise. Angles are kept modulo a turn in 64-bit
-    fixed point: far positions lose nothing.
+    fixed point: they are off by less than 2^-27 turns at positions up to 2^36, and beyond (int64) by |position| *
+    2^-64 turns.
 
     q_weight / k_weight (BF16 [128], each optional): the head is first divided by its root mean square
     (mean of squares + eps) and multiplied by the weight, in FP32 with the rotation. Gradients flow to q,

@@ -216,6 +216,28 @@ def test_rotary_matches_the_plain_form(native, tokens, heads, kv_heads, sections
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('position,fastest', [(2 ** 31 - 5, 1e7), (2 ** 48 + 12345, 1.0), (-2 ** 50 + 7, 3.0), (5, 1e9)])
+def test_rotary_angles_of_far_positions_and_high_frequencies(native, position, fastest):
+    """Against angles in 60 digits. One position's rounding of a frequency, |position| * 2^-64 turns, and 2^-27 turns of
+    FP32 steps are all that the angle may be off by; it moves an element by that times the length of its pair."""
+    from mpmath import mp
+    rotary, _ = ops()
+    gen = torch.Generator(device='cuda').manual_seed(19)
+    freq = (fastest * 1.07 ** -torch.arange(64, dtype=torch.float64)) * 0.9173
+    x = normal(gen, 1, 4, 128)
+    with mp.workdps(60):
+        angles = [mp.mpf(f) * position for f in freq.tolist()]
+        turn = torch.tensor([[float(mp.cos(a)), float(mp.sin(a))] for a in angles], dtype=torch.float64, device='cuda')
+    a, b = x.double()[..., 0::2], x.double()[..., 1::2]
+    want = torch.stack((a * turn[:, 0] - b * turn[:, 1], b * turn[:, 0] + a * turn[:, 1]), -1).flatten(-2)
+    length = torch.stack((a.hypot(b),) * 2, -1).flatten(-2)
+    off = 2 * 3.1416 * (abs(position) * 2.0 ** -64 + 2.0 ** -27)
+    assert off < HALF / 8                                    # far below the rounding of the output
+    got = rotary(x, x, torch.tensor([position], device='cuda'), freq.cuda())[0]
+    within(got, want, HALF * want.abs() + (off + FINE) * length, 'output')
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('heads,kv_heads', [(1, 1), (6, 2), (3, 3), (5, 1), (4, 4)])
 def test_rotary_weight_gradients_without_an_epsilon(native, heads, kv_heads):
     """eps = 0 and head counts that do not fill a group of four head rows."""
