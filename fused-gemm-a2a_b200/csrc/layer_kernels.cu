@@ -595,13 +595,16 @@ __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormPara
 // dshift = sum dy, a = sum dy * n, from which dscale = a * weight and dweight gets (1 + scale) * a. The
 // mean over a centred row of dc is rstd * mean(dn), because the mean of n is zero up to rounding.
 //
-// n comes from r as the forward pass stored it: one rounding to BF16 (at most 2^-9 of r) that y does not have.
-// Gradients are then 2.4e-3 from 64 bits in the 2-norm, where rounding them alone gives 1.7e-3; computing
-// r again would read x and the branch in place of r, five streams instead of four in a pass bound by memory.
-template <int kVec, bool kMod>
+// With a gate, whose gradient needs the branch anyway, r is computed again from x and the branch, exactly as
+// the forward pass did. So it is where the norm is centred: r as it was stored is off by up to 2^-8 of r, which
+// beside r - mean is anything (a mean of 40 deviations: 10 % of n). An RMS norm without a gate reads the stored
+// r, whose rounding is then at most 2^-8 of n: gradients are 2.4e-3 from 64 bits in the 2-norm, where rounding
+// them alone gives 1.7e-3, and computing r again would be five streams instead of four in a pass bound by memory.
+template <int kVec, bool kMod, bool kRebuild>
 __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormParams P) {
   __shared__ float buf[2][64];
-  extern __shared__ uint4 ring[];  // every thread's own pieces: [row][r, dy, dr, branch][kVec][thread]
+  extern __shared__ uint4 ring[];  // every thread's own pieces: [row][r or x, dy, dr, branch][kVec][thread]
+  static_assert(kMod || !kRebuild, "the branch has a place in the ring only there");
   constexpr int kParts = kMod ? 4 : 3;
   const int warps = blockDim.x >> 5;
   const int row0 = blockIdx.x * P.chunk_rows, row1 = min(row0 + P.chunk_rows, P.tokens);
@@ -637,6 +640,10 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
 #pragma unroll
     for (int k = 0; k < kVec; ++k)
       if (on[k]) keep(0, k, P.weight + col[k]);
+  if (kRebuild && P.gate == nullptr)  // a gate of 1: the sum comes out as an addition's
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kept + (kVec + k) * piece), "r"(0x3f803f80) : "memory");
   auto fetch = [&](int row) {  // a group per row, also when there is none left
     if (row < row1) {
       const uint32_t at = mine + (row % kRowsAhead) * kParts * kVec * piece;
@@ -647,7 +654,7 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
           copy16_async(at + k * piece, P.x + from);
           if (P.dy != nullptr) copy16_async(at + (kVec + k) * piece, P.dy + from);
           if (P.dr != nullptr) copy16_async(at + (2 * kVec + k) * piece, P.dr + from);
-          if (kMod && P.gate != nullptr) copy16_async(at + (3 * kVec + k) * piece, P.branch + from);
+          if (kMod && P.branch != nullptr) copy16_async(at + (3 * kVec + k) * piece, P.branch + from);
         }
     }
     copy_commit();
@@ -729,6 +736,13 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
       if (!padding && on[k]) {
         F2 e[4];
         unpack8(shared16(slot + k * piece), n[k]);
+        if constexpr (kRebuild) {
+          F2 g[4];
+          unpack8(shared16(slot + (3 * kVec + k) * piece), e);
+          unpack8(kept_row(1, k), g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) n[k][i] = fma2(g[i], e[i], n[k][i]);
+        }
         unpack8(P.dy != nullptr ? shared16(slot + (kVec + k) * piece) : make_uint4(0, 0, 0, 0), dn[k]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -824,7 +838,7 @@ int run_norm(void (*kernel)(NormParams), uint64_t& done, int grid, NormShape sha
   kernel<<<grid, shape.threads, norm_smem(shape, parts, kept), st>>>(P);
   return kSuccess;
 }
-uint64_t g_norm_smem[6];  // forward, backward, modulated backward; each with 8 and 16 columns a thread
+uint64_t g_norm_smem[8];  // forward, backward, modulated, with r built again; each with 8 and 16 columns a thread
 
 int rotary_grid(long long units, bool sums, int sms) {
   // With sums every block leaves a row of partials behind, so the grid is what is resident at once.
@@ -1026,11 +1040,13 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
   NormParams P = {};
   int rc = check_norm(args, true, P);
   if (rc != kSuccess) return rc;
-  P.x = P.r;  // what the forward normalised: the residual sum, or x itself where there is no branch
+  const bool rebuild = P.x != nullptr && P.branch != nullptr;
+  if (!rebuild) P.x = P.r;  // what the forward normalised: the residual sum, or x itself where there is no branch
+  if (!rebuild && P.gate == nullptr) P.branch = nullptr;
   const bool modulated = args->dgate || args->dscale || args->dshift;
   FGA_REQUIRE(P.x != nullptr && P.dx != nullptr && P.rstd != nullptr && (!P.center || P.mean != nullptr),
               "norm: null pointer");
-  FGA_REQUIRE(P.gate == nullptr || P.dbranch != nullptr, "norm: a gate needs dbranch");
+  FGA_REQUIRE((P.gate == nullptr) == (P.dbranch == nullptr), "norm: dbranch exactly where there is a gate");
   FGA_REQUIRE(args->scratch != nullptr || (!modulated && args->dweight == nullptr), "norm: sums over rows need scratch");
   const long long chunks = ceil_div(P.tokens, P.chunk_rows);
   if (args->dweight != nullptr) P.part_weight = args->scratch;
@@ -1038,13 +1054,15 @@ int fga_norm_backward(const FgaNorm* args, void* stream) {
   const NormShape shape = norm_shape(P.hidden);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int grid = static_cast<int>(chunks);
-  const bool mod = P.gate || P.scale || modulated;
+  const bool mod = P.branch || P.scale || modulated;
   if (shape.vec == 1)
-    rc = mod ? run_norm(norm_backward_kernel<1, true>, g_norm_smem[4], grid, shape, 4, 3, P, st)
-             : run_norm(norm_backward_kernel<1, false>, g_norm_smem[2], grid, shape, 3, 1, P, st);
+    rc = rebuild ? run_norm(norm_backward_kernel<1, true, true>, g_norm_smem[6], grid, shape, 4, 3, P, st)
+         : mod   ? run_norm(norm_backward_kernel<1, true, false>, g_norm_smem[4], grid, shape, 4, 3, P, st)
+                 : run_norm(norm_backward_kernel<1, false, false>, g_norm_smem[2], grid, shape, 3, 1, P, st);
   else
-    rc = mod ? run_norm(norm_backward_kernel<2, true>, g_norm_smem[5], grid, shape, 4, 3, P, st)
-             : run_norm(norm_backward_kernel<2, false>, g_norm_smem[3], grid, shape, 3, 1, P, st);
+    rc = rebuild ? run_norm(norm_backward_kernel<2, true, true>, g_norm_smem[7], grid, shape, 4, 3, P, st)
+         : mod   ? run_norm(norm_backward_kernel<2, true, false>, g_norm_smem[5], grid, shape, 4, 3, P, st)
+                 : run_norm(norm_backward_kernel<2, false, false>, g_norm_smem[3], grid, shape, 3, 1, P, st);
   if (rc != kSuccess) return rc;
   FGA_LAUNCHED();
   const int blocks = static_cast<int>(ceil_div(P.hidden, 128));

@@ -404,7 +404,10 @@ class _ResidualNorm(torch.autograd.Function):
         mean = torch.empty_like(rstd) if center else None
         y, r = _normalise(x, branch, weight, gate, scale, shift, cu_seqlens, samples, eps, center, rstd, mean)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(r, branch if gate is not None else None, weight, gate, scale, cu_seqlens, rstd, mean)
+        # r as it is returned has been rounded, which a centred norm may not bear; a gate keeps the branch anyway
+        ctx.rebuild = branch is not None and (gate is not None or center)
+        kept = (x, branch) if ctx.rebuild else (r, None)
+        ctx.save_for_backward(*kept, weight, gate, scale, cu_seqlens, rstd, mean)
         ctx.owner, ctx.has_branch, ctx.has_shift = weight, branch is not None, shift is not None
         ctx.rule = (samples, eps, center)
         return y, r
@@ -412,15 +415,15 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dr):
-        r, branch, weight, gate, scale, cu_seqlens, rstd, mean = ctx.saved_tensors
+        base, branch, weight, gate, scale, cu_seqlens, rstd, mean = ctx.saved_tensors
         samples, eps, center = ctx.rule
-        tokens, hidden = r.shape
+        tokens, hidden = base.shape
         needs = ctx.needs_input_grad
-        dy, dr = (None if g is None else _grad_rows(g, r.shape) for g in (dy, dr))
-        dx = torch.empty_like(r)
-        dbranch = torch.empty_like(r) if gate is not None else None
+        dy, dr = (None if g is None else _grad_rows(g, base.shape) for g in (dy, dr))
+        dx = torch.empty_like(base)
+        dbranch = torch.empty_like(base) if gate is not None else None
         target, accumulate = _weight_target(ctx.owner, needs[2])
-        rows = [torch.empty((samples, hidden), device=r.device, dtype=r.dtype) if present and needed else None
+        rows = [torch.empty((samples, hidden), device=base.device, dtype=base.dtype) if present and needed else None
                 for present, needed in ((gate is not None, needs[3]), (scale is not None, needs[4]),
                                         (ctx.has_shift, needs[5]))]
         if tokens:
@@ -428,14 +431,15 @@ class _ResidualNorm(torch.autograd.Function):
             modulated = any(t is not None for t in rows)
             scratch = None
             if target is not None or modulated:
-                scratch = _floats(lib.fga_norm_scratch_floats, r.device, tokens, hidden, samples, target is not None,
+                scratch = _floats(lib.fga_norm_scratch_floats, base.device, tokens, hidden, samples, target is not None,
                                   modulated)
+            x, r = (base.data_ptr(), 0) if ctx.rebuild else (0, base.data_ptr())
             args = _native.NORM_BYTES.pack(
-                0, _address(branch), _address(weight), _address(gate), _address(scale), 0, _address(cu_seqlens), 0,
-                r.data_ptr(), rstd.data_ptr(), _address(mean), _address(dy), _address(dr), dx.data_ptr(), _address(dbranch),
+                x, _address(branch), _address(weight), _address(gate), _address(scale), 0, _address(cu_seqlens), 0, r,
+                rstd.data_ptr(), _address(mean), _address(dy), _address(dr), dx.data_ptr(), _address(dbranch),
                 _address(target), *(_address(t) for t in rows), _address(scratch), tokens, hidden, samples, center,
                 target is not None and target.dtype is torch.float32, accumulate, eps)
-            _launch(lib.fga_norm_backward, args, r.device)
+            _launch(lib.fga_norm_backward, args, base.device)
         else:
             for t in (*rows, None if accumulate else target):
                 if t is not None:
@@ -449,7 +453,8 @@ def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=N
                   center=False):
     """The step between two blocks: r = x + gate * branch, y = norm(r) * weight * (1 + scale) + shift, in
     one pass. Returns (y, r); without a branch r is x. All BF16; sums and statistics in FP32, y computed
-    from the unrounded r.
+    from the unrounded r. The backward pass computes r again from x and the branch, which it keeps, where there is a
+    gate or a centred norm; an RMS norm without a gate keeps r as it is returned, rounded to BF16.
 
     x, branch: contiguous [tokens, hidden], hidden a multiple of 8 up to 8192, at most 2^31 - 2^16 tokens.
     The norm divides by the root mean square of the row, after subtracting its mean with `center` (a layer

@@ -339,7 +339,7 @@ def test_one_head_norm_weight_for_queries_and_keys(native):
         assert torch.equal(tied.main_grad, want)
 
 
-def norm_bounds(t, cu, center, dy, dr, has_branch):
+def norm_bounds(t, cu, center, dy, dr, has_branch, rounded=True):
     """Expected values and error bounds of y, r and every gradient, in 64 bits."""
     names = ('x', 'branch', 'weight', 'gate', 'scale', 'shift')
     leaves = {n: None if t[n] is None else t[n].double().requires_grad_() for n in names}
@@ -359,7 +359,7 @@ def norm_bounds(t, cu, center, dy, dr, has_branch):
     c = r - r.mean(-1, keepdim=True) if center else r
     rstd = 1 / (c.square().mean(-1, keepdim=True) + 1e-6).sqrt()
     n = c * rstd
-    stored = HALF * r.abs() * rstd if has_branch else 0 * r           # error of n from the stored residual sum
+    stored = HALF * r.abs() * rstd if has_branch and rounded else 0 * r    # error of n from the stored residual sum
     stored = stored + FINE * (r.abs() + r.abs().mean(-1, keepdim=True)) * rstd
     bounds = {'y': HALF * y.abs() + FINE * ((r.abs() + r.abs().mean(-1, keepdim=True)) * rstd * w.abs() * gain.abs()
                                             + n.abs() * w.abs() * gain.abs() + row['shift'].abs() * (t['shift'] is not None)),
@@ -432,6 +432,37 @@ def test_norm_matches_the_plain_form(native, lengths, pad, hidden, parts, center
     within(r.detach(), want_r, bounds['r'], 'r')
     for name in present:
         within(got[name], grads[name], bounds[name], f'gradient of {name}')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('parts', ['branch', 'branch+weight', 'gate', 'all', 'scale'])
+@pytest.mark.parametrize('hidden', [512, 4096])
+@pytest.mark.parametrize('center', [False, True])
+def test_norm_gradients_of_rows_far_from_zero(native, parts, hidden, center):
+    """Rows whose mean is many deviations from zero: a residual sum that has been rounded to BF16 would leave little of
+    what a centred norm makes of it. Bounds without that rounding; an RMS norm with a gate has none either."""
+    if not center and parts not in ('gate', 'all'):
+        pytest.skip('reads the rounded residual sum')
+    _, norm = ops()
+    gen = torch.Generator(device='cuda').manual_seed(hidden)
+    lengths, pad = [70, 0, 1, 40], 5
+    tokens, cu = sum(lengths) + pad, [0, 70, 70, 71, 111]
+    t = dict(x=normal(gen, tokens, hidden, mean=40.0), branch=normal(gen, tokens, hidden), weight=None, gate=None, scale=None,
+             shift=None)
+    if parts in ('branch+weight', 'all'):
+        t['weight'] = normal(gen, hidden, std=0.2, mean=1.0)
+    for name, uses in (('gate', ('gate', 'all')), ('scale', ('scale', 'all')), ('shift', ('all',))):
+        if parts in uses:
+            t[name] = normal(gen, 4, hidden, std=0.5)
+    dy, dr = normal(gen, tokens, hidden), normal(gen, tokens, hidden)
+    leaves = {n: None if v is None else v.detach().requires_grad_() for n, v in t.items()}
+    outs = norm(leaves['x'], leaves['branch'], **{n: leaves[n] for n in ('weight', 'gate', 'scale', 'shift')},
+                cu_seqlens=torch.tensor(cu, dtype=torch.int32, device='cuda'), center=center)
+    present = [n for n in leaves if leaves[n] is not None]
+    got = torch.autograd.grad(outs, [leaves[n] for n in present], (dy, dr))
+    _, _, grads, bounds = norm_bounds(t, cu, center, dy, dr, True, rounded=False)
+    for name, value in zip(present, got):
+        within(value, grads[name], bounds[name], f'gradient of {name}')
 
 
 @pytest.mark.gpu
