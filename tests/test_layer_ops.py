@@ -143,6 +143,40 @@ def test_the_c_entries_refuse_what_the_kernels_cannot_do(native):
         assert native.fga_rotary_forward(ctypes.byref(broken), None) == -1 and message in native.fga_last_error()
 
 
+def test_the_norm_takes_a_branch_gradient_exactly_where_there_is_a_gate(native):
+    import ctypes
+
+    import _fga_native as api
+    for gate, dbranch in ((16, None), (None, 16)):
+        norm = api.FgaNorm(16, 16, tokens=4, hidden=64, samples=1, gate=gate, dbranch=dbranch, dx=16, rstd=16)
+        assert native.fga_norm_backward(ctypes.byref(norm), None) == -1 and b'dbranch' in native.fga_last_error()
+
+
+@pytest.mark.gpu
+def test_the_c_entry_takes_the_stored_residual_sum_too(native):
+    """backward with r and, for a gate, the branch, as a caller that keeps no x has them."""
+    import _fga_native as api
+    gen = torch.Generator(device='cuda').manual_seed(21)
+    tokens, hidden = 50, 512
+    t = dict(x=normal(gen, tokens, hidden), branch=normal(gen, tokens, hidden), weight=None,
+             gate=normal(gen, 1, hidden), scale=None, shift=None)
+    dy, dr = normal(gen, tokens, hidden), normal(gen, tokens, hidden)
+    y, r, dx, dbranch = (torch.empty_like(dy) for _ in range(4))
+    dgate, rstd = torch.empty_like(t['gate']), torch.empty(tokens, device='cuda')
+    scratch = torch.empty(native.fga_norm_scratch_floats(tokens, hidden, 1, 0, 1), device='cuda')
+    stream = torch.cuda.current_stream().cuda_stream
+    gate, branch = t['gate'].data_ptr(), t['branch'].data_ptr()
+    assert native.fga_norm_forward(api.NORM_BYTES.pack(
+        t['x'].data_ptr(), branch, 0, gate, 0, 0, 0, y.data_ptr(), r.data_ptr(), rstd.data_ptr(), *(0,) * 10,
+        tokens, hidden, 1, 0, 0, 0, 1e-6), stream) == 0
+    assert native.fga_norm_backward(api.NORM_BYTES.pack(
+        0, branch, 0, gate, 0, 0, 0, 0, r.data_ptr(), rstd.data_ptr(), 0, dy.data_ptr(), dr.data_ptr(), dx.data_ptr(),
+        dbranch.data_ptr(), 0, dgate.data_ptr(), 0, 0, scratch.data_ptr(), tokens, hidden, 1, 0, 0, 0, 1e-6), stream) == 0
+    _, _, grads, bounds = norm_bounds(t, [0, tokens], False, dy, dr, True)
+    for name, value in (('x', dx), ('branch', dbranch), ('gate', dgate)):
+        within(value, grads[name], bounds[name], name)
+
+
 @pytest.mark.parametrize('tokens', [(1 << 31) - 1, (1 << 31) - (1 << 16) + 1])
 def test_norm_rows_leave_room_for_32_bit_sums(native, tokens):
     import ctypes

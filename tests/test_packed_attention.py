@@ -285,6 +285,61 @@ def test_gradients_match_the_plain_form(native, lengths, pad, heads, kv_heads, c
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('tokens,heads,kv_heads', [(4200, 1, 1), (4200, 2, 1), (2500, 3, 1)])
+def test_blocks_of_a_cluster_without_a_query(native, tokens, heads, kv_heads):
+    """Four blocks share a key/value tile; the last tiles of a causal sequence have fewer query tiles than that."""
+    gen = torch.Generator(device='cuda').manual_seed(tokens + heads)
+    q, k, v = normal(gen, tokens, heads, 128, std=1.5), normal(gen, tokens, kv_heads, 128), normal(gen, tokens, kv_heads, 128)
+    do = normal(gen, tokens, heads, 128)
+    o, eo, _, grads = expected(q, k, v, None, True, do=do)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = attention(*leaves, causal=True)
+    within(got.detach(), o, eo + 1e-30, 'o')
+    for name, g in zip('qkv', torch.autograd.grad(got, leaves, do)):
+        within(g, grads[name][0], grads[name][1] + 1e-30, 'd' + name)
+
+
+def expected_in_pieces(q, k, v, do, causal, rows=2048):
+    """o and the gradients of one sequence and one key/value head in 64 bits, some queries at a time."""
+    tokens, heads, dim = q.shape
+    kk, vv = k[:, 0].double(), v[:, 0].double()
+    o, dq = (torch.zeros(q.shape, dtype=torch.float64, device=q.device) for _ in range(2))
+    dk, dv = torch.zeros_like(kk), torch.zeros_like(vv)
+    at = torch.arange(tokens, device=q.device)
+    for h in range(heads):
+        for a in range(0, tokens, rows):
+            qq, d = q[a:a + rows, h].double(), do[a:a + rows, h].double()
+            p = qq @ kk.T * dim ** -0.5
+            if causal:
+                p.masked_fill_(at > at[a:a + rows, None], -math.inf)
+            p = p.softmax(-1)
+            o[a:a + rows, h] = p @ vv
+            dv += p.T @ d
+            p *= d @ vv.T - (d * o[a:a + rows, h]).sum(-1, keepdim=True)
+            dq[a:a + rows, h] = p @ kk * dim ** -0.5
+            dk += p.T @ qq * dim ** -0.5
+    return o, dq, dk[:, None], dv[:, None]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('tokens', [16383, 131072])
+def test_long_sequences(native, tokens, causal):
+    """Thousands of keys make every element a small sum of many terms, to which the bounds above (the sum of the terms'
+    sizes) say little. The terms' roundings are independent and the sum grows with their root as they do, so the error
+    of any 128 rows is the chain of four roundings beside their norm; a missing key tile would be 3 % at 131072."""
+    gen = torch.Generator(device='cuda').manual_seed(tokens)
+    q, k, v, do = (normal(gen, tokens, h, 128) for h in (2, 1, 1, 2))
+    want = expected_in_pieces(q, k, v, do, causal)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = attention(*leaves, causal=causal)
+    for name, a, b in zip(('o', 'dq', 'dk', 'dv'), (o.detach(), *torch.autograd.grad(o, leaves, do)), want):
+        for first in range(0, tokens, 128):
+            error = (a[first:first + 128].double() - b[first:first + 128]).norm() / b[first:first + 128].norm()
+            assert error <= 4 * HALF, (name, first, error.item())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('scale,std', [(1.0, 0.5), (0.02, 4.0), (0.3, 3.0)])
 def test_other_scales_and_peaked_rows(native, scale, std):
     """Scores that reach the hundreds: the running maximum moves, and most probabilities vanish."""
@@ -505,6 +560,59 @@ def test_an_error_reaches_the_next_call_without_a_synchronizing_one(native, call
             fused_gemm_a2a.check_status(clear=True)
     assert torch.equal(attention(q, q, q), q)
     fused_gemm_a2a.check_status()
+
+
+@pytest.mark.gpu
+def test_a_capture_that_is_the_first_to_ask_for_the_hosts_copy(native):
+    """The device's word may be there without it, made by another operator; pinned memory cannot be had in a capture."""
+    import fused_gemm_a2a_kernels as kernels
+    q = torch.ones(4, 1, 128, dtype=torch.bfloat16, device='cuda')
+    attention(q, q, q)
+    copy = kernels._local_host_status.pop(q.device)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = attention(q, q, q)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, q) and not kernels._local_host_status
+    finally:
+        kernels._local_host_status[q.device] = copy
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once(native):
+    """Forward and backward of two sizes, each thread on its own stream: the same bits as alone."""
+    import threading
+    gen = torch.Generator(device='cuda').manual_seed(20)
+    sizes = ((700, 4, 2), (130, 8, 1))
+    inputs = [[normal(gen, n, h, 128) for h in (heads, kv, kv, heads)] for n, heads, kv in sizes]
+
+    def step(q, k, v, do):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        o = attention(*leaves, causal=True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    want, failures, start = [step(*t) for t in inputs], [], threading.Barrier(2)
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(50):
+                    got = step(*inputs[i])
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+        except Exception as error:                                                  # noqa: BLE001
+            failures.append(repr(error))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
 
 
 @pytest.mark.gpu
