@@ -2,7 +2,8 @@
 // sequence and head, optionally causal, with shared key/value heads; forward and backward, BF16 operands,
 // FP32 accumulation and statistics. Head dimension 128.
 //
-// Common to the kernels: one block per SM works alone (no cluster). Operand tiles are 128 rows x 128
+// Common to the kernels: one block per SM, which works alone except in the dK/dV kernel, where a cluster of two
+// or four may share a tile. Operand tiles are 128 rows x 128
 // columns, 32 KiB in two 64-column halves with the 128-byte swizzle, TMA-loaded from a 3-D map [tokens,
 // heads, 128], so any row may start a tile and rows behind the tensor read as zero. The same tile serves as
 // K-major operand (reduction over its columns) and as MN-major one (reduction over its rows): only the
@@ -99,7 +100,9 @@ __device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a_tmem, uint32
 }
 
 // Work tile `t` of `rows` rows: tiles are numbered sequence by sequence, the rows behind the last
-// sequence last. Executed by whole warps.
+// sequence last. Executed by whole warps. Every block walks over the offsets, 32 a step, and every sequence has
+// blocks of its own however short it is: packs of a thousand sequences cost more for that than for their
+// products (16 tokens each, 8 heads, forward: 100 sequences 40 us, 1000 575 us, 5000 7.7 ms).
 struct WorkTile {
   int first, len;  // rows of the sequence
   int row0;        // first row of the tile within the sequence
@@ -299,8 +302,11 @@ __device__ __forceinline__ bool begin(const AttentionParams& P, const CUtensorMa
 // the next S (640) and the latencies of two hand-overs; both tiles run that chain half a period apart. An
 // issuing warp for each tile (263 against 247 us for the packed prompts below), key tiles of 64 with two score
 // buffers per query tile (271 us), one hand-over instead of two (the same) and a polynomial in place of a
-// quarter of the exponentials (258 us) do not shorten it. 16383 tokens x 8 heads: 1.0 ms, 1.1 PFLOP/s at the 1.6 GHz that the
-// power limit leaves; 8192 tokens of packed causal prompts, 32 heads on 8: 240 us, 0.84 PFLOP/s.
+// quarter of the exponentials (258 us) do not shorten it. 16383 tokens x 8 heads: 0.94 ms in a few calls, 1.07 ms
+// (1.03 PFLOP/s) at the 1.6 GHz that the power limit leaves in longer runs; its 512 blocks are 3.46 rounds of 148
+// SMs and take the time of 4. 8192 tokens of packed causal prompts, 32 heads on 8: 225 to 248 us, 0.81 to 0.90
+// PFLOP/s. Nothing splits the keys of a block, so few heads on a long sequence leave SMs idle (4097 causal tokens:
+// 65 us for 1 head as for 4; 8191: 118 us).
 // =============================================================================================
 constexpr int kFwdThreads = 384;
 constexpr uint32_t kFwdStageBytes = 2 * kTileBytes;  // V(j) and K(j + 1): the operands of one iteration
@@ -566,8 +572,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // write their halves of P or dS as BF16 over their own halves of the scores, 64 columns apart. (Four
 // warpgroups of 32 columns each were 3 % slower.)
 //
-// 16383 tokens x 8 heads: 1.2 ms for dQ (2070 cycles per tile, 1536 of products) and 1.6 ms for dK and dV
-// (2790, 2048 of products), together 1.4 PFLOP/s of tensor work under the power limit.
+// 16383 tokens x 8 heads: 1.15 ms for dQ (2070 cycles per tile, 1536 of products) and 1.56 ms for dK and dV
+// (2790, 2048 of products) in a few calls, together 1.42 PFLOP/s of tensor work; 1.26 and 1.70 ms, 1.30 PFLOP/s,
+// under the power limit of longer runs. The dK/dV kernel spills 8 bytes a thread at its 168 registers.
 // =============================================================================================
 constexpr int kBwdThreads = 384;
 

@@ -62,9 +62,10 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
 // cosines once for all heads. Eight lanes hold a head row, each 8 elements of its lower and 8 of its upper
 // half, so both kinds of pairs turn inside a lane; a warp takes four head rows at a time. The first version
 // (16 lanes a row, scalar arithmetic) issued 870 instructions per token of 8 heads and was bound by that, at
-// 3.7 TB/s. Now 131072 tokens x (4 + 4) heads with head norms take 99 us forward (5.4 TB/s) and 158 us
-// backward (5.1 TB/s; its registers hold it to 16 warps an SM), 16384 x (32 + 8) without norms 54 us
-// (6.2 TB/s, where a plain copy measures 6.55).
+// 3.7 TB/s. Now 131072 tokens x (4 + 4) heads with head norms take 101 us forward (5.3 TB/s) and 162 us
+// backward (5.0 TB/s; its registers hold it to 16 warps an SM), 16384 x (32 + 8) without norms 55 us
+// (6.1 TB/s, where a plain copy measures 6.55). At the 80 registers of three blocks an SM the forward kernels with
+// norms spill 32 and 44 bytes a thread.
 // =============================================================================================
 constexpr int kRotaryWarps = 8;
 
@@ -407,15 +408,16 @@ __global__ void __launch_bounds__(512) finish_sums_kernel(const __grid_constant_
 // y = n * weight * (1 + scale) + shift.  gate, scale and shift are one row per packed sample.
 //
 // A block takes a chunk of consecutive rows, a thread the same 8 * kVec columns of each, so weight,
-// scale, shift and gate stay on the SM from row to row (forward in registers, backward in shared memory: see
-// norm_smem()) and the column sums of the backward pass are
-// register sums over the chunk. Slot chunk + sample of the partial sums is unique: walking down the rows
+// scale, shift and gate stay on the SM from row to row (forward in registers; backward in shared memory, because
+// the column sums, register sums over the chunk, leave no registers for them: 156 -> 134 us at 16384 x 4096
+// with gate, scale and shift). Slot chunk + sample of the partial sums is unique: walking down the rows
 // either of the two grows. The next rows are on their way to shared memory meanwhile, each thread fetching
 // what it will read itself, so a row costs one barrier (two when centred) for its sums.
 //
 // Bound by memory: 8191 x 5120 with a residual sum 53 us (6.3 TB/s), 16384 x 4096 centred with gate, scale
-// and shift 90 us forward (6.0 TB/s) and 134 us backward (6.0 TB/s: six streams, 48 FP32 column sums a
-// thread).
+// and shift 89 us forward (6.0 TB/s) and 132 to 135 us backward (6.0 TB/s: six streams, 48 FP32 column sums a
+// thread). Narrow rows are bound by latency: norm_chunk_rows() counts on the same four blocks an SM for all widths up
+// to 1024, whose warps are then few (32768 rows backward: 71 us at 64 columns as at 512, 75 us at 1024).
 // =============================================================================================
 struct NormParams {
   const uint16_t *x, *branch, *weight, *gate, *scale, *shift;
@@ -463,7 +465,7 @@ __device__ __forceinline__ RowRange range_of(const NormParams& P, int row) {
   return s;
 }
 
-constexpr int kRowsAhead = 2;  // rows in flight: more (3 or 4) cost up to a fifth, see norm_smem()
+constexpr int kRowsAhead = 2;  // rows in flight: more (3 or 4) cost up to a fifth, their shared memory costs a block
 
 template <int kVec>
 __global__ void __launch_bounds__(256 * kVec) norm_forward_kernel(const NormParams P) {
@@ -807,8 +809,8 @@ __global__ void __launch_bounds__(256 * kVec) norm_backward_kernel(const NormPar
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Rows a norm block walks: the blocks that are resident at once (four on an SM up to 1024 columns, else
-// two) share the rows evenly; at least one row. A forward pass that has no per-sample rows to load takes a
+// Rows a norm block walks: as many blocks as are taken to be resident at once (four on an SM up to 1024 columns,
+// else two) share the rows evenly; at least one row. A forward pass that has no per-sample rows to load takes a
 // fourth of that, so that SMs which are ahead take more (8191 x 5120: 62.5 -> 55.2 us; with gate, scale and
 // shift loaded four times as often 16384 x 4096 went from 90 to 94 us). In the backward pass every block
 // leaves its sums behind.
@@ -820,7 +822,8 @@ struct NormShape {
   int vec, threads;
 };
 // 8 columns a thread up to 2048 columns, 16 above: a block of at most 256 threads for 2048 columns and
-// 512 for 8192 keeps two blocks on an SM beside the FP32 column sums.
+// 512 for 8192. The modulated backward kernels have 126 registers at 16 columns, so two blocks share an SM up to
+// 4096 columns; above, one does, and the grid of two an SM takes two rounds there.
 NormShape norm_shape(int hidden) {
   const int vecs = hidden / 8, vec = hidden <= 2048 ? 1 : 2;
   return {vec, static_cast<int>(ceil_div(ceil_div(vecs, vec), 32) * 32)};

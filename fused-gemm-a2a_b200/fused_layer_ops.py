@@ -256,15 +256,18 @@ def packed_attention(q, k, v, cu_seqlens=None, *, causal=False, scale=None, retu
     [heads, tokens] logarithms of the rows' sums of exponentials (-inf behind the last sequence; no gradient
     flows through them).
 
-    Range of the scores: the output holds its precision while a row's largest |scale * q k| is below 2^28, and
-    the row is NaN from 2^29 on. In the backward pass probabilities are off by about 2^-23 of the score: less than their
-    rounding to BF16 up to scores of 2^14, an eighth at 2^20; gradients of and through rows beyond that are NaN.
+    Range of the scores: the output holds its precision while a row's largest |scale * q k| is below 2^28,
+    and the row is NaN from 2^29 on. In the backward pass probabilities are off by about 2^-23 of the score:
+    less than their rounding to BF16 up to scores of 2^14, an eighth at 2^20; gradients of and through rows
+    beyond that are NaN.
 
     Scores, softmax statistics and all sums are FP32; the probabilities (and in the backward pass the
-    gradients of the scores) are rounded to BF16 for the second product. Results, gradients included, are
-    the same bits in every run. Kernel waits are bounded as in the projections. One that expires is recorded in the
-    device's status word, which check_status() and a group's comm.check_status() read, and raised by the first
-    later call, forward or backward, that finds it in host memory."""
+    gradients of the scores) are rounded to BF16 for the second product. The backward pass takes the row
+    sums of do * o from o as it was returned, rounded to BF16, for rows that may see more than 128 keys.
+    Results, gradients included, are the same bits in every run. Kernel waits are bounded as in the
+    projections. One that expires is recorded in the device's status word, which check_status() and a
+    group's comm.check_status() read, and raised by the first later call, forward or backward, that finds it
+    in host memory."""
     for t, label in ((q, 'q'), (k, 'k'), (v, 'v')):
         _head_tensor(t, label)
     if k.shape != v.shape or k.shape[0] != q.shape[0]:
@@ -453,15 +456,15 @@ def residual_norm(x, branch=None, *, weight=None, gate=None, scale=None, shift=N
                   center=False):
     """The step between two blocks: r = x + gate * branch, y = norm(r) * weight * (1 + scale) + shift, in
     one pass. Returns (y, r); without a branch r is x. All BF16; sums and statistics in FP32, y computed
-    from the unrounded r. The backward pass computes r again from x and the branch, which it keeps, where there is a
-    gate or a centred norm; an RMS norm without a gate keeps r as it is returned, rounded to BF16.
+    from the unrounded r. Where there is a gate or a centred norm, the backward pass computes r again from x
+    and the branch, which it keeps; for an RMS norm without a gate it keeps r as it is returned, rounded.
 
     x, branch: contiguous [tokens, hidden], hidden a multiple of 8 up to 8192, at most 2^31 - 2^16 tokens.
     The norm divides by the root mean square of the row, after subtracting its mean with `center` (a layer
     norm). weight: [hidden]. gate, scale, shift: [samples, hidden], one row for each packed sequence of
-    cu_seqlens (one sample, or [hidden], without it). With cu_seqlens, rows behind the last sequence have a
-    gate of 0 and y = 0, and pass dr through to x in the backward pass. Gradients flow to everything but
-    cu_seqlens."""
+    cu_seqlens (one sample, or [hidden], without it). With cu_seqlens, rows behind the last sequence have
+    y = 0 and r = x, or x + branch where there is no gate, and pass dr through to what r is the sum of.
+    Gradients flow to everything but cu_seqlens."""
     if x.ndim != 2 or x.dtype != torch.bfloat16 or not x.is_contiguous() or x.data_ptr() % 16:
         raise ValueError('x must be a contiguous, 16-byte aligned BF16 tensor [tokens, hidden]')
     tokens, hidden = x.shape

@@ -278,11 +278,11 @@ int fga_rotary_backward(const FgaRotary* args, void* stream);
 /* Norm around a block: r = x + gate * branch (gate 1 where NULL; no r without a branch),
  * n = r * rsqrt(mean(r^2) + eps), or (r - mean) * rsqrt(var + eps) with center; y = n * weight * (1 +
  * scale) + shift. weight: [hidden]; gate, scale, shift: one row of [samples, hidden] for each packed
- * sequence. Rows behind the last sequence have a gate of 0 and y = 0: dx = dr. hidden: a multiple of 8
- * up to 8192; at most 2^31 - 2^16 tokens. backward computes r again from x and
- * branch where it gets both, which is exact; otherwise it reads r as the forward left it, rounded to BF16 (x where
- * there is no branch). A gate needs the branch in either case. It reads rstd and mean; dy and dr may be NULL.
- * dbranch belongs to a gate: the gradient of a branch without one is dx. scratch: fga_norm_scratch_floats() with
+ * sequence. Rows behind the last sequence have a gate of 0, where there is one, and y = 0: dx = dr.
+ * hidden: a multiple of 8 up to 8192; at most 2^31 - 2^16 tokens. backward computes r again from x and
+ * branch where it gets both, which is exact; otherwise it reads r as the forward left it, rounded to BF16
+ * (x where there is no branch). A gate needs the branch in either case. It reads rstd and mean; dy and dr
+ * may be NULL. dbranch belongs to a gate: the gradient of a branch without one is dx. scratch: fga_norm_scratch_floats() with
  * has_weight = (dweight != NULL) and modulated = (any of dgate, dscale, dshift). */
 typedef struct FgaNorm {
   const void *x, *branch, *weight, *gate, *scale, *shift;
