@@ -3,8 +3,9 @@ the 64-bit forms on the GPU.
 
 Tolerances. A BF16 output is off by at most half a step, 2^-8 of its value; FP32 arithmetic in front of it
 by a few 2^-24 of the terms it is made of, for which 2^-20 of the largest term is allowed (sixteen
-roundings). The backward pass of the norm reads the residual sum as the forward stored it, each element off
-by 2^-8 of its value; what that does to each gradient is carried through with absolute values below.
+roundings). The backward pass of an RMS norm without a gate reads the residual sum as the forward stored it, each
+element off by 2^-8 of its value; what that does to each gradient is carried through with absolute values below.
+Other norms compute the sum again and stay within these bounds by far; theirs without that rounding are tested apart.
 """
 import pytest
 import torch
